@@ -116,10 +116,10 @@ def work(c):
 
 # -- the plain forms -----------------------------------------------------------------------------------------------------
 def _quantise(x):
-    """Codes (e4m3) and scale bytes of rows [..., D]: the least power of two 2^e with max|x| <= 448 * 2^e per 32 values."""
+    """Codes (e4m3) and scale bytes of rows [..., D]: the least power of two 2^e, -50 <= e <= 64, with max|x| <= 448 * 2^e per 32 values."""
     b = x.float().unflatten(-1, (D // BLOCK, BLOCK))
     m, e = torch.frexp(b.abs().amax(-1, keepdim=True))
-    e = torch.where(m > 0, e - 9 + (m > 0.875), torch.full_like(e, -110)).clamp(-110, 119)
+    e = torch.where(m > 0, e - 9 + (m > 0.875), torch.full_like(e, -50)).clamp(-50, 64)
     codes = torch.ldexp(b, -e).clamp(-448, 448).to(torch.float8_e4m3fn)
     return codes.flatten(-2), (e + 127).to(torch.uint8).squeeze(-1)
 
@@ -303,7 +303,7 @@ def _exact_codes(x):
     most = blocks.abs().max(-1).values
     e = torch.ceil(torch.log2(most.clamp_min(2.0 ** -1000) / 448.0) - 1e-9)  # 1e-9: far below what bf16 tells apart
     e = e + (most > 448.0 * torch.exp2(e)).double()
-    e = torch.where(most > 0, e, torch.full_like(e, -110.0)).clamp(-110, 119)
+    e = torch.where(most > 0, e, torch.full_like(e, -50.0)).clamp(-50, 64)
     y = blocks / torch.exp2(e).unsqueeze(-1)
     grid = _e4m3_grid()
     # the value's own step: 2^-9 below 2^-6, else an eighth of its power of two; both sides of the tie are on the grid
