@@ -413,6 +413,76 @@ MB_API int mb_last_cuda_error(char* buf, int32_t len);
 /* Library version, major * 1000 + minor. */
 MB_API int mb_version(void);
 
+/* ---------------------------------------------------------------------------
+ * Keys and values in pages: a cache that is written as tokens arrive, read back
+ * into one packed buffer, and attended to by new tokens.  No counterpart in the
+ * reference, whose K/V are contiguous shards; the results merge with those of
+ * the block ops (o, lse), and what is read back is the packed kv that the ring
+ * schedules take.
+ *
+ * Sequence b holds seq_lens[b] keys, the new ones included.  Key j lies in slot
+ * j % page_size of page page_table[b][j / page_size].  Its new tokens are the
+ * rows [cu_seqlens[b], cu_seqlens[b + 1]) of the call's [tokens, heads, head_dim]
+ * tensors (cu_seqlens == NULL: rows [b * n, (b + 1) * n) with n = tokens / batch,
+ * stride_b apart per sequence), and the last of them is the sequence's last key.
+ * Lengths, offsets and page numbers are read on the device (a captured graph may be
+ * replayed with others).  One that lies outside the table, the pages or the
+ * rows does not leave them: it is clamped or skipped and reported as status 110,
+ * and the results of that call are invalid. */
+#define MB_DTYPE_E4M3 2
+
+typedef struct mb_paged_kv {
+  void* k; /* [pages, page_size, hkv, head_dim], 16-byte aligned; bf16 or e4m3 */
+  void* v;
+  int64_t stride_page, stride_slot, stride_h; /* elements, shared by k and v; multiples of 16 bytes */
+  /* e4m3: [pages, hkv, page_size, head_dim / 32] bytes, contiguous.  Byte x is the power of two
+   * 2^(x - 127) that 32 values along head_dim share (77..191 as written; from 192 on: not a number).  bf16: NULL. */
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  const int32_t* page_table; /* [batch, max_pages] */
+  int64_t page_table_stride; /* elements between sequences */
+  const int32_t* seq_lens;   /* [batch] */
+  const int32_t* cu_seqlens; /* [batch + 1], or NULL */
+  int32_t batch, tokens;     /* tokens: rows of the call's token tensors */
+  int32_t pages, page_size, max_pages, hkv, head_dim;
+  int32_t dtype; /* MB_DTYPE_BF16 or MB_DTYPE_E4M3 */
+  int32_t* status; /* device word for errors; NULL selects the library's own word */
+} mb_paged_kv;
+
+/* Stores the new tokens' keys and values [tokens, hkv, head_dim] (bf16) in their pages; e4m3: a block of 32
+ * values takes the least power of two 2^e, -50 <= e <= 64, with max|x| <= 448 * 2^e, and its values x * 2^-e are
+ * rounded to the nearest e4m3 (beyond 448: 448).  A block with an infinity or a NaN gets scale byte 255, and all
+ * of its values read as NaN.  New tokens that lie before the first key (more of them than keys) are not stored. */
+MB_API int mb_kv_cache_write(const mb_paged_kv* kv, const void* k_new, const void* v_new, int64_t stride_b,
+                             int64_t stride_t, int64_t stride_h, void* cuda_stream);
+
+/* The first min(seq_lens[b], rows) keys and values of every sequence, in bf16, into k_out and v_out [batch, rows,
+ * hkv, head_dim]; the rows behind a sequence's last key are left as they are.  A code times its power of two is
+ * exact in bf16.  cu_seqlens and tokens are not used. */
+MB_API int mb_kv_cache_read(const mb_paged_kv* kv, void* k_out, void* v_out, int64_t stride_b, int64_t stride_s,
+                            int64_t stride_h, int32_t rows, void* cuda_stream);
+
+typedef struct mb_attn_paged_args {
+  mb_paged_kv kv;
+  const void* q; /* [tokens, hq, head_dim] bf16, 16-byte aligned rows */
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+  void* o; /* like q, written */
+  int64_t o_stride_b, o_stride_t, o_stride_h;
+  float* lse; /* written: cu_seqlens: [hq, tokens]; else [batch, hq, tokens / batch] */
+  int64_t lse_stride_b, lse_stride_h;
+  int32_t hq;
+  int32_t max_queries; /* no sequence has more new tokens */
+  int32_t max_keys;    /* no sequence has more keys */
+  int32_t causal;      /* new token i of n sees keys j <= seq_lens - n + i; else all keys */
+  float softmax_scale; /* > 0 */
+} mb_attn_paged_args;
+
+/* Attention of every sequence's new tokens over its cached keys.  Rows without a visible key get o = 0, lse = -inf;
+ * rows behind the last sequence are left as they are.  The workspace (16-byte aligned, contents arbitrary, at least
+ * mb_attn_paged_workspace bytes, which is 0 for bad arguments) belongs to the call until its work on the stream is done. */
+MB_API int64_t mb_attn_paged_workspace(const mb_attn_paged_args* args);
+MB_API int mb_attn_paged(const mb_attn_paged_args* args, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,3 +6,4 @@ from .integration import (install_backend, install_search_hooks, load_generated,
                           remove_search_hooks)
 from .ops import (_flash_attn_backward, _flash_attn_forward, flash_reduce, get_default_args,  # noqa: F401
                   update_out_and_lse)
+from .paged import PagedKV, attn_fwd_paged, kv_cache_read, kv_cache_write  # noqa: F401

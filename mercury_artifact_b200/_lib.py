@@ -34,7 +34,14 @@ STATUS_NAMES = {
     107: "staged shard chunk never became ready",
     108: "unspecified wait",
     109: "a K/V shard's arrival flag never reached its value (in-kernel wait)",
+    110: "a page number, sequence length or row offset lies outside the cache or the tensors",
 }
+
+
+def _status_text(code: int, timeout: str) -> str:
+    """What happened, for the message of an exception: `timeout`, unless the code is that of a failed check."""
+    kind = "a device-side check failed" if code >= 110 else timeout
+    return f"{kind}: {STATUS_NAMES.get(code, code)} (code {code})"
 
 
 class KVSegment(C.Structure):
@@ -152,6 +159,7 @@ class PullArgs(C.Structure):
 
 MB_DTYPE_BF16 = 0
 MB_DTYPE_F32 = 1
+MB_DTYPE_E4M3 = 2
 
 
 class MergeArgs(C.Structure):
@@ -300,7 +308,55 @@ class MercuryB200Error(RuntimeError):
 
 
 # entry points that return something other than an MB_* code
-_RESTYPES = {"mb_attn_fwd_workspace": C.c_int64}
+_RESTYPES = {"mb_attn_fwd_workspace": C.c_int64, "mb_attn_paged_workspace": C.c_int64}
+
+
+class PagedKVArgs(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("stride_page", C.c_int64),
+        ("stride_slot", C.c_int64),
+        ("stride_h", C.c_int64),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("page_table", C.c_void_p),
+        ("page_table_stride", C.c_int64),
+        ("seq_lens", C.c_void_p),
+        ("cu_seqlens", C.c_void_p),
+        ("batch", C.c_int32),
+        ("tokens", C.c_int32),
+        ("pages", C.c_int32),
+        ("page_size", C.c_int32),
+        ("max_pages", C.c_int32),
+        ("hkv", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("dtype", C.c_int32),
+        ("status", C.c_void_p),
+    ]
+
+
+class AttnPagedArgs(C.Structure):
+    _fields_ = [
+        ("kv", PagedKVArgs),
+        ("q", C.c_void_p),
+        ("q_stride_b", C.c_int64),
+        ("q_stride_t", C.c_int64),
+        ("q_stride_h", C.c_int64),
+        ("o", C.c_void_p),
+        ("o_stride_b", C.c_int64),
+        ("o_stride_t", C.c_int64),
+        ("o_stride_h", C.c_int64),
+        ("lse", C.c_void_p),
+        ("lse_stride_b", C.c_int64),
+        ("lse_stride_h", C.c_int64),
+        ("hq", C.c_int32),
+        ("max_queries", C.c_int32),
+        ("max_keys", C.c_int32),
+        ("causal", C.c_int32),
+        ("softmax_scale", C.c_float),
+    ]
+
 
 _SIGNATURES = {
     "mb_version": [],
@@ -335,6 +391,11 @@ _SIGNATURES = {
     "mb_status_peek_async": [C.c_void_p, C.c_void_p],
     "mb_status_fetch": [C.POINTER(C.c_int32), C.c_void_p],
     "mb_last_cuda_error": [C.c_char_p, C.c_int32],
+    "mb_kv_cache_write": [C.POINTER(PagedKVArgs), C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p],
+    "mb_kv_cache_read": [C.POINTER(PagedKVArgs), C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int32,
+                         C.c_void_p],
+    "mb_attn_paged_workspace": [C.POINTER(AttnPagedArgs)],
+    "mb_attn_paged": [C.POINTER(AttnPagedArgs), C.c_void_p, C.c_uint64, C.c_void_p],
 }
 
 
@@ -462,11 +523,11 @@ class StatusMonitor:
         if bad:
             status_fetch(self._torch.cuda.current_stream().cuda_stream)   # synchronise and clear the device word
             raise MercuryB200Error(
-                f"a device-side wait of an earlier call timed out: {STATUS_NAMES.get(bad, bad)} (code {bad}); "
+                f"{_status_text(bad, 'a device-side wait of an earlier call timed out')}; "
                 "the results of that call are invalid")
 
 
 def raise_on_status(stream_ptr: int) -> None:
     st = status_fetch(stream_ptr)
     if st != 0:
-        raise MercuryB200Error(f"device-side timeout: {STATUS_NAMES.get(st, st)} (code {st})")
+        raise MercuryB200Error(_status_text(st, "device-side timeout"))

@@ -1,0 +1,33 @@
+// Arguments shared by the two attention kernels over pages and their host side.
+#pragma once
+
+#include "paged_common.cuh"
+
+namespace mb {
+
+struct PagedAttnArgs {
+  PagedView c;
+  const __nv_bfloat16* q;
+  long long q_sb, q_st, q_sh;  // element strides: sequence (0 with offsets), token, head
+  __nv_bfloat16* o;
+  long long o_sb, o_st, o_sh;
+  float* lse;
+  long long lse_sb, lse_sh;
+  int hq, group, max_queries, max_keys, causal;
+  float scale, scale_log2;  // of the raw scores that the products give (the bias of e4m3 values taken out)
+  float out_scale;          // of the raw sums of values
+  // rows of a sequence: new tokens x heads of a group.  Sequences with at most `few` rows belong to the kernel for
+  // few rows, the others to the kernel for tiles.
+  int few;
+  // partial results: [slot][row][128] and (maximum, sum) [slot][row]; open: the unit that a CTA began and left to the
+  // next ones (sequence, K/V head, number of CTAs; 0: none)
+  float* part_o;
+  float2* part_ml;
+  int4* open;
+};
+
+int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream);
+long long paged_rows_workspace(int rows, int ctas);
+int paged_rows_ctas();
+
+}  // namespace mb

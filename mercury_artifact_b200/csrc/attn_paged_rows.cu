@@ -1,0 +1,702 @@
+// Attention of few rows over keys and values in pages: single new tokens, drafted tokens.
+//
+// The rows of a unit are the new tokens of one sequence times the query heads of one K/V head (row = token * group +
+// head); at most 32 of them, so that a key and a value are used 64 times at most between their load and their end:
+// the kernel is bound by the bytes of the cache, and everything else has to stay out of the way of the loads.
+//
+// One CTA per SM, eight warps, no roles: a warp loads its own keys and values with cp.async into its own three stages
+// (16-byte pieces; rows behind the sequence's end are filled with zeros and never read, so that what lies in
+// unwritten slots does not matter) and multiplies them with mma.sync, 16 rows x 16 keys x 128.  With so few rows the
+// matrix instructions take a twentieth of the time the loads take, and registers are where the operands should be:
+// tcgen05 would take scores and probabilities through tensor memory and a hand-over between roles for every 128 keys.
+// Only the end of a unit needs the other warps: their states are merged in shared memory.
+//
+// The work of a launch is a list of steps (128 keys of one sequence and K/V head in bf16, 256 in e4m3), sequence by sequence, head by head;
+// every CTA takes an equal, contiguous part.  The lengths are on the device, so that every CTA finds its part
+// itself (one load per sequence and a scan).  A unit that lies in several CTAs leaves a partial state in each, and
+// paged_merge_kernel joins them in order: results do not depend on timing.
+#include "attn_paged.cuh"
+
+namespace mb {
+
+constexpr int kRowWarps = 8;
+constexpr int kRowThreads = 32 * kRowWarps;
+constexpr int kRowStages = 3;
+
+template <bool kFp8>
+struct RowShape {
+  static constexpr int kKeys = kFp8 ? 32 : 16;                     // keys of a warp's stage
+  static constexpr int kRowBytes = kFp8 ? kHeadDim : 2 * kHeadDim;
+  static constexpr int kPieces = kRowBytes / 16;
+  static constexpr int kHalf = kKeys * kRowBytes;                  // K or V of a stage: 4 KiB
+  static constexpr int kScaleBytes = kFp8 ? kKeys * kScalesPerRow : 0;
+  static constexpr int kStage = 2 * kHalf + 2 * kScaleBytes;
+  static constexpr int kStep = kKeys * kRowWarps;                  // keys of a CTA's step
+  // pitch of the merge buffer, in floats: what the lanes of a warp store together falls into different banks
+  static constexpr int kPitch = kFp8 ? 144 : 136;
+};
+
+struct RowSmem {
+  int total, warp_sum[kRowWarps];
+  int b, step;                               // where this CTA's part starts: sequence, and step inside it
+  float2 ml[kRowWarps][32];
+};
+
+template <bool kFp8>
+constexpr int row_smem_bytes() {
+  // merge buffers: two of 16 rows or one of 32
+  return kRowWarps * kRowStages * RowShape<kFp8>::kStage + 32 * 2 * kHeadDim + 32 * RowShape<kFp8>::kPitch * 4 + (int)sizeof(RowSmem);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A place in the list of steps.
+struct RowIter {
+  int b, h, step, steps;  // steps: of the unit
+  PagedSeq s;
+};
+
+template <int kStep>
+__device__ __forceinline__ int unit_steps(const PagedAttnArgs& a, const PagedSeq& s) {
+  return s.n > 0 && s.n * a.group <= a.few ? (s.len + kStep - 1) / kStep : 0;
+}
+template <int kStep>
+__device__ __forceinline__ void next_sequence(const PagedAttnArgs& a, RowIter& it) {
+  it.steps = 0;
+  while (it.b < a.c.batch) {
+    it.s = paged_seq(a.c, it.b, a.max_queries, a.max_keys);
+    it.steps = unit_steps<kStep>(a, it.s);
+    if (it.steps > 0) return;
+    ++it.b;
+  }
+}
+template <int kStep>
+__device__ __forceinline__ void next_step(const PagedAttnArgs& a, RowIter& it) {
+  if (++it.step < it.steps) return;
+  it.step = 0;
+  if (++it.h < a.c.hkv) return;
+  it.h = 0;
+  ++it.b;
+  next_sequence<kStep>(a, it);
+}
+
+// Steps of all sequences, and where step `first` lies (all threads take part; two barriers per 256 sequences).
+template <int kStep>
+__device__ __forceinline__ int row_total(const PagedAttnArgs& a, RowSmem* sm) {
+  int mine = 0;
+  for (int b = threadIdx.x; b < a.c.batch; b += kRowThreads)
+    mine += unit_steps<kStep>(a, paged_seq(a.c, b, a.max_queries, a.max_keys)) * a.c.hkv;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+  if ((threadIdx.x & 31) == 0) sm->warp_sum[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < kRowWarps; ++w) total += sm->warp_sum[w];
+  __syncthreads();
+  return total;
+}
+// Inclusive scan over the block of one value per thread, plus `before`.
+__device__ __forceinline__ int row_scan(int mine, int before, int* warp_sum, int& all) {
+  int incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, incl, d);
+    if ((int)(threadIdx.x & 31) >= d) incl += up;
+  }
+  if ((threadIdx.x & 31) == 31) warp_sum[threadIdx.x >> 5] = incl;
+  __syncthreads();
+  int add = before;
+  all = before;
+  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
+    if (w < (int)(threadIdx.x >> 5)) add += warp_sum[w];
+    all += warp_sum[w];
+  }
+  __syncthreads();
+  return incl + add;
+}
+
+// CTA i of n takes steps [total * i / n, total * (i + 1) / n).  Short lists use fewer CTAs: at least kMinSteps each.
+constexpr int kMinSteps = 2;
+__device__ __forceinline__ int row_ctas(int total, int grid) { return max(1, min(grid, total / kMinSteps)); }
+__device__ __forceinline__ int row_begin(int total, int i, int n) { return (int)((long long)total * i / n); }
+
+template <bool kFp8, int kTiles>
+__global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
+  using S = RowShape<kFp8>;
+  constexpr int kStep = S::kStep, kKeys = S::kKeys, kBlocks = kKeys / 8;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* stages = smem_raw + warp * (kRowStages * S::kStage);
+  uint8_t* queries = smem_raw + kRowWarps * kRowStages * S::kStage;  // rows of 256 bytes, pieces swapped like the keys'
+  float* merge = reinterpret_cast<float*>(queries + 32 * 2 * kHeadDim);
+  RowSmem* sm = reinterpret_cast<RowSmem*>(merge + 32 * S::kPitch);
+  const uint32_t stage0 = smem_u32(stages);
+
+  grid_dependents_launch();
+  grid_dependency_wait();
+
+  // sequences without keys: their rows see nothing
+  for (int b = blockIdx.x; b < a.c.batch; b += gridDim.x) {
+    const PagedSeq seq = paged_seq(a.c, b, a.max_queries, a.max_keys);
+    if (seq.len > 0 || seq.n * a.group > a.few) continue;
+    for (int i = warp; i < seq.n * a.hq; i += kRowWarps) {
+      const int tok = seq.start + i / a.hq, hd = i % a.hq;
+      *reinterpret_cast<uint2*>(a.o + b * a.o_sb + (long long)tok * a.o_st + (long long)hd * a.o_sh + lane * 4) = make_uint2(0, 0);
+      if (lane == 0) a.lse[b * a.lse_sb + hd * a.lse_sh + tok] = -INFINITY;
+    }
+  }
+
+  // this CTA's part of the list
+  const int total = row_total<kStep>(a, sm);
+  const int ctas = row_ctas(total, gridDim.x);
+  if (tid == 0) a.open[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if ((int)blockIdx.x >= ctas || total == 0) return;
+  const int first = row_begin(total, blockIdx.x, ctas), last = row_begin(total, blockIdx.x + 1, ctas);
+  int before = 0;
+  for (int b0 = 0; b0 < a.c.batch; b0 += kRowThreads) {
+    const int b = b0 + tid;
+    const int mine = b < a.c.batch ? unit_steps<kStep>(a, paged_seq(a.c, b, a.max_queries, a.max_keys)) * a.c.hkv : 0;
+    const int incl = row_scan(mine, before, sm->warp_sum, before);
+    if (first >= incl - mine && first < incl) {
+      sm->b = b;
+      sm->step = first - (incl - mine);
+    }
+  }
+  __syncthreads();
+
+  RowIter in;  // what is loaded next
+  in.b = sm->b;
+  in.s = paged_seq(a.c, in.b, a.max_queries, a.max_keys);
+  in.steps = unit_steps<kStep>(a, in.s);
+  in.h = sm->step / in.steps;
+  in.step = sm->step - in.h * in.steps;
+  RowIter at = in;  // what is computed next
+
+  // page of this lane's key of the step to load, fetched one step ahead
+  auto page_of = [&](const RowIter& it) {
+    const int pos = it.step * kStep + warp * kKeys + (lane & (kKeys - 1));
+    if (pos >= it.s.len) return -1;
+    const int id = a.c.table[it.b * a.c.table_stride + page_index(a.c, pos)];
+    if (id < 0 || id >= a.c.pages) {
+      paged_error(a.c);
+      return -1;
+    }
+    return id;
+  };
+  int page = page_of(in);
+
+  auto load = [&](int stage) {
+    const int pos = in.step * kStep + warp * kKeys + (lane & (kKeys - 1));
+    const int slot = pos - page_index(a.c, pos) * a.c.page_size;
+    const long long off = page >= 0 ? paged_offset(a.c, page, slot, in.h) : -1;
+    const uint32_t dst = stage0 + stage * S::kStage;
+#pragma unroll
+    for (int i = 0; i < kKeys * S::kPieces / 32; ++i) {
+      const int key = i * (32 / S::kPieces) + lane / S::kPieces, piece = lane % S::kPieces;
+      const long long from = __shfl_sync(0xffffffffu, off, key);
+      const bool real = from >= 0;
+      const uint32_t to = dst + key * S::kRowBytes + ((piece ^ (key & 7)) << 4);
+      cp_async16(to, real ? a.c.k + from + piece * 16 : a.c.k, real);
+      cp_async16(to + S::kHalf, real ? a.c.v + from + piece * 16 : a.c.v, real);
+    }
+    if constexpr (kFp8) {
+      const long long so = page >= 0 ? scale_offset(a.c, page, slot, in.h) : 0;
+      cp_async4(dst + 2 * S::kHalf + lane * 4, a.c.k_scale + so, page >= 0);
+      cp_async4(dst + 2 * S::kHalf + S::kScaleBytes + lane * 4, a.c.v_scale + so, page >= 0);
+    }
+  };
+
+  int to_load = last - first;
+#pragma unroll
+  for (int i = 0; i < kRowStages - 1; ++i) {
+    if (to_load > 0) {
+      load(i);
+      if (--to_load > 0) {
+        next_step<kStep>(a, in);
+        page = page_of(in);
+      }
+    }
+    cp_async_commit();
+  }
+
+  // Queries: the next unit's are fetched into registers while this one's are in use (from shared memory).
+  RowIter nx = at;  // the unit behind this one
+  uint4 qx[kTiles];
+  auto next_unit = [&]() {
+    nx.step = 0;
+    if (++nx.h < a.c.hkv) return;
+    nx.h = 0;
+    ++nx.b;
+    next_sequence<kStep>(a, nx);
+  };
+  auto fetch_q = [&]() {
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      const int r = m * 16 + (tid >> 4), tok = r / a.group, hd = r - tok * a.group;
+      qx[m] = make_uint4(0, 0, 0, 0);
+      if (nx.b < a.c.batch && r < nx.s.n * a.group)
+        qx[m] = __ldg(reinterpret_cast<const uint4*>(a.q + nx.b * a.q_sb + (long long)(nx.s.start + tok) * a.q_st +
+                                                     (long long)(nx.h * a.group + hd) * a.q_sh) + (tid & 15));
+    }
+  };
+  // A lane of the matrix instruction takes element pairs (2 t, 2 t + 1) and (8 + 2 t, ...) of 16 along head_dim.  Of e4m3 keys
+  // it gets four neighbouring values at once, so that its two pairs are 4 t .. 4 t + 3; the queries are put in that order.
+  auto store_q = [&]() {
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      const int r = m * 16 + (tid >> 4), piece = tid & 15;
+      uint8_t* row = queries + r * 2 * kHeadDim;
+      if constexpr (!kFp8) {
+        *reinterpret_cast<uint4*>(row + ((piece ^ (r & 7)) << 4)) = qx[m];
+      } else {
+        *reinterpret_cast<uint2*>(row + (((piece & 14) ^ (r & 7)) << 4) + (piece & 1) * 8) = make_uint2(qx[m].x, qx[m].z);
+        *reinterpret_cast<uint2*>(row + (((piece | 1) ^ (r & 7)) << 4) + (piece & 1) * 8) = make_uint2(qx[m].y, qx[m].w);
+      }
+    }
+  };
+  const uint32_t q_addr = smem_u32(queries) + (lane & 15) * 2 * kHeadDim;
+  auto query = [&](uint32_t (&qf)[4], int m, int k) {
+    ldsm4(qf, q_addr + m * 16 * 2 * kHeadDim + (((2 * k + (lane >> 4)) ^ (lane & 7)) << 4));
+  };
+
+  float acc[kTiles][16][4], m_ref[kTiles][2], l[kTiles][2];
+  int limit[kTiles][2];  // keys that the row sees
+  auto begin_unit = [&]() {
+    store_q();
+    next_unit();
+    fetch_q();
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        m_ref[m][half] = -INFINITY;
+        l[m][half] = 0.f;
+        limit[m][half] = at.s.len;
+        if (a.causal) limit[m][half] = min(at.s.len, at.s.len - at.s.n + (m * 16 + half * 8 + g) / a.group + 1);
+      }
+    }
+  };
+  fetch_q();
+  begin_unit();
+  __syncthreads();
+
+  bool from_start = at.step == 0;  // the unit's earlier steps are not another CTA's
+  int stage = 0;
+  for (int s = first; s < last; ++s) {
+    // ---- keep the loads going
+    if (to_load > 0) {
+      load(stage == 0 ? kRowStages - 1 : stage - 1);
+      if (--to_load > 0) {
+        next_step<kStep>(a, in);
+        page = page_of(in);
+      }
+    }
+    cp_async_commit();
+    cp_async_wait<kRowStages - 1>();
+    __syncwarp();
+
+    // ---- one step
+    const uint32_t sk = stage0 + stage * S::kStage, sv = sk + S::kHalf;
+    const int key0 = at.step * kStep + warp * kKeys;
+    float sc[kTiles][kBlocks][4];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[m][j][e] = 0.f;
+    if constexpr (!kFp8) {
+      // four 8 x 8 matrices: keys 0-7 and 8-15 x two 16-byte pieces
+      const int row = (lane & 7) + ((lane >> 4) << 3), odd = (lane >> 3) & 1;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t b[4];
+        ldsm4(b, sk + row * S::kRowBytes + (((2 * k + odd) ^ (row & 7)) << 4));
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m) {
+          uint32_t qf[4];
+          query(qf, m, k);
+          mma16816(sc[m][0], qf, b[0], b[1]);
+          mma16816(sc[m][1], qf, b[2], b[3]);
+        }
+      }
+    } else {
+      // four matrices: the 32 keys x one piece of 16 values
+      const uint8_t* ks = stages + stage * S::kStage + 2 * S::kHalf;
+      uint32_t kb[kBlocks];
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) kb[j] = *reinterpret_cast<const uint32_t*>(ks + (j * 8 + g) * 4);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t b[4];
+        ldsm4(b, sk + lane * S::kRowBytes + ((k ^ (lane & 7)) << 4));
+        uint32_t qf[kTiles][4];
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m) query(qf[m], m, k);
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j) {
+          const uint32_t mult = ((((kb[j] >> (8 * (k >> 1))) & 0xffu) + kScaleAdd) << 7) * 0x10001u;
+          const uint32_t b0 = mul_bf16x2(e4m3_bits(__byte_perm(b[j], 0, 0x1404)), mult);
+          const uint32_t b1 = mul_bf16x2(e4m3_bits(__byte_perm(b[j], 0, 0x3424)), mult);
+#pragma unroll
+          for (int m = 0; m < kTiles; ++m) mma16816(sc[m][j], qf[m], b0, b1);
+        }
+      }
+      // scale bytes beyond the written range: the key's scores are not numbers
+      uint32_t odd = 0;
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) odd |= kb[j] & (kb[j] << 1) & 0x80808080u;
+      if (__any_sync(0xffffffffu, odd != 0)) {
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(ks + (j * 8 + 2 * t + (e & 1)) * 4);
+            if (w & (w << 1) & 0x80808080u)
+#pragma unroll
+              for (int m = 0; m < kTiles; ++m) sc[m][j][e] = __int_as_float(0x7fffffff);
+          }
+      }
+    }
+
+    // ---- softmax; a lane holds keys 8 j + 2 t + {0, 1} of rows g and g + 8 of a tile
+    uint32_t pf[kTiles][kBlocks / 2][4];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (key0 + j * 8 + 2 * t + (e & 1) >= limit[m][e >> 1]) sc[m][j][e] = -INFINITY;
+          top[e >> 1] = fmaxf(top[e >> 1], sc[m][j][e]);
+        }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
+        top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
+      }
+      // The reference maximum only moves when a score exceeds it by 2^8 in the exponentials' scale.
+      const bool need0 = (top[0] - m_ref[m][0]) * a.scale_log2 > 8.f, need1 = (top[1] - m_ref[m][1]) * a.scale_log2 > 8.f;
+      if (__any_sync(0xffffffffu, need0 || need1)) {
+        float f[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const bool need = half ? need1 : need0;
+          f[half] = need ? fast_exp2((m_ref[m][half] - top[half]) * a.scale_log2) : 1.f;
+          if (need) m_ref[m][half] = top[half];
+          l[m][half] *= f[half];
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[m][j][e] *= f[e >> 1];
+      }
+      const float ms[2] = {m_ref[m][0] == -INFINITY ? 0.f : m_ref[m][0] * a.scale_log2,
+                           m_ref[m][1] == -INFINITY ? 0.f : m_ref[m][1] * a.scale_log2};
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = fast_exp2(fmaf(sc[m][j][e], a.scale_log2, -ms[e >> 1]));
+          l[m][e >> 1] += p[e];
+        }
+        pf[m][j >> 1][(j & 1) * 2 + 0] = pack_bf16x2(p[0], p[1]);
+        pf[m][j >> 1][(j & 1) * 2 + 1] = pack_bf16x2(p[2], p[3]);
+      }
+    }
+
+    // ---- values
+    if constexpr (!kFp8) {
+      const int row = lane & 15, odd = lane >> 4;  // keys 0-7, 8-15 x two pieces
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        uint32_t b[4];
+        ldsm4_t(b, sv + row * S::kRowBytes + (((j + odd) ^ (row & 7)) << 4));
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m) {
+          mma16816(acc[m][j], pf[m][0], b[0], b[1]);
+          mma16816(acc[m][j + 1], pf[m][0], b[2], b[3]);
+        }
+      }
+    } else {
+      // Transposed 16-bit units are pairs of neighbouring values: a lane gets values (2 g, 2 g + 1) of keys (2 t, 2 t + 1) of
+      // each 8; the even ones make one 8-column block of the product and the odd ones the next.
+      const uint8_t* vs = stages + stage * S::kStage + 2 * S::kHalf + S::kScaleBytes;
+      uint2 vb[kBlocks];
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) vb[j] = *reinterpret_cast<const uint2*>(vs + (j * 8 + 2 * t) * 4);
+      uint32_t mult[kBlocks];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if ((c & 1) == 0) {
+#pragma unroll
+          for (int j = 0; j < kBlocks; ++j) {
+            const uint32_t two = __byte_perm(vb[j].x, vb[j].y, (c >> 1) | ((4 + (c >> 1)) << 4));  // bytes 0 and 1
+            mult[j] = (((two & 0xffu) | ((two & 0xff00u) << 8)) + kScaleAdd * 0x10001u) << 7;
+          }
+        }
+        uint32_t b[4];
+        ldsm4_t(b, sv + lane * S::kRowBytes + ((c ^ (lane & 7)) << 4));
+        uint32_t even[4], odd[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          even[j] = mul_bf16x2(e4m3_bits(__byte_perm(b[j], 0, 0x2404)), mult[j]);
+          odd[j] = mul_bf16x2(e4m3_bits(__byte_perm(b[j], 0, 0x3414)), mult[j]);
+        }
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m) {
+          mma16816(acc[m][2 * c], pf[m][0], even[0], even[1]);
+          mma16816(acc[m][2 * c + 1], pf[m][0], odd[0], odd[1]);
+          mma16816(acc[m][2 * c], pf[m][1], even[2], even[3]);
+          mma16816(acc[m][2 * c + 1], pf[m][1], odd[2], odd[3]);
+        }
+      }
+      uint32_t bad = 0;  // by scale block
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) bad |= (vb[j].x & (vb[j].x << 1) & 0x80808080u) | (vb[j].y & (vb[j].y << 1) & 0x80808080u);
+      if (__any_sync(0xffffffffu, bad != 0)) {
+        bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
+        bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (bad & (0x80u << (8 * (j >> 2))))
+#pragma unroll
+            for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[m][j][e] = __int_as_float(0x7fffffff);
+      }
+    }
+    __syncwarp();
+    stage = stage + 1 == kRowStages ? 0 : stage + 1;
+
+    // ---- end of the unit, or of this CTA's part of it
+    const bool done = at.step + 1 == at.steps;
+    if (!done && s + 1 < last) {
+      ++at.step;
+      continue;
+    }
+    const int rows = at.s.n * a.group;
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x = l[m][half];
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        if (t == 0) sm->ml[warp][m * 16 + half * 8 + g] = make_float2(m_ref[m][half], x);
+      }
+    __syncthreads();
+    float f[kTiles][2];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm->ml[w][m * 16 + half * 8 + g].x);
+        f[m][half] = m_ref[m][half] == -INFINITY ? 0.f : fast_exp2((m_ref[m][half] - top) * a.scale_log2);
+        // a warp without a visible key has nothing, whatever its masked products gave
+        if (m_ref[m][half] == -INFINITY && !(l[m][half] != l[m][half])) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[m][j][2 * half] = acc[m][j][2 * half + 1] = 0.f;
+        }
+      }
+    constexpr int kBuffers = 2 / kTiles;
+    for (int round = 0; round < kRowWarps / kBuffers; ++round) {
+      if (warp / kBuffers == round) {
+        float* buf = merge + (kTiles == 1 ? (warp & 1) * 16 * S::kPitch : 0);
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int r = m * 16 + half * 8 + g;
+            if (r < rows) {
+              if constexpr (!kFp8) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  float2* p = reinterpret_cast<float2*>(buf + r * S::kPitch + j * 8 + t * 2);
+                  float2 x = make_float2(acc[m][j][2 * half] * f[m][half], acc[m][j][2 * half + 1] * f[m][half]);
+                  if (round > 0) {
+                    const float2 y = *p;
+                    x.x += y.x; x.y += y.y;
+                  }
+                  *p = x;
+                }
+              } else {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                  float4* p = reinterpret_cast<float4*>(buf + r * S::kPitch + c * 16 + t * 4);
+                  const float* ev = acc[m][2 * c] + 2 * half;
+                  const float* od = acc[m][2 * c + 1] + 2 * half;
+                  float4 x = make_float4(ev[0] * f[m][half], od[0] * f[m][half], ev[1] * f[m][half], od[1] * f[m][half]);
+                  if (round > 0) {
+                    const float4 y = *p;
+                    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+                  }
+                  *p = x;
+                }
+              }
+            }
+          }
+      }
+      __syncthreads();
+    }
+    const bool whole = from_start && done;
+    const int slot = 2 * blockIdx.x + (from_start ? 1 : 0);
+    for (int r = warp; r < rows; r += kRowWarps) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm->ml[w][r].x);
+#pragma unroll
+      for (int w = 0; w < kRowWarps; ++w) {
+        const float2 x = sm->ml[w][r];
+        sum += x.x == -INFINITY ? x.y : x.y * fast_exp2((x.x - top) * a.scale_log2);
+      }
+      float4 x = *reinterpret_cast<const float4*>(merge + r * S::kPitch + lane * 4);
+      if constexpr (kTiles == 1) {
+        const float4 y = *reinterpret_cast<const float4*>(merge + (16 + r) * S::kPitch + lane * 4);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
+      if (whole) {
+        const int tok = r / a.group, hd = at.h * a.group + r - tok * a.group;
+        const float inv = sum == 0.f ? 0.f : a.out_scale / sum;
+        const uint2 w = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+        *reinterpret_cast<uint2*>(a.o + at.b * a.o_sb + (long long)(at.s.start + tok) * a.o_st + (long long)hd * a.o_sh + lane * 4) = w;
+        if (lane == 0)
+          a.lse[at.b * a.lse_sb + hd * a.lse_sh + at.s.start + tok] = sum == 0.f ? -INFINITY : top * a.scale + __logf(sum);
+      } else {
+        *reinterpret_cast<float4*>(a.part_o + ((long long)slot * (16 * kTiles) + r) * kHeadDim + lane * 4) = x;
+        if (lane == 0) a.part_ml[slot * (16 * kTiles) + r] = make_float2(top, sum);
+      }
+    }
+    if (from_start && !done && tid == 0) {
+      // the unit goes on in the next CTAs: how many of them it takes
+      const int end = s + at.steps - at.step;  // behind its last step
+      int n = 1;
+      while (row_begin(total, blockIdx.x + n, ctas) < end) ++n;
+      a.open[blockIdx.x] = make_int4(at.b, at.h, n, 0);
+    }
+    if (s + 1 < last) {
+      at = nx;
+      from_start = true;
+      begin_unit();
+      __syncthreads();  // the buffers are free again
+    }
+  }
+}
+
+// Joins the partial states of the unit that CTA blockIdx.x of the launch before began and did not finish (if there is one):
+// row blockIdx.y.  A warp takes every eighth of the parts, four columns a lane; the warps' sums are added in order.
+template <int kRows>
+__global__ void __launch_bounds__(kRowThreads) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
+  __shared__ float4 part[kRowWarps][32];
+  __shared__ float part_l[kRowWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y;
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int4 unit = a.open[blockIdx.x];
+  if (unit.z == 0) return;
+  const PagedSeq seq = paged_seq(a.c, unit.x, a.max_queries, a.max_keys);
+  if (r >= seq.n * a.group) return;
+  const int n = unit.z;
+  // slot of the unit's p-th CTA: it ends the list of the first one and starts those of the others
+  auto slot = [&](int p) { return (long long)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * kRows + r; };
+  float top = -INFINITY;
+  for (int p = lane; p < n; p += 32) top = fmaxf(top, a.part_ml[slot(p)].x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  float sum = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int p = warp; p < n; p += kRowWarps) {
+    const float2 ml = a.part_ml[slot(p)];
+    const float4 y = *reinterpret_cast<const float4*>(a.part_o + slot(p) * kHeadDim + lane * 4);
+    // (a part without visible keys holds zeros, or what is not a number)
+    const float w = ml.x == -INFINITY ? 1.f : fast_exp2((ml.x - top) * a.scale_log2);
+    sum = fmaf(w, ml.y, sum);
+    x.x = fmaf(w, y.x, x.x);
+    x.y = fmaf(w, y.y, x.y);
+    x.z = fmaf(w, y.z, x.z);
+    x.w = fmaf(w, y.w, x.w);
+  }
+  part[warp][lane] = x;
+  if (lane == 0) part_l[warp] = sum;
+  __syncthreads();
+  if (warp != 0) return;
+#pragma unroll
+  for (int w = 1; w < kRowWarps; ++w) {
+    const float4 y = part[w][lane];
+    sum += part_l[w];
+    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+  }
+  const int tok = seq.start + r / a.group, hd = unit.y * a.group + r % a.group;
+  const float inv = sum == 0.f ? 0.f : a.out_scale / sum;
+  const uint2 w = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+  *reinterpret_cast<uint2*>(a.o + unit.x * a.o_sb + (long long)tok * a.o_st + (long long)hd * a.o_sh + lane * 4) = w;
+  if (lane == 0) a.lse[unit.x * a.lse_sb + hd * a.lse_sh + tok] = sum == 0.f ? -INFINITY : top * a.scale + __logf(sum);
+}
+
+int paged_rows_ctas() { return sm_count(); }
+
+long long paged_rows_workspace(int rows, int ctas) {
+  const int padded = rows <= 16 ? 16 : 32;
+  return 2ll * ctas * padded * (kHeadDim * (long long)sizeof(float) + (long long)sizeof(float2)) + ctas * (long long)sizeof(int4);
+}
+
+template <bool kFp8, int kTiles>
+static int launch_rows(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
+  static bool attr_set[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MB_E_CUDA;
+  constexpr int bytes = row_smem_bytes<kFp8>();
+  static_assert(bytes <= 232448, "shared memory budget of one CTA");
+  if (!attr_set[dev]) {
+    if (!cuda_ok(cudaFuncSetAttribute(paged_rows_kernel<kFp8, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                 "paged_rows_kernel shared memory"))
+      return MB_E_CUDA;
+    attr_set[dev] = true;
+  }
+  if (!launch_overlapped("launch paged_rows_kernel", paged_rows_kernel<kFp8, kTiles>, dim3(ctas), kRowThreads, bytes, stream, a))
+    return MB_E_CUDA;
+  if (!launch_overlapped("launch paged_merge_kernel", paged_merge_kernel<16 * kTiles>,
+                         dim3(ctas, min(a.few, a.max_queries * a.group)), kRowThreads, 0, stream, a))
+    return MB_E_CUDA;
+  return MB_SUCCESS;
+}
+
+int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream) {
+  if (rows <= 16) return fp8 ? launch_rows<true, 1>(a, ctas, stream) : launch_rows<false, 1>(a, ctas, stream);
+  return fp8 ? launch_rows<true, 2>(a, ctas, stream) : launch_rows<false, 2>(a, ctas, stream);
+}
+
+}  // namespace mb

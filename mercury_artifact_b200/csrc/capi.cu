@@ -117,6 +117,23 @@ int mb_attn_bwd_block_noalloc(const mb_attn_bwd_block_args* args, void* cuda_str
   return mb::launch_bwd_block_noalloc(args, static_cast<cudaStream_t>(cuda_stream));
 }
 
+int mb_kv_cache_write(const mb_paged_kv* kv, const void* k_new, const void* v_new, int64_t stride_b, int64_t stride_t,
+                      int64_t stride_h, void* cuda_stream) {
+  return mb::launch_kv_cache_write(kv, k_new, v_new, stride_b, stride_t, stride_h, static_cast<cudaStream_t>(cuda_stream));
+}
+
+int mb_kv_cache_read(const mb_paged_kv* kv, void* k_out, void* v_out, int64_t stride_b, int64_t stride_s,
+                     int64_t stride_h, int32_t rows, void* cuda_stream) {
+  return mb::launch_kv_cache_read(kv, k_out, v_out, stride_b, stride_s, stride_h, rows,
+                                  static_cast<cudaStream_t>(cuda_stream));
+}
+
+int64_t mb_attn_paged_workspace(const mb_attn_paged_args* args) { return mb::attn_paged_workspace(args); }
+
+int mb_attn_paged(const mb_attn_paged_args* args, void* workspace, uint64_t workspace_bytes, void* cuda_stream) {
+  return mb::launch_attn_paged(args, workspace, workspace_bytes, static_cast<cudaStream_t>(cuda_stream));
+}
+
 int mb_flash_reduce(const float* lhs, const float* rhs, float* out, int64_t rows, int32_t head_dim_plus_1,
                     void* cuda_stream) {
   return mb::launch_flash_reduce(lhs, rhs, out, rows, head_dim_plus_1, static_cast<cudaStream_t>(cuda_stream));

@@ -55,6 +55,12 @@ int launch_attn_bwd(const mb_attn_bwd_args* args, cudaStream_t stream);
 int launch_dq_convert(const float* acc, void* dq, long long sb, long long ss, long long sh, int batch, int sq, int hq,
                       int pad, int out_mode, float scale, cudaStream_t stream);
 int launch_bwd_block_sweep(const mb_attn_bwd_block_args* args, float* stats, float* dq_accum, cudaStream_t stream);
+int launch_kv_cache_write(const mb_paged_kv* kv, const void* k_new, const void* v_new, long long sb, long long st,
+                          long long sh, cudaStream_t stream);
+int launch_kv_cache_read(const mb_paged_kv* kv, void* k_out, void* v_out, long long sb, long long ss, long long sh,
+                         int rows, cudaStream_t stream);
+long long attn_paged_workspace(const mb_attn_paged_args* args);
+int launch_attn_paged(const mb_attn_paged_args* args, void* ws, unsigned long long ws_bytes, cudaStream_t stream);
 int launch_bwd_block_noalloc(const mb_attn_bwd_block_args* args, cudaStream_t stream);
 
 }  // namespace mb
