@@ -6,30 +6,61 @@ namespace mb {
 constexpr int kFewRows = 32;  // most rows that paged_rows_kernel takes
 
 struct PagedPlan {
-  int few, rows, ctas;
-  long long rows_bytes;  // workspace of the kernel for few rows
+  int few;               // most rows of a sequence that go to the kernel for few rows
+  int rows, row_ctas;    // rows of its units (0: it has nothing to do)
+  int tile_ctas;         // grid of the kernel for tiles (0: it has nothing to do)
+  int share_tiles;
+  bool split;
+  long long rows_bytes, tiles_bytes;  // workspaces
 };
 
+// Everything here goes by the bounds that the host knows; the lengths are on the device.
 static int plan_paged(const mb_attn_paged_args* x, PagedPlan* p) {
   if (x->hq <= 0 || x->kv.hkv <= 0 || x->hq % x->kv.hkv != 0) return MB_E_INVALID;
   if (x->max_queries < 0 || x->max_keys < 0 || !(x->softmax_scale > 0.f) || x->softmax_scale > 3e38f) return MB_E_INVALID;
-  if (x->kv.batch < 0 || x->kv.page_size <= 0 || x->kv.max_pages < 0) return MB_E_INVALID;
-  const int group = x->hq / x->kv.hkv;
-  if ((long long)x->max_queries * group > 0x7fffff00ll) return MB_E_INVALID;
+  if (x->kv.batch < 0 || x->kv.tokens < 0 || x->kv.page_size <= 0 || x->kv.max_pages < 0) return MB_E_INVALID;
+  const long long group = x->hq / x->kv.hkv, rows = x->max_queries * group;
+  if (rows > 0x7fffff00ll) return MB_E_TOO_LARGE;
   // steps of a launch are counted in 32 bits
   if ((double)x->kv.batch * x->kv.hkv * ((double)x->max_keys / 128 + 1) > 2e9) return MB_E_TOO_LARGE;
+  const int sms = sm_count();
+  if (sms <= 0) return MB_E_CUDA;
+  memset(p, 0, sizeof(*p));
+  const bool padded = x->kv.cu_seqlens == nullptr;
   p->few = kFewRows;
-  p->rows = min(x->max_queries * group, kFewRows);
-  p->ctas = paged_rows_ctas();
-  if (p->ctas <= 0) return MB_E_CUDA;
-  p->rows_bytes = paged_rows_workspace(p->rows, p->ctas);
+  if (rows <= kFewRows || !padded) {
+    p->rows = (int)min(rows, (long long)kFewRows);
+    p->row_ctas = paged_rows_ctas();
+    p->rows_bytes = paged_rows_workspace(p->rows, p->row_ctas);
+  }
+  if (rows > kFewRows) {
+    // units: blocks of 256 rows of a sequence and K/V head.  A ragged batch has at most one partly filled block per sequence.
+    const long long blocks = padded ? x->kv.batch * ((rows + 255) / 256) : min(x->kv.batch * ((rows + 255) / 256), x->kv.tokens * group / 256 + x->kv.batch);
+    const long long units = blocks * x->kv.hkv, tiles = max(1, (x->max_keys + 127) / 128);
+    // Costs in steps of one K/V tile against both query tiles: starting and ending a CTA, and joining the shares.
+    constexpr double kCta = 2.0, kMerge = 2.0, kSlot = 0.02;
+    long long best = 1;
+    double t_best = ((units + sms - 1) / sms) * (tiles + kCta);
+    for (long long ns = 2; ns <= 64 && ns <= tiles && units * ns <= 3ll * sms; ++ns) {
+      const double t = ((units * ns + sms - 1) / sms) * ((tiles + ns - 1) / ns + kCta) + kMerge + kSlot * units * ns;
+      if (t < t_best) {
+        t_best = t;
+        best = ns;
+      }
+    }
+    if (units * best > 0x7fffff00ll) return MB_E_TOO_LARGE;
+    p->share_tiles = (int)((tiles + best - 1) / best);
+    p->split = best > 1;
+    p->tile_ctas = (int)(units * ((tiles + p->share_tiles - 1) / p->share_tiles));
+    if (p->split) p->tiles_bytes = paged_tiles_workspace(p->tile_ctas);
+  }
   return MB_SUCCESS;
 }
 
 long long attn_paged_workspace(const mb_attn_paged_args* x) {
   PagedPlan p;
   if (x == nullptr || plan_paged(x, &p) != MB_SUCCESS) return 0;
-  return p.rows_bytes;
+  return max(p.rows_bytes, p.tiles_bytes);
 }
 
 int launch_attn_paged(const mb_attn_paged_args* x, void* ws, unsigned long long ws_bytes, cudaStream_t stream) {
@@ -48,7 +79,8 @@ int launch_attn_paged(const mb_attn_paged_args* x, void* ws, unsigned long long 
                        (uintptr_t)(x->q_stride_t * 2) | (uintptr_t)(x->q_stride_h * 2) | (uintptr_t)(x->o_stride_b * 2) |
                        (uintptr_t)(x->o_stride_t * 2) | (uintptr_t)(x->o_stride_h * 2);
   if (al & 15u) return MB_E_INVALID;
-  if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15u) || ws_bytes < (unsigned long long)p.rows_bytes) return MB_E_INVALID;
+  const long long need = max(p.rows_bytes, p.tiles_bytes);
+  if (need > 0 && (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15u) || ws_bytes < (unsigned long long)need)) return MB_E_INVALID;
 
   a.q = static_cast<const __nv_bfloat16*>(x->q);
   a.q_sb = a.c.cu != nullptr ? 0 : x->q_stride_b;
@@ -72,14 +104,34 @@ int launch_attn_paged(const mb_attn_paged_args* x, void* ws, unsigned long long 
   a.scale_log2 = x->softmax_scale * 1.4426950408889634f * unbias;
   a.out_scale = unbias;
   a.few = p.few;
-  if (x->max_queries * a.group > kFewRows) return MB_E_UNSUPPORTED;
+  a.share_tiles = max(p.share_tiles, 1);
+  a.head_bytes = fp8 ? 2 * kHeadDim : 4 * kHeadDim;
+  a.tile_o = nullptr;
+  a.tile_ml = nullptr;
+  a.tile_open = nullptr;
+  a.part_o = nullptr;
+  a.part_ml = nullptr;
+  a.open = nullptr;
 
-  // [partial rows | (maximum, sum) | open units]
-  const long long slots = 2ll * p.ctas * (p.rows <= 16 ? 16 : 32);
-  a.part_o = static_cast<float*>(ws);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * kHeadDim);
-  a.open = reinterpret_cast<int4*>(a.part_ml + slots);
-  return launch_paged_rows(a, fp8, p.rows, p.ctas, stream);
+  // The two kernels run one after the other and use the workspace in turn.
+  if (p.tile_ctas > 0) {
+    if (p.split) {  // [rows | (maximum, sum) | split units]
+      a.tile_o = static_cast<float4*>(ws);
+      a.tile_ml = reinterpret_cast<float2*>(a.tile_o + (long long)p.tile_ctas * (256 * kHeadDim / 4));
+      a.tile_open = reinterpret_cast<int4*>(a.tile_ml + (long long)p.tile_ctas * 256);
+    }
+    rc = launch_paged_tiles(a, fp8, p.tile_ctas, stream);
+    if (rc != MB_SUCCESS) return rc;
+  }
+  if (p.row_ctas > 0) {
+    // [partial rows | (maximum, sum) | open units]
+    const long long slots = 2ll * p.row_ctas * (p.rows <= 16 ? 16 : 32);
+    a.part_o = static_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * kHeadDim);
+    a.open = reinterpret_cast<int4*>(a.part_ml + slots);
+    rc = launch_paged_rows(a, fp8, p.rows, p.row_ctas, stream);
+  }
+  return rc;
 }
 
 }  // namespace mb

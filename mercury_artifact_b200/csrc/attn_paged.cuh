@@ -24,10 +24,20 @@ struct PagedAttnArgs {
   float* part_o;
   float2* part_ml;
   int4* open;
+  // tiles: keys (in tiles of 128) of a share of a unit; partial results [CTA][32 column groups][256 rows], (maximum, sum)
+  // [CTA][256]; tile_open: the split unit whose first share a CTA has (sequence, K/V head, row block, shares; 0: none).
+  // All null where no unit is split.
+  int share_tiles;
+  int head_bytes;  // of a cached key and value of one head
+  float4* tile_o;
+  float2* tile_ml;
+  int4* tile_open;
 };
 
 int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream);
 long long paged_rows_workspace(int rows, int ctas);
 int paged_rows_ctas();
+int launch_paged_tiles(const PagedAttnArgs& a, bool fp8, int ctas, cudaStream_t stream);
+long long paged_tiles_workspace(long long ctas);
 
 }  // namespace mb

@@ -1,0 +1,650 @@
+// Attention of many rows over keys and values in pages: chunks of a prompt, cross attention.
+//
+// The rows of a unit are the new tokens of one sequence times the query heads of one K/V head (row = token * group +
+// head): the heads of a group share every key and value that is loaded.  One CTA owns two tiles of 128 rows and
+// streams tiles of 128 keys through them, like attn_fwd_kernel, whose tensor-memory layout and hand-overs it has: scores
+// S = Q K^T by tcgen05 into one score region that the two query tiles use in turn, online softmax with one thread
+// per row, probabilities in bf16 as the tensor-memory operand of O += P V.
+//
+// What differs is how keys and values arrive.  A page may end anywhere inside a tile, pages lie anywhere, and
+// the slots behind a sequence's end hold anything, so that a warpgroup of four warps gathers each tile row by row:
+// bf16 with cp.async, 16 bytes a piece, straight into the swizzled layout that tcgen05 reads; e4m3 through registers,
+// where a code becomes code * 2^n in bf16 on the way (see paged_common.cuh), one tile ahead.  Rows behind the end are
+// filled with zeros.
+//
+//   warps 0-3   softmax + epilogue of query tile 0 (one thread per row)
+//   warps 4-7   softmax + epilogue of query tile 1
+//   warp  8     issues Q K^T, owns tensor memory;  warp 10 issues P V;  warps 9 and 11 idle
+//   warps 12-15 gather queries, keys and values
+//
+// A launch has one CTA per (sequence, 256 rows, K/V head, share of the keys), found on the device from the lengths that
+// are there; CTAs beyond the last of them return.  Shares leave their unnormalised rows, maxima and sums in
+// the workspace and paged_tiles_merge_kernel joins them in order.
+#include "attn_paged.cuh"
+#include "attn_fwd_common.cuh"
+
+namespace mb {
+
+constexpr int kTileThreads = 512;
+constexpr int kTileStages = 4;
+constexpr int kGather = 128;  // threads that gather
+// Registers of the softmax warps and of the others, out of 128 a thread at launch (an increase beyond that pool would block
+// forever, hence the check).
+template <bool kFp8>
+struct TileRegs {
+  static constexpr int kSoftmax = kFp8 ? 200 : 208, kOthers = kFp8 ? 56 : 48;
+  static_assert(256 * kSoftmax + 256 * kOthers <= kTileThreads * 128, "more registers than the CTA is launched with");
+};
+template <int kRegs>
+__device__ __forceinline__ void give_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+struct TileSmem {
+  uint64_t q_full, kv_full[kTileStages], kv_empty[kTileStages], s_full[2], s_free, p_full[2][2], o_full[2], drain;
+  uint32_t tmem_base;
+  int abort_word;
+  int valid;                // this CTA has an item
+  int b, h, block, part, parts;
+  PagedSeq seq;
+  int first, last[2];       // tiles of 128 keys: [first, last[i]) of query tile i
+  long long off[3][kGather];       // byte offsets of a tile's rows in k and v (-1: zeros)
+  long long off_scale[3][kGather]; // of their scales
+};
+
+constexpr int kTileSmemBytes = 2 * kTileBytes + kTileStages * kTileBytes + 1024 /* alignment */ + (int)sizeof(TileSmem);
+static_assert(kTileSmemBytes <= 232448, "shared memory budget of one CTA");
+
+__device__ __forceinline__ int tiles_of(int keys) { return (keys + kBN - 1) / kBN; }
+
+// Tiles that rows up to `row` (inclusive) of a sequence see.
+__device__ __forceinline__ int visible_keys(const PagedAttnArgs& a, const PagedSeq& s, int row) {
+  return a.causal ? min(s.len, max(0, s.len - s.n + row / a.group + 1)) : s.len;
+}
+// Blocks of 256 rows of a sequence, and shares of the keys of each of its units.
+__device__ __forceinline__ int row_blocks(const PagedAttnArgs& a, const PagedSeq& s) {
+  const int rows = s.n * a.group;
+  return rows > a.few ? (rows + 2 * kBM - 1) / (2 * kBM) : 0;
+}
+__device__ __forceinline__ int key_shares(const PagedAttnArgs& a, const PagedSeq& s) {
+  return max(1, (tiles_of(s.len) + a.share_tiles - 1) / a.share_tiles);
+}
+
+// The item of this CTA: sequences one after the other; inside one, blocks of heads whose keys and values fit a part
+// of L2, in such a block the row blocks from the last (longest) to the first, then heads, then shares.  (One warp.)
+__device__ __forceinline__ void find_item(const PagedAttnArgs& a, TileSmem* ctl, int lane) {
+  int before = 0, found = 0;
+  const int want = blockIdx.x;
+  for (int b0 = 0; b0 < a.c.batch && !found; b0 += 32) {
+    const int b = b0 + lane;
+    PagedSeq s{0, 0, 0};
+    int items = 0;
+    if (b < a.c.batch) {
+      s = paged_seq(a.c, b, a.max_queries, a.max_keys);
+      items = row_blocks(a, s) * a.c.hkv * key_shares(a, s);
+    }
+    int incl = items;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += up;
+    }
+    incl += before;
+    const bool mine = want < incl && want >= incl - items;
+    if (mine) {
+      const int shares = key_shares(a, s), blocks = row_blocks(a, s);
+      int i = want - (incl - items);
+      ctl->part = i % shares;
+      i /= shares;
+      const long long head_bytes = max(1ll, (long long)s.len * a.head_bytes);
+      const int fit = (int)min((long long)a.c.hkv, max(1ll, (48ll << 20) / head_bytes));
+      const int hb = (a.c.hkv + (a.c.hkv + fit - 1) / fit - 1) / ((a.c.hkv + fit - 1) / fit);  // equal blocks
+      const int group = i / (hb * blocks), rem = i - group * hb * blocks;
+      const int n = min(hb, a.c.hkv - group * hb);
+      ctl->b = b;
+      ctl->h = group * hb + rem % n;
+      ctl->block = blocks - 1 - rem / n;
+      ctl->parts = shares;
+      ctl->seq = s;
+    }
+    found = __any_sync(0xffffffffu, mine);
+    before = __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (lane == 0) ctl->valid = found;
+}
+
+template <bool kFp8>
+__global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __grid_constant__ PagedAttnArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + 2 * kTileBytes;
+  TileSmem* ctl = reinterpret_cast<TileSmem*>(sKV + kTileStages * kTileBytes);
+  volatile int* abort_word = &ctl->abort_word;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  grid_dependents_launch();
+  grid_dependency_wait();
+  if (warp == 0) {
+    find_item(a, ctl, lane);
+    __syncwarp();
+    if (lane == 0) {
+      if (ctl->valid) {
+        const PagedSeq s = ctl->seq;
+        const int rows = s.n * a.group, row0 = ctl->block * 2 * kBM;
+        int n[2];
+        for (int i = 0; i < 2; ++i)
+          n[i] = row0 + i * kBM < rows ? tiles_of(visible_keys(a, s, min(row0 + (i + 1) * kBM, rows) - 1)) : 0;
+        const long long all = max(n[0], n[1]);
+        ctl->first = (int)(all * ctl->part / ctl->parts);
+        const int end = (int)(all * (ctl->part + 1) / ctl->parts);
+        ctl->last[0] = min(n[0], end);
+        ctl->last[1] = min(n[1], end);
+      }
+      // the merge finds a split unit at the CTA of its first share
+      if (a.tile_open != nullptr)
+        a.tile_open[blockIdx.x] = ctl->valid && ctl->part == 0 && ctl->parts > 1
+                                      ? make_int4(ctl->b, ctl->h, ctl->block, ctl->parts) : make_int4(0, 0, 0, 0);
+    }
+  } else if (warp == 1 && lane == 0) {
+    mbar_init(&ctl->q_full, kGather);
+    for (int s = 0; s < kTileStages; ++s) {
+      mbar_init(&ctl->kv_full[s], kGather);
+      mbar_init(&ctl->kv_empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl->s_full[i], 1);
+      mbar_init(&ctl->p_full[i][0], 128);
+      mbar_init(&ctl->p_full[i][1], 128);
+      mbar_init(&ctl->o_full[i], 1);
+    }
+    mbar_init(&ctl->s_free, 4);
+    mbar_init(&ctl->drain, 2);
+    ctl->abort_word = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+  if (!ctl->valid) return;
+  if (warp == 8) {
+    tmem_alloc(&ctl->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem_base;  // columns: S [0,128) P0 [128,192) P1 [192,256) O0 [256,384) O1 [384,512)
+  const int first = ctl->first, n0 = ctl->last[0], n1 = ctl->last[1], total = max(max(n0, n1) - first, 0);
+
+  if (warp >= 12) {
+    // ------------------------------------------------------------------ gather
+    give_registers<TileRegs<kFp8>::kOthers>();
+    const int r = tid - 12 * 32;
+    bool ok = true;  // (every thread goes through the same barriers, also after a wait ran out)
+    const int len = ctl->seq.len, hkv = ctl->h;
+    // queries: the rows' places, then the rows
+    {
+      const int rows = ctl->seq.n * a.group, row0 = ctl->block * 2 * kBM;
+      for (int i = 0; i < 2; ++i) {
+        const int row = row0 + i * kBM + r, tok = row / a.group, hd = row - tok * a.group;
+        ctl->off[i][r] = row < rows ? 2 * (ctl->b * a.q_sb + (long long)(ctl->seq.start + tok) * a.q_st +
+                                           (long long)(hkv * a.group + hd) * a.q_sh) : -1;
+      }
+      asm volatile("bar.sync 2, 128;" ::: "memory");
+      const int piece = r & 15;
+#pragma unroll 8
+      for (int i = 0; i < 32; ++i) {
+        const int row = (r >> 4) + 8 * (i & 15);
+        const long long from = ctl->off[i >> 4][row];
+        const uint32_t to = smem_u32(sQ) + (i >> 4) * kTileBytes + (piece >> 3) * kHalfBytes + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to),
+                     "l"(reinterpret_cast<const uint8_t*>(a.q) + (from >= 0 ? from + piece * 16 : 0)), "r"(from >= 0 ? 16 : 0) : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async_smem();
+      mbar_arrive(&ctl->q_full);
+      asm volatile("bar.sync 2, 128;" ::: "memory");  // the places are free again
+    }
+    // page of this thread's key of tile j
+    auto page_of = [&](int j) {
+      const int pos = (first + j) * kBN + r;
+      if (j >= total || pos >= len) return -1;
+      const int id = a.c.table[ctl->b * a.c.table_stride + page_index(a.c, pos)];
+      if (id < 0 || id >= a.c.pages) {
+        paged_error(a.c);
+        return -1;
+      }
+      return id;
+    };
+    auto put_place = [&](int j, int page) {
+      const int pos = (first + j) * kBN + r, slot = pos - page_index(a.c, pos) * a.c.page_size;
+      ctl->off[j % 3][r] = page >= 0 ? paged_offset(a.c, page, slot, hkv) : -1;
+      if constexpr (kFp8) ctl->off_scale[j % 3][r] = page >= 0 ? scale_offset(a.c, page, slot, hkv) : 0;
+    };
+    // Positions in the ring: K0 K1 V0 K2 V1 ... (tile, K or V) of position n
+    const int positions = 2 * total;
+    auto tile_of = [&](int n, int& which) {
+      if (n == 0) { which = 0; return 0; }
+      if (n == positions - 1) { which = 1; return total - 1; }
+      which = (n & 1) ^ 1;
+      return which ? n / 2 - 1 : (n + 1) / 2;
+    };
+    int page = page_of(0);
+    if constexpr (!kFp8) {
+      const int piece = r & 15, row0 = r >> 4;
+      const uint32_t col = (piece >> 3) * kHalfBytes;
+      int placed = 0;  // tiles whose places are in shared memory
+      for (int n = 0; n < positions; ++n) {
+        int which;
+        const int j = tile_of(n, which);
+        if (j == placed) {
+          put_place(j, page);
+          page = page_of(j + 1);
+          ++placed;
+          asm volatile("bar.sync 2, 128;" ::: "memory");
+        }
+        const int stage = n % kTileStages, round = n / kTileStages;
+        if (ok && round > 0) ok = mbar_wait(&ctl->kv_empty[stage], (round - 1) & 1, abort_word, MB_ERR_TIMEOUT_KV_EMPTY);
+        if (ok) {
+          const uint8_t* base = which ? a.c.v : a.c.k;
+          const uint32_t dst = smem_u32(sKV) + stage * kTileBytes + col;
+          const long long* off = ctl->off[j % 3];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int row = row0 + 8 * i;
+            const long long from = off[row];
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + row * 128 + (((piece & 7) ^ (row & 7)) << 4)),
+                         "l"(from >= 0 ? base + from + piece * 16 : base), "r"(from >= 0 ? 16 : 0) : "memory");
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (n >= 1) {
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          fence_proxy_async_smem();
+          mbar_arrive(&ctl->kv_full[(n - 1) % kTileStages]);
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async_smem();
+      if (positions > 0) mbar_arrive(&ctl->kv_full[(positions - 1) % kTileStages]);
+    } else {
+      const int piece = r & 7, row0 = r >> 3;
+      uint4 x[8];
+      uint32_t sc[8];
+      auto fetch = [&](int n, int i) {  // piece i of position n
+        int which;
+        const int j = tile_of(n, which), row = row0 + 16 * i;
+        const long long from = ctl->off[j % 3][row];
+        x[i] = make_uint4(0, 0, 0, 0);
+        sc[i] = 127;
+        if (from >= 0) {
+          x[i] = __ldg(reinterpret_cast<const uint4*>((which ? a.c.v : a.c.k) + from) + piece);
+          sc[i] = __ldg((which ? a.c.v_scale : a.c.k_scale) + ctl->off_scale[j % 3][row] + (piece >> 1));
+        }
+      };
+      int placed = 0;
+      auto place_up_to = [&](int j) {  // uniform over the warpgroup
+        if (j == placed && j < total) {
+          put_place(j, page);
+          page = page_of(j + 1);
+          ++placed;
+          asm volatile("bar.sync 2, 128;" ::: "memory");
+        }
+      };
+      place_up_to(0);
+      if (positions > 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) fetch(0, i);
+      }
+      for (int n = 0; n < positions; ++n) {
+        const int stage = n % kTileStages, round = n / kTileStages;
+        int which;
+        if (n + 1 < positions) place_up_to(tile_of(n + 1, which));
+        if (ok && round > 0) ok = mbar_wait(&ctl->kv_empty[stage], (round - 1) & 1, abort_word, MB_ERR_TIMEOUT_KV_EMPTY);
+        uint8_t* dst = sKV + stage * kTileBytes + (piece >> 2) * kHalfBytes;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = row0 + 16 * i;
+          const uint32_t mult = scale_mult(sc[i]);
+          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          uint32_t y[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[2 * e] = mul_bf16x2(e4m3_bits(__byte_perm(w[e], 0, 0x1404)), mult);
+            y[2 * e + 1] = mul_bf16x2(e4m3_bits(__byte_perm(w[e], 0, 0x3424)), mult);
+          }
+          if (n + 1 < positions) fetch(n + 1, i);
+          if (ok) {
+            // the lanes of a row store even pieces of one half and odd pieces of the other at a time: different banks
+            const int c0 = (2 * piece) & 7, swap = (piece >> 2) & 1;
+            uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
+            uint8_t* at = dst + row * 128;
+            *reinterpret_cast<uint4*>(at + (((c0 + swap) ^ (row & 7)) << 4)) = swap ? hi : lo;
+            *reinterpret_cast<uint4*>(at + (((c0 + 1 - swap) ^ (row & 7)) << 4)) = swap ? lo : hi;
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&ctl->kv_full[stage]);
+      }
+    }
+  } else if (warp == 9 || warp == 11) {
+    give_registers<TileRegs<kFp8>::kOthers>();
+  } else if (warp == 8 || warp == 10) {
+    // ------------------------------------------------------------------ tcgen05 issuers (see attn_fwd.cu)
+    give_registers<TileRegs<kFp8>::kOthers>();
+    if (total > 0) {
+      constexpr uint32_t kStageUnits = kTileBytes / 16;
+      bool ok = true;
+      if (warp == 8) {
+        constexpr uint32_t idesc_qk = umma_idesc_bf16(kBM, kBN, false, false);
+        const uint64_t q_desc = umma_smem_desc(smem_u32(sQ), 16, 1024);
+        const uint64_t k_desc0 = umma_smem_desc(smem_u32(sKV), 16, 1024);
+        int use = 0;
+        ok = mbar_wait_warp(&ctl->q_full, 0, abort_word, MB_ERR_TIMEOUT_Q);
+        for (int g = 0; g < total && ok; ++g) {
+          const int pos = g == 0 ? 0 : 2 * g - 1, stage = pos % kTileStages;
+          ok = mbar_wait_warp(&ctl->kv_full[stage], (pos / kTileStages) & 1, abort_word, MB_ERR_TIMEOUT_KV_FULL);
+          if (!ok) break;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (first + g < (i ? n1 : n0)) {
+              if (use > 0) {
+                ok = mbar_wait_warp(&ctl->s_free, (use - 1) & 1, abort_word, MB_ERR_TIMEOUT_S);
+                if (!ok) break;
+              }
+              tc_fence_after();
+              issue_qk(tmem, q_desc + i * kStageUnits, k_desc0 + stage * kStageUnits, idesc_qk);
+              umma_commit_elect(&ctl->s_full[i]);
+              ++use;
+            }
+          }
+          if (!ok) break;
+          umma_commit_elect(&ctl->kv_empty[stage]);
+        }
+      } else {
+        constexpr uint32_t idesc_pv = umma_idesc_bf16(kBM, kD, false, true);
+        const uint64_t v_desc0 = umma_smem_desc(smem_u32(sKV), kHalfBytes, 1024);
+        int cnt[2] = {0, 0};
+        for (int g = 0; g < total && ok; ++g) {
+          const int pos = g == total - 1 ? 2 * total - 1 : 2 * g + 2, stage = pos % kTileStages;
+          ok = mbar_wait_warp(&ctl->kv_full[stage], (pos / kTileStages) & 1, abort_word, MB_ERR_TIMEOUT_KV_FULL);
+          if (!ok) break;
+          const uint64_t v_desc = v_desc0 + stage * kStageUnits;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (first + g < (i ? n1 : n0)) {
+              const uint32_t tPi = tmem + 128 + i * 64, tOi = tmem + 256 + i * 128;
+              ok = mbar_wait_warp(&ctl->p_full[i][0], cnt[i] & 1, abort_word, MB_ERR_TIMEOUT_P);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv_half(tOi, tPi, v_desc, idesc_pv, cnt[i] == 0 ? 0u : 1u);
+              ok = mbar_wait_warp(&ctl->p_full[i][1], cnt[i] & 1, abort_word, MB_ERR_TIMEOUT_P);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv_half(tOi, tPi + 32, v_desc + 4 * 128, idesc_pv, 1u);
+              umma_commit_elect(&ctl->o_full[i]);
+              ++cnt[i];
+            }
+          }
+          if (!ok) break;
+          umma_commit_elect(&ctl->kv_empty[stage]);
+        }
+      }
+      if (!ok) {
+        // let tensor-core work already issued finish (bounded) before tensor memory is released
+        umma_commit_elect(&ctl->drain);
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&ctl->drain, 0) && clock64() - t0 < kWaitCycleLimit / 16) {
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax + epilogue
+    take_registers<TileRegs<kFp8>::kSoftmax>();
+    const int i = warp >> 2;                   // query tile
+    const int row = ((warp & 3) << 5) | lane;  // row inside the tile == tensor-memory lane
+    const uint32_t lane_field = static_cast<uint32_t>((warp & 3) << 5) << 16;
+    const uint32_t tS = tmem + lane_field;
+    const uint32_t tPi = tmem + 128 + i * 64 + lane_field;
+    const uint32_t tOi = tmem + 256 + i * 128 + lane_field;
+    const int tile_row = ctl->block * 2 * kBM + i * kBM;  // the tile's first row of the sequence
+    const int visible = visible_keys(a, ctl->seq, tile_row + row), visible_first = visible_keys(a, ctl->seq, tile_row);
+    const int last = i ? n1 : n0;
+
+    float m_ref = -INFINITY, l = 0.f;
+    int cnt = 0;
+    bool ok = true;
+    for (int jt = first; jt < last; ++jt) {
+      ok = mbar_wait_warp(&ctl->s_full[i], cnt & 1, abort_word, MB_ERR_TIMEOUT_S);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t sr[4][32];
+      tmem_ld32(tS + 0, sr[0]);
+      tmem_ld32(tS + 32, sr[1]);
+      tmem_ld32(tS + 64, sr[2]);
+      tmem_ld32(tS + 96, sr[3]);
+      tmem_wait_ld();
+      tc_fence_before();
+      mbar_arrive_elect(&ctl->s_free);  // the scores are in registers: the score region has its next user
+
+      const int k0 = jt * kBN;
+      if (k0 + kBN > visible_first) {  // some row of the tile does not see all of these keys
+        const int limit = visible - k0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c * 32 + e >= limit) sr[c][e] = 0xff800000u;  // -inf
+      }
+      float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        mx0 = max3(mx0, __uint_as_float(sr[0][e]), __uint_as_float(sr[0][e + 1]));
+        mx1 = max3(mx1, __uint_as_float(sr[1][e]), __uint_as_float(sr[1][e + 1]));
+        mx2 = max3(mx2, __uint_as_float(sr[2][e]), __uint_as_float(sr[2][e + 1]));
+        mx3 = max3(mx3, __uint_as_float(sr[3][e]), __uint_as_float(sr[3][e + 1]));
+      }
+      const float m_tile = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+      if (cnt == 0) {
+        m_ref = m_tile;
+      } else {
+        // the previous P V of this query tile must be complete before its probabilities are overwritten or O is rescaled
+        ok = mbar_wait_warp(&ctl->o_full[i], (cnt - 1) & 1, abort_word, MB_ERR_TIMEOUT_O);
+        if (!ok) break;
+        tc_fence_after();
+        const float m_new = fmaxf(m_ref, m_tile);
+        const bool need = (m_new - m_ref) * a.scale_log2 > kRescaleThreshold;
+        if (__any_sync(0xffffffffu, need)) {
+          const float f = need ? fast_exp2((m_ref - m_new) * a.scale_log2) : 1.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t orow[32];
+            tmem_ld32(tOi + c * 32, orow);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) orow[e] = __float_as_uint(__uint_as_float(orow[e]) * f);
+            tmem_st32(tOi + c * 32, orow);
+          }
+          tmem_wait_st();
+          if (need) {
+            l *= f;
+            m_ref = m_new;
+          }
+        }
+      }
+      const float m_scaled = (m_ref == -INFINITY) ? 0.f : m_ref * a.scale_log2;
+      const uint64_t c2 = pack2(a.scale_log2, a.scale_log2);
+      const uint64_t nm2 = pack2(-m_scaled, -m_scaled);
+      uint64_t sum_a = pack2(0.f, 0.f), sum_b = pack2(0.f, 0.f);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          const int c = half * 2 + cc;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const uint64_t x2 = fma2(pack2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1])), c2, nm2);
+            float x0, x1;
+            unpack2(x2, x0, x1);
+            const uint64_t p2 = pack2(fast_exp2(x0), fast_exp2(x1));
+            if ((e >> 1) & 1) sum_b = add2(sum_b, p2);
+            else sum_a = add2(sum_a, p2);
+            float p0, p1;
+            unpack2(p2, p0, p1);
+            pk[cc * 16 + (e >> 1)] = pack_bf16x2(p0, p1);
+          }
+        }
+        tmem_st32(tPi + half * 32, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&ctl->p_full[i][half]);
+      }
+      float s0, s1;
+      unpack2(add2(sum_a, sum_b), s0, s1);
+      l += s0 + s1;
+      ++cnt;
+    }
+
+    // epilogue; tiles whose rows all lie behind the sequence's skip it
+    const int rows = ctl->seq.n * a.group;
+    if (ok && tile_row < rows) {
+      if (cnt > 0) ok = mbar_wait_warp(&ctl->o_full[i], (cnt - 1) & 1, abort_word, MB_ERR_TIMEOUT_O);
+      if (ok) {
+        if (cnt > 0) tc_fence_after();
+        const bool store = tile_row + row < rows;
+        if (ctl->parts > 1) {
+          // a share: rows as they are, column group by column group (contiguous over a warp)
+          const int r = i * kBM + row;
+          if (cnt > 0) {
+            float4* dst = a.tile_o + (long long)blockIdx.x * (32 * 2 * kBM) + r;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t orow[32];
+              tmem_ld32(tOi + c * 32, orow);
+              tmem_wait_ld();
+#pragma unroll
+              for (int v = 0; v < 8; ++v)
+                dst[(c * 8 + v) * (2 * kBM)] =
+                    make_float4(__uint_as_float(orow[v * 4 + 0]), __uint_as_float(orow[v * 4 + 1]),
+                                __uint_as_float(orow[v * 4 + 2]), __uint_as_float(orow[v * 4 + 3]));
+            }
+          }
+          a.tile_ml[(long long)blockIdx.x * (2 * kBM) + r] = make_float2(m_ref, l);
+        } else {
+          const float inv = l == 0.f ? 0.f : a.out_scale / l;
+          const int tok = (tile_row + row) / a.group, hd = ctl->h * a.group + (tile_row + row) - tok * a.group;
+          __nv_bfloat16* optr = a.o + ctl->b * a.o_sb + (long long)(ctl->seq.start + tok) * a.o_st + (long long)hd * a.o_sh;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t orow[32];
+            if (cnt > 0) {
+              tmem_ld32(tOi + c * 32, orow);
+              tmem_wait_ld();
+            }
+            // a row that sees no key is zero, whatever its masked products gave
+            if (cnt == 0 || l == 0.f) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) orow[e] = 0u;
+            }
+            if (store) {
+              uint4* dst = reinterpret_cast<uint4*>(optr + c * 32);
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                uint4 w;
+                w.x = pack_bf16x2(__uint_as_float(orow[v * 8 + 0]) * inv, __uint_as_float(orow[v * 8 + 1]) * inv);
+                w.y = pack_bf16x2(__uint_as_float(orow[v * 8 + 2]) * inv, __uint_as_float(orow[v * 8 + 3]) * inv);
+                w.z = pack_bf16x2(__uint_as_float(orow[v * 8 + 4]) * inv, __uint_as_float(orow[v * 8 + 5]) * inv);
+                w.w = pack_bf16x2(__uint_as_float(orow[v * 8 + 6]) * inv, __uint_as_float(orow[v * 8 + 7]) * inv);
+                dst[v] = w;
+              }
+            }
+          }
+          if (store)
+            a.lse[ctl->b * a.lse_sb + hd * a.lse_sh + ctl->seq.start + tok] = l == 0.f ? -INFINITY : m_ref * a.scale + __logf(l);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (tid == 0 && ctl->abort_word != 0) atomicCAS(a.c.status, 0, ctl->abort_word);
+}
+
+// Joins the shares of the unit whose first share CTA blockIdx.x had (if there is one): 8 rows a block; warp w has columns
+// [16 w, 16 w + 16), a lane 4 of them of one row, so that the lanes of a column group read 128 contiguous bytes.
+constexpr int kTileMergeRows = 8;
+__global__ void __launch_bounds__(256) paged_tiles_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
+  const int lane = threadIdx.x & 31, chunk = (threadIdx.x >> 5) * 4 + (lane >> 3);
+  const int r = blockIdx.y * kTileMergeRows + (lane & 7);
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int4 unit = a.tile_open[blockIdx.x];
+  if (unit.w == 0) return;
+  const PagedSeq seq = paged_seq(a.c, unit.x, a.max_queries, a.max_keys);
+  const int row = unit.z * 2 * kBM + r;
+  if (row >= seq.n * a.group) return;
+  const float2* ml = a.tile_ml + (long long)blockIdx.x * (2 * kBM) + r;
+  const float4* src = a.tile_o + ((long long)blockIdx.x * 32 + chunk) * (2 * kBM) + r;
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int p = 0; p < unit.w; ++p) m = fmaxf(m, ml[p * 2 * kBM].x);
+  float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = 0; p < unit.w; ++p) {
+    const float2 s = ml[p * 2 * kBM];
+    if (s.y == 0.f) continue;  // a share without visible keys has stored no rows, or products of hidden keys
+    const float4 x = src[(long long)p * 32 * 2 * kBM];
+    const float w = s.x == -INFINITY ? 1.f : fast_exp2((s.x - m) * a.scale_log2);
+    l = fmaf(w, s.y, l);
+    acc[0] = fmaf(w, x.x, acc[0]);
+    acc[1] = fmaf(w, x.y, acc[1]);
+    acc[2] = fmaf(w, x.z, acc[2]);
+    acc[3] = fmaf(w, x.w, acc[3]);
+  }
+  const float inv = l == 0.f ? 0.f : a.out_scale / l;
+  const int tok = row / a.group, hd = unit.y * a.group + row - tok * a.group;
+  const uint2 o = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+  *reinterpret_cast<uint2*>(a.o + unit.x * a.o_sb + (long long)(seq.start + tok) * a.o_st + (long long)hd * a.o_sh + chunk * 4) = o;
+  if (chunk == 0) a.lse[unit.x * a.lse_sb + hd * a.lse_sh + seq.start + tok] = l == 0.f ? -INFINITY : m * a.scale + __logf(l);
+}
+
+long long paged_tiles_workspace(long long ctas) {
+  return ctas * (2ll * kBM * (kHeadDim * (long long)sizeof(float) + (long long)sizeof(float2)) + (long long)sizeof(int4));
+}
+
+template <bool kFp8>
+static int launch_tiles(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
+  static bool attr_set[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MB_E_CUDA;
+  if (!attr_set[dev]) {
+    if (!cuda_ok(cudaFuncSetAttribute(paged_tiles_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmemBytes),
+                 "paged_tiles_kernel shared memory"))
+      return MB_E_CUDA;
+    attr_set[dev] = true;
+  }
+  if (!launch_overlapped("launch paged_tiles_kernel", paged_tiles_kernel<kFp8>, dim3(ctas), kTileThreads, kTileSmemBytes, stream, a))
+    return MB_E_CUDA;
+  if (a.tile_open != nullptr &&
+      !launch_overlapped("launch paged_tiles_merge_kernel", paged_tiles_merge_kernel,
+                         dim3(ctas, (2 * kBM) / kTileMergeRows), 256, 0, stream, a))
+    return MB_E_CUDA;
+  return MB_SUCCESS;
+}
+
+int launch_paged_tiles(const PagedAttnArgs& a, bool fp8, int ctas, cudaStream_t stream) {
+  return fp8 ? launch_tiles<true>(a, ctas, stream) : launch_tiles<false>(a, ctas, stream);
+}
+
+}  // namespace mb

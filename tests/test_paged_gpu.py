@@ -181,3 +181,42 @@ def test_one_long_sequence_over_all_sms(fp8):
     assert torch.equal(o, o2) and torch.equal(lse, lse2)
     o_, lse_, mass, size = batch.expected(tensors, True)
     check(batch, o, lse, (o_, lse_, mass, size))
+
+
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads", [(1, 1), (8, 8), (8, 2), (14, 2), (16, 1)])
+def test_chunks_ragged(fp8, causal, heads):
+    """Chunks around the sizes of tiles beside single tokens and nothing: both kernels in one call."""
+    lens = [1, 64, 300, 128, 129, 0, 257, 1000, 40, 5]
+    new = [1, 64, 7, 128, 127, 0, 257, 33, 90, 0]  # the ninth has more new tokens than keys
+    batch = Batch(lens, new, heads, 16, fp8, seed=7, spread=2.0)
+    tensors = batch.cache_tensors()
+    o, lse = _attend(batch, _cache(batch, tensors), causal)
+    assert _status() == 0
+    check(batch, o, lse, batch.expected(tensors, causal))
+
+
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("page", [1, 7, 24, 128, 1000])
+def test_chunks_page_sizes(fp8, page):
+    batch = Batch([513, 90, 1200], [100, 90, 270], (8, 2), page, fp8, seed=8)
+    tensors = batch.cache_tensors()
+    o, lse = _attend(batch, _cache(batch, tensors))
+    assert _status() == 0
+    check(batch, o, lse, batch.expected(tensors, True))
+
+
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("lens,new,heads", [([5000], [64], (8, 2)), ([4000, 100], [150, 150], (4, 4)), ([3000], [1500], (2, 1)),
+                                            ([20000], [40], (4, 4))])
+def test_chunks_split_over_keys(fp8, lens, new, heads):
+    """Few units against many keys: shares and their merge; bits repeat."""
+    batch = Batch(lens, new, heads, 64, fp8, ragged=False, seed=9, spread=2.0)
+    tensors = batch.cache_tensors()
+    cache = _cache(batch, tensors)
+    o, lse = _attend(batch, cache)
+    o2, lse2 = _attend(batch, cache)
+    assert _status() == 0
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    check(batch, o, lse, batch.expected(tensors, True))
