@@ -99,10 +99,7 @@ int launch_attn_paged(const mb_attn_paged_args* x, void* ws, unsigned long long 
   a.max_keys = x->max_keys;
   a.causal = x->causal ? 1 : 0;
   const bool fp8 = x->kv.dtype == MB_DTYPE_E4M3;
-  const float unbias = fp8 ? (float)(1ull << kScaleBias) : 1.f;
-  a.scale = x->softmax_scale * unbias;
-  a.scale_log2 = x->softmax_scale * 1.4426950408889634f * unbias;
-  a.out_scale = unbias;
+  a.scale_log2 = x->softmax_scale * 1.4426950408889634f;
   a.few = p.few;
   a.share_tiles = max(p.share_tiles, 1);
   a.head_bytes = fp8 ? 2 * kHeadDim : 4 * kHeadDim;

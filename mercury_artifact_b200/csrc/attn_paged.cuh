@@ -14,8 +14,7 @@ struct PagedAttnArgs {
   float* lse;
   long long lse_sb, lse_sh;
   int hq, group, max_queries, max_keys, causal;
-  float scale, scale_log2;  // of the raw scores that the products give (the bias of e4m3 values taken out)
-  float out_scale;          // of the raw sums of values
+  float scale_log2;  // softmax scale * log2(e): maxima are kept in units of the exponent of two
   // rows of a sequence: new tokens x heads of a group.  Sequences with at most `few` rows belong to the kernel for
   // few rows, the others to the kernel for tiles.
   int few;
@@ -33,6 +32,8 @@ struct PagedAttnArgs {
   float2* tile_ml;
   int4* tile_open;
 };
+
+constexpr float kLn2 = 0.6931471805599453f;
 
 int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream);
 long long paged_rows_workspace(int rows, int ctas);

@@ -40,6 +40,7 @@ struct RowSmem {
   int total, warp_sum[kRowWarps];
   int b, step;                               // where this CTA's part starts: sequence, and step inside it
   float2 ml[kRowWarps][32];
+  float q_scale[32];  // e4m3: power of two that a row of queries was divided by
 };
 
 template <bool kFp8>
@@ -48,17 +49,6 @@ constexpr int row_smem_bytes() {
   return kRowWarps * kRowStages * RowShape<kFp8>::kStage + 32 * 2 * kHeadDim + 32 * RowShape<kFp8>::kPitch * 4 + (int)sizeof(RowSmem);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kLeft>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -67,10 +57,16 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+template <bool kF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if constexpr (kF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // A place in the list of steps.
@@ -154,6 +150,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   uint8_t* queries = smem_raw + kRowWarps * kRowStages * S::kStage;  // rows of 256 bytes, pieces swapped like the keys'
   float* merge = reinterpret_cast<float*>(queries + 32 * 2 * kHeadDim);
   RowSmem* sm = reinterpret_cast<RowSmem*>(merge + 32 * S::kPitch);
+  // e4m3: a step's powers of two in f16, twice [32 keys][4 blocks] for the keys, [4 blocks][32 keys] for the values; where
+  // the states are merged at a unit's end
+  uint32_t* key_scale = reinterpret_cast<uint32_t*>(merge) + warp * 192;
+  uint16_t* value_scale = reinterpret_cast<uint16_t*>(key_scale + 128);
   const uint32_t stage0 = smem_u32(stages);
 
   grid_dependents_launch();
@@ -196,22 +196,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   in.step = sm->step - in.h * in.steps;
   RowIter at = in;  // what is computed next
 
-  // page of this lane's key of the step to load, fetched one step ahead
-  auto page_of = [&](const RowIter& it) {
+  // the page table's entry for this lane's key of the step to load, fetched one step ahead
+  auto entry_of = [&](const RowIter& it) {
     const int pos = it.step * kStep + warp * kKeys + (lane & (kKeys - 1));
-    if (pos >= it.s.len) return -1;
-    const int id = a.c.table[it.b * a.c.table_stride + page_index(a.c, pos)];
-    if (id < 0 || id >= a.c.pages) {
-      paged_error(a.c);
-      return -1;
-    }
-    return id;
+    return pos < it.s.len ? paged_entry(a.c, it.b, pos) : 0;
   };
-  int page = page_of(in);
+  int entry = entry_of(in);
 
   auto load = [&](int stage) {
     const int pos = in.step * kStep + warp * kKeys + (lane & (kKeys - 1));
     const int slot = pos - page_index(a.c, pos) * a.c.page_size;
+    const int page = pos < in.s.len ? paged_id(a.c, entry, -1) : -1;
     const long long off = page >= 0 ? paged_offset(a.c, page, slot, in.h) : -1;
     const uint32_t dst = stage0 + stage * S::kStage;
 #pragma unroll
@@ -237,7 +232,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       load(i);
       if (--to_load > 0) {
         next_step<kStep>(a, in);
-        page = page_of(in);
+        entry = entry_of(in);
       }
     }
     cp_async_commit();
@@ -270,6 +265,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     for (int m = 0; m < kTiles; ++m) {
       const int r = m * 16 + (tid >> 4), piece = tid & 15;
       uint8_t* row = queries + r * 2 * kHeadDim;
+      if constexpr (kFp8) {
+        const float scale = query_to_f16(qx[m]);
+        if (piece == 0) sm->q_scale[r] = scale;
+      }
       if constexpr (!kFp8) {
         *reinterpret_cast<uint4*>(row + ((piece ^ (r & 7)) << 4)) = qx[m];
       } else {
@@ -284,7 +283,14 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   };
 
   float acc[kTiles][16][4], m_ref[kTiles][2], l[kTiles][2];
-  int limit[kTiles][2];  // keys that the row sees
+  int limit[kTiles][2];        // keys that the row sees
+  float row_scale[kTiles][2];  // e4m3: power of two of the row's queries
+  auto row_scales = [&]() {
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) row_scale[m][half] = kFp8 ? sm->q_scale[m * 16 + half * 8 + g] : 1.f;
+  };
   auto begin_unit = [&]() {
     store_q();
     next_unit();
@@ -307,6 +313,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   fetch_q();
   begin_unit();
   __syncthreads();
+  row_scales();
 
   bool from_start = at.step == 0;  // the unit's earlier steps are not another CTA's
   int stage = 0;
@@ -316,7 +323,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       load(stage == 0 ? kRowStages - 1 : stage - 1);
       if (--to_load > 0) {
         next_step<kStep>(a, in);
-        page = page_of(in);
+        entry = entry_of(in);
       }
     }
     cp_async_commit();
@@ -333,6 +340,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       for (int j = 0; j < kBlocks; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[m][j][e] = 0.f;
+    float step_scale = a.scale_log2;  // of the step's scores; e4m3: with the keys' power of two
+    int value_exp = 0;                // exponent of the power of two that the values were divided by
     if constexpr (!kFp8) {
       // four 8 x 8 matrices: keys 0-7 and 8-15 x two 16-byte pieces
       const int row = (lane & 7) + ((lane >> 4) << 3), odd = (lane >> 3) & 1;
@@ -344,18 +353,35 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         for (int m = 0; m < kTiles; ++m) {
           uint32_t qf[4];
           query(qf, m, k);
-          mma16816(sc[m][0], qf, b[0], b[1]);
-          mma16816(sc[m][1], qf, b[2], b[3]);
+          mma16816<kFp8>(sc[m][0], qf, b[0], b[1]);
+          mma16816<kFp8>(sc[m][1], qf, b[2], b[3]);
         }
       }
     } else {
-      // four matrices: the 32 keys x one piece of 16 values
-      const uint8_t* ks = stages + stage * S::kStage + 2 * S::kHalf;
-      uint32_t kb[kBlocks];
+      // The powers of two of this lane's key, relative to the largest of the step
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(stages + stage * S::kStage + 2 * S::kHalf);
+      const uint32_t kw = words[lane], vw = words[kKeys + lane];
+      const int k_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(kw)), kMinScale);
+      const int v_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(vw)), kMinScale);
+      uint32_t ks[4];
 #pragma unroll
-      for (int j = 0; j < kBlocks; ++j) kb[j] = *reinterpret_cast<const uint32_t*>(ks + (j * 8 + g) * 4);
+      for (int b = 0; b < 4; ++b) {
+        const float k2 = scale_relative((kw >> (8 * b)) & 0xffu, k_top);
+        ks[b] = pack_f16x2(k2, k2);
+        value_scale[b * kKeys + lane] = (uint16_t)pack_f16x2(scale_relative((vw >> (8 * b)) & 0xffu, v_top), 0.f);
+      }
+      *reinterpret_cast<uint4*>(key_scale + lane * 4) = make_uint4(ks[0], ks[1], ks[2], ks[3]);
+      __syncwarp();
+      step_scale = a.scale_log2 * exp2_int(k_top - 127);
+      value_exp = v_top - 127;
+      // four matrices: the 32 keys x one piece of 16 values
+      uint32_t mult[kBlocks];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
+        if ((k & 1) == 0) {
+#pragma unroll
+          for (int j = 0; j < kBlocks; ++j) mult[j] = key_scale[(j * 8 + g) * 4 + (k >> 1)];
+        }
         uint32_t b[4];
         ldsm4(b, sk + lane * S::kRowBytes + ((k ^ (lane & 7)) << 4));
         uint32_t qf[kTiles][4];
@@ -363,27 +389,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         for (int m = 0; m < kTiles; ++m) query(qf[m], m, k);
 #pragma unroll
         for (int j = 0; j < kBlocks; ++j) {
-          const uint32_t mult = ((((kb[j] >> (8 * (k >> 1))) & 0xffu) + kScaleAdd) << 7) * 0x10001u;
-          const uint32_t b0 = mul_bf16x2(e4m3_bits(__byte_perm(b[j], 0, 0x1404)), mult);
-          const uint32_t b1 = mul_bf16x2(e4m3_bits(__byte_perm(b[j], 0, 0x3424)), mult);
+          const uint32_t b0 = mul_f16x2(e4m3_f16(b[j]), mult[j]), b1 = mul_f16x2(e4m3_f16_high(b[j]), mult[j]);
 #pragma unroll
-          for (int m = 0; m < kTiles; ++m) mma16816(sc[m][j], qf[m], b0, b1);
+          for (int m = 0; m < kTiles; ++m) mma16816<kFp8>(sc[m][j], qf[m], b0, b1);
         }
-      }
-      // scale bytes beyond the written range: the key's scores are not numbers
-      uint32_t odd = 0;
-#pragma unroll
-      for (int j = 0; j < kBlocks; ++j) odd |= kb[j] & (kb[j] << 1) & 0x80808080u;
-      if (__any_sync(0xffffffffu, odd != 0)) {
-#pragma unroll
-        for (int j = 0; j < kBlocks; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(ks + (j * 8 + 2 * t + (e & 1)) * 4);
-            if (w & (w << 1) & 0x80808080u)
-#pragma unroll
-              for (int m = 0; m < kTiles; ++m) sc[m][j][e] = __int_as_float(0x7fffffff);
-          }
       }
     }
 
@@ -404,15 +413,23 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
         top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
       }
-      // The reference maximum only moves when a score exceeds it by 2^8 in the exponentials' scale.
-      const bool need0 = (top[0] - m_ref[m][0]) * a.scale_log2 > 8.f, need1 = (top[1] - m_ref[m][1]) * a.scale_log2 > 8.f;
-      if (__any_sync(0xffffffffu, need0 || need1)) {
+      // A row's reference is the exponent of its largest term exp2(score) * 2^value_exp; it only moves when a term
+      // exceeds it by 2^8.
+      float c[2], lift[2];
+      bool need[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        // (not zero, with which hidden scores would make no number)
+        c[half] = kFp8 ? fmaxf(step_scale * row_scale[m][half], 1.2e-38f) : step_scale;
+        top[half] = top[half] == -INFINITY ? -INFINITY : fmaf(top[half], c[half], (float)value_exp);
+        need[half] = top[half] - m_ref[m][half] > 8.f;
+      }
+      if (__any_sync(0xffffffffu, need[0] || need[1])) {
         float f[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const bool need = half ? need1 : need0;
-          f[half] = need ? fast_exp2((m_ref[m][half] - top[half]) * a.scale_log2) : 1.f;
-          if (need) m_ref[m][half] = top[half];
+          f[half] = need[half] ? fast_exp2(m_ref[m][half] - top[half]) : 1.f;
+          if (need[half]) m_ref[m][half] = top[half];
           l[m][half] *= f[half];
         }
 #pragma unroll
@@ -420,19 +437,27 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[m][j][e] *= f[e >> 1];
       }
-      const float ms[2] = {m_ref[m][0] == -INFINITY ? 0.f : m_ref[m][0] * a.scale_log2,
-                           m_ref[m][1] == -INFINITY ? 0.f : m_ref[m][1] * a.scale_log2};
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) lift[half] = (float)value_exp - (m_ref[m][half] == -INFINITY ? 0.f : m_ref[m][half]);
 #pragma unroll
       for (int j = 0; j < kBlocks; ++j) {
         float p[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p[e] = fast_exp2(fmaf(sc[m][j][e], a.scale_log2, -ms[e >> 1]));
-          l[m][e >> 1] += p[e];
+          p[e] = fast_exp2(fmaf(sc[m][j][e], c[e >> 1], lift[e >> 1]));
+          sum[e >> 1] += p[e];
         }
-        pf[m][j >> 1][(j & 1) * 2 + 0] = pack_bf16x2(p[0], p[1]);
-        pf[m][j >> 1][(j & 1) * 2 + 1] = pack_bf16x2(p[2], p[3]);
+        if constexpr (kFp8) {
+          pf[m][j >> 1][(j & 1) * 2 + 0] = pack_f16x2(p[0], p[1]);
+          pf[m][j >> 1][(j & 1) * 2 + 1] = pack_f16x2(p[2], p[3]);
+        } else {
+          pf[m][j >> 1][(j & 1) * 2 + 0] = pack_bf16x2(p[0], p[1]);
+          pf[m][j >> 1][(j & 1) * 2 + 1] = pack_bf16x2(p[2], p[3]);
+        }
       }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) l[m][half] = kFp8 ? fmaf(sum[half], exp2_int(-value_exp), l[m][half]) : l[m][half] + sum[half];
     }
 
     // ---- values
@@ -444,56 +469,37 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         ldsm4_t(b, sv + row * S::kRowBytes + (((j + odd) ^ (row & 7)) << 4));
 #pragma unroll
         for (int m = 0; m < kTiles; ++m) {
-          mma16816(acc[m][j], pf[m][0], b[0], b[1]);
-          mma16816(acc[m][j + 1], pf[m][0], b[2], b[3]);
+          mma16816<kFp8>(acc[m][j], pf[m][0], b[0], b[1]);
+          mma16816<kFp8>(acc[m][j + 1], pf[m][0], b[2], b[3]);
         }
       }
     } else {
       // Transposed 16-bit units are pairs of neighbouring values: a lane gets values (2 g, 2 g + 1) of keys (2 t, 2 t + 1) of
       // each 8; the even ones make one 8-column block of the product and the odd ones the next.
-      const uint8_t* vs = stages + stage * S::kStage + 2 * S::kHalf + S::kScaleBytes;
-      uint2 vb[kBlocks];
-#pragma unroll
-      for (int j = 0; j < kBlocks; ++j) vb[j] = *reinterpret_cast<const uint2*>(vs + (j * 8 + 2 * t) * 4);
       uint32_t mult[kBlocks];
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         if ((c & 1) == 0) {
 #pragma unroll
-          for (int j = 0; j < kBlocks; ++j) {
-            const uint32_t two = __byte_perm(vb[j].x, vb[j].y, (c >> 1) | ((4 + (c >> 1)) << 4));  // bytes 0 and 1
-            mult[j] = (((two & 0xffu) | ((two & 0xff00u) << 8)) + kScaleAdd * 0x10001u) << 7;
-          }
+          for (int j = 0; j < kBlocks; ++j)
+            mult[j] = *reinterpret_cast<const uint32_t*>(value_scale + (c >> 1) * kKeys + j * 8 + 2 * t);
         }
         uint32_t b[4];
         ldsm4_t(b, sv + lane * S::kRowBytes + ((c ^ (lane & 7)) << 4));
         uint32_t even[4], odd[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          even[j] = mul_bf16x2(e4m3_bits(__byte_perm(b[j], 0, 0x2404)), mult[j]);
-          odd[j] = mul_bf16x2(e4m3_bits(__byte_perm(b[j], 0, 0x3414)), mult[j]);
+          const uint32_t x = __byte_perm(b[j], 0, 0x3120);  // the even ones of both keys, then the odd ones
+          even[j] = mul_f16x2(e4m3_f16(x), mult[j]);
+          odd[j] = mul_f16x2(e4m3_f16_high(x), mult[j]);
         }
 #pragma unroll
         for (int m = 0; m < kTiles; ++m) {
-          mma16816(acc[m][2 * c], pf[m][0], even[0], even[1]);
-          mma16816(acc[m][2 * c + 1], pf[m][0], odd[0], odd[1]);
-          mma16816(acc[m][2 * c], pf[m][1], even[2], even[3]);
-          mma16816(acc[m][2 * c + 1], pf[m][1], odd[2], odd[3]);
+          mma16816<kFp8>(acc[m][2 * c], pf[m][0], even[0], even[1]);
+          mma16816<kFp8>(acc[m][2 * c + 1], pf[m][0], odd[0], odd[1]);
+          mma16816<kFp8>(acc[m][2 * c], pf[m][1], even[2], even[3]);
+          mma16816<kFp8>(acc[m][2 * c + 1], pf[m][1], odd[2], odd[3]);
         }
-      }
-      uint32_t bad = 0;  // by scale block
-#pragma unroll
-      for (int j = 0; j < kBlocks; ++j) bad |= (vb[j].x & (vb[j].x << 1) & 0x80808080u) | (vb[j].y & (vb[j].y << 1) & 0x80808080u);
-      if (__any_sync(0xffffffffu, bad != 0)) {
-        bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
-        bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (bad & (0x80u << (8 * (j >> 2))))
-#pragma unroll
-            for (int m = 0; m < kTiles; ++m)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[m][j][e] = __int_as_float(0x7fffffff);
       }
     }
     __syncwarp();
@@ -524,7 +530,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm->ml[w][m * 16 + half * 8 + g].x);
-        f[m][half] = m_ref[m][half] == -INFINITY ? 0.f : fast_exp2((m_ref[m][half] - top) * a.scale_log2);
+        f[m][half] = m_ref[m][half] == -INFINITY ? 0.f : fast_exp2(m_ref[m][half] - top);
         // a warp without a visible key has nothing, whatever its masked products gave
         if (m_ref[m][half] == -INFINITY && !(l[m][half] != l[m][half])) {
 #pragma unroll
@@ -580,7 +586,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
 #pragma unroll
       for (int w = 0; w < kRowWarps; ++w) {
         const float2 x = sm->ml[w][r];
-        sum += x.x == -INFINITY ? x.y : x.y * fast_exp2((x.x - top) * a.scale_log2);
+        sum += x.x == -INFINITY ? x.y : x.y * fast_exp2(x.x - top);
       }
       float4 x = *reinterpret_cast<const float4*>(merge + r * S::kPitch + lane * 4);
       if constexpr (kTiles == 1) {
@@ -589,11 +595,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       }
       if (whole) {
         const int tok = r / a.group, hd = at.h * a.group + r - tok * a.group;
-        const float inv = sum == 0.f ? 0.f : a.out_scale / sum;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const uint2 w = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
         *reinterpret_cast<uint2*>(a.o + at.b * a.o_sb + (long long)(at.s.start + tok) * a.o_st + (long long)hd * a.o_sh + lane * 4) = w;
         if (lane == 0)
-          a.lse[at.b * a.lse_sb + hd * a.lse_sh + at.s.start + tok] = sum == 0.f ? -INFINITY : top * a.scale + __logf(sum);
+          a.lse[at.b * a.lse_sb + hd * a.lse_sh + at.s.start + tok] = sum == 0.f ? -INFINITY : top * kLn2 + __logf(sum);
       } else {
         *reinterpret_cast<float4*>(a.part_o + ((long long)slot * (16 * kTiles) + r) * kHeadDim + lane * 4) = x;
         if (lane == 0) a.part_ml[slot * (16 * kTiles) + r] = make_float2(top, sum);
@@ -610,7 +616,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       at = nx;
       from_start = true;
       begin_unit();
-      __syncthreads();  // the buffers are free again
+      __syncthreads();  // the buffers are free again, the queries there
+      row_scales();
     }
   }
 }
@@ -642,7 +649,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_merge_kernel(const __grid_c
     const float2 ml = a.part_ml[slot(p)];
     const float4 y = *reinterpret_cast<const float4*>(a.part_o + slot(p) * kHeadDim + lane * 4);
     // (a part without visible keys holds zeros, or what is not a number)
-    const float w = ml.x == -INFINITY ? 1.f : fast_exp2((ml.x - top) * a.scale_log2);
+    const float w = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top);
     sum = fmaf(w, ml.y, sum);
     x.x = fmaf(w, y.x, x.x);
     x.y = fmaf(w, y.y, x.y);
@@ -660,10 +667,10 @@ __global__ void __launch_bounds__(kRowThreads) paged_merge_kernel(const __grid_c
     x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
   }
   const int tok = seq.start + r / a.group, hd = unit.y * a.group + r % a.group;
-  const float inv = sum == 0.f ? 0.f : a.out_scale / sum;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const uint2 w = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
   *reinterpret_cast<uint2*>(a.o + unit.x * a.o_sb + (long long)tok * a.o_st + (long long)hd * a.o_sh + lane * 4) = w;
-  if (lane == 0) a.lse[unit.x * a.lse_sb + hd * a.lse_sh + tok] = sum == 0.f ? -INFINITY : top * a.scale + __logf(sum);
+  if (lane == 0) a.lse[unit.x * a.lse_sb + hd * a.lse_sh + tok] = sum == 0.f ? -INFINITY : top * kLn2 + __logf(sum);
 }
 
 int paged_rows_ctas() { return sm_count(); }

@@ -7,15 +7,21 @@
 // per row, probabilities in bf16 as the tensor-memory operand of O += P V.
 //
 // What differs is how keys and values arrive.  A page may end anywhere inside a tile, pages lie anywhere, and
-// the slots behind a sequence's end hold anything, so that a warpgroup of four warps gathers each tile row by row:
-// bf16 with cp.async, 16 bytes a piece, straight into the swizzled layout that tcgen05 reads; e4m3 through registers,
-// where a code becomes code * 2^n in bf16 on the way (see paged_common.cuh), one tile ahead.  Rows behind the end are
-// filled with zeros.
+// the slots behind a sequence's end hold anything (values that are not numbers among it).  Three ways:
+//   kBoxes   bf16, pages of a multiple of 8 slots: TMA boxes of the largest power of two of slots that divides a page; boxes
+//            behind the end are fetched from behind the last page, which fills in zeros, and the rows of the
+//            last box that lie behind the end are cleared before the values are used (hidden scores are replaced anyway).
+//   kRows    bf16, other pages: four more warps gather row by row with cp.async, 16 bytes a piece, straight into the
+//            swizzled layout that tcgen05 reads.
+//   kCodes   e4m3: two warps gather codes row by row with cp.async, up to three tiles ahead, and those four turn them into
+//            f16 (see paged_common.cuh) on their way from one place in shared memory to another.  Scores and
+//            probabilities of a tile are then in units of the tile's largest power of two, which goes into the scale of
+//            the scores and into the exponents.
 //
 //   warps 0-3   softmax + epilogue of query tile 0 (one thread per row)
-//   warps 4-7   softmax + epilogue of query tile 1
-//   warp  8     issues Q K^T, owns tensor memory;  warp 10 issues P V;  warps 9 and 11 idle
-//   warps 12-15 gather queries, keys and values
+//   warps 4-7   softmax + epilogue of query tile 1; warps 0-7 also gather the queries
+//   warp  8     issues Q K^T, owns tensor memory;  warp 10 issues P V;  warps 9 and 11 issue TMA (kBoxes) or gather codes
+//   warps 12-15 gather keys and values (kRows), turn codes into f16 (kCodes)
 //
 // A launch has one CTA per (sequence, 256 rows, K/V head, share of the keys), found on the device from the lengths that
 // are there; CTAs beyond the last of them return.  Shares leave their unnormalised rows, maxima and sums in
@@ -25,15 +31,20 @@
 
 namespace mb {
 
-constexpr int kTileThreads = 512;
-constexpr int kTileStages = 4;
-constexpr int kGather = 128;  // threads that gather
-// Registers of the softmax warps and of the others, out of 128 a thread at launch (an increase beyond that pool would block
-// forever, hence the check).
-template <bool kFp8>
-struct TileRegs {
-  static constexpr int kSoftmax = kFp8 ? 200 : 208, kOthers = kFp8 ? 56 : 48;
-  static_assert(256 * kSoftmax + 256 * kOthers <= kTileThreads * 128, "more registers than the CTA is launched with");
+enum TileMode { kBoxes, kRows, kCodes };
+
+// Threads; registers at launch, of the softmax warps and of the others (an increase beyond what the CTA was launched with
+// would block forever, hence the check).  Stages of 32 KiB in bf16; of codes, 16 KiB.
+template <int kMode>
+struct TileShape {
+  static constexpr int kGather = kMode == kBoxes ? 0 : 128;  // threads of warps 12-15
+  static constexpr int kThreads = 384 + kGather;
+  static constexpr int kLaunch = kMode == kBoxes ? 160 : 128;
+  static constexpr int kSoftmax = kMode == kBoxes ? 216 : 208, kOthers = 48;
+  static_assert(256 * kSoftmax + (kThreads - 256) * kOthers <= kThreads * kLaunch, "more registers than the CTA is launched with");
+  static constexpr int kStages = kMode == kCodes ? 3 : 4;
+  static constexpr int kCodeStages = kMode == kCodes ? 3 : 0;
+  static constexpr int kCodeStage = kBN * kHeadDim;
 };
 template <int kRegs>
 __device__ __forceinline__ void give_registers() {
@@ -44,20 +55,39 @@ __device__ __forceinline__ void take_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
+// Instruction descriptor of a product of 128 rows: bf16, or f16 (both operands alike), fp32 sums.
+template <int kMode>
+__host__ __device__ constexpr uint32_t tile_idesc(int n, bool b_mn_major) {
+  return umma_idesc_bf16(kBM, n, false, b_mn_major) & ~(kMode == kCodes ? (1u << 7) | (1u << 10) : 0u);
+}
+
+struct TileMaps {
+  CUtensorMap k, v;
+  int box;  // slots of a box
+};
+
 struct TileSmem {
-  uint64_t q_full, kv_full[kTileStages], kv_empty[kTileStages], s_full[2], s_free, p_full[2][2], o_full[2], drain;
+  uint64_t q_full, kv_full[4], kv_empty[4], s_full[2], s_free, p_full[2][2], o_full[2], drain, tail, codes_full[3], codes_empty[3];
   uint32_t tmem_base;
   int abort_word;
   int valid;                // this CTA has an item
   int b, h, block, part, parts;
   PagedSeq seq;
   int first, last[2];       // tiles of 128 keys: [first, last[i]) of query tile i
-  long long off[3][kGather];       // byte offsets of a tile's rows in k and v (-1: zeros)
-  long long off_scale[3][kGather]; // of their scales
+  long long off[3][kBN];       // byte offsets of a tile's rows in k and v (-1: zeros)
+  // e4m3: scale bytes of the keys and values of a tile; exponents of their largest; power of two of a row of queries
+  uint32_t scales[4][2][kBN];
+  int warp_top[4][2][2];  // largest scale byte of half of the rows
+  int top[8][2];
+  float q_scale[2 * kBM];
 };
 
-constexpr int kTileSmemBytes = 2 * kTileBytes + kTileStages * kTileBytes + 1024 /* alignment */ + (int)sizeof(TileSmem);
-static_assert(kTileSmemBytes <= 232448, "shared memory budget of one CTA");
+template <int kMode>
+constexpr int tile_smem_bytes() {
+  return (2 + TileShape<kMode>::kStages) * kTileBytes + TileShape<kMode>::kCodeStages * TileShape<kMode>::kCodeStage +
+         1024 /* alignment */ + (int)sizeof(TileSmem);
+}
+static_assert(tile_smem_bytes<kRows>() <= 232448 && tile_smem_bytes<kCodes>() <= 232448, "shared memory budget of one CTA");
 
 __device__ __forceinline__ int tiles_of(int keys) { return (keys + kBN - 1) / kBN; }
 
@@ -117,13 +147,17 @@ __device__ __forceinline__ void find_item(const PagedAttnArgs& a, TileSmem* ctl,
   if (lane == 0) ctl->valid = found;
 }
 
-template <bool kFp8>
-__global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __grid_constant__ PagedAttnArgs a) {
+template <int kMode>
+__global__ void __maxnreg__(TileShape<kMode>::kLaunch)
+paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ PagedAttnArgs a) {
+  using Shape = TileShape<kMode>;
+  constexpr int kStages = Shape::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sKV = smem + 2 * kTileBytes;
-  TileSmem* ctl = reinterpret_cast<TileSmem*>(sKV + kTileStages * kTileBytes);
+  uint8_t* sCodes = sKV + kStages * kTileBytes;
+  TileSmem* ctl = reinterpret_cast<TileSmem*>(sCodes + Shape::kCodeStages * Shape::kCodeStage);
   volatile int* abort_word = &ctl->abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -151,9 +185,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
                                       ? make_int4(ctl->b, ctl->h, ctl->block, ctl->parts) : make_int4(0, 0, 0, 0);
     }
   } else if (warp == 1 && lane == 0) {
-    mbar_init(&ctl->q_full, kGather);
-    for (int s = 0; s < kTileStages; ++s) {
-      mbar_init(&ctl->kv_full[s], kGather);
+    mbar_init(&ctl->q_full, 256);
+    mbar_init(&ctl->tail, 1);
+    for (int s = 0; s < Shape::kCodeStages; ++s) {
+      mbar_init(&ctl->codes_full[s], 128);  // of 64 threads, when their copies are there and when their other stores are
+      mbar_init(&ctl->codes_empty[s], 128);
+    }
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&ctl->kv_full[s], kMode == kBoxes ? 1 : Shape::kGather);
       mbar_init(&ctl->kv_empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -180,174 +219,281 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
   const uint32_t tmem = ctl->tmem_base;  // columns: S [0,128) P0 [128,192) P1 [192,256) O0 [256,384) O1 [384,512)
   const int first = ctl->first, n0 = ctl->last[0], n1 = ctl->last[1], total = max(max(n0, n1) - first, 0);
 
+  if (warp < 8 && total > 0) {
+    // queries: sixteen lanes have a row
+    const int rows = ctl->seq.n * a.group, row0 = ctl->block * 2 * kBM, piece = tid & 15;
+    const __nv_bfloat16* q = a.q + ctl->b * a.q_sb + ctl->seq.start * a.q_st + (long long)(ctl->h * a.group) * a.q_sh;
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      const int x = (tid >> 4) + 16 * i, row = row0 + x, tok = row / a.group, hd = row - tok * a.group;
+      const bool real = row < rows;
+      const __nv_bfloat16* from = real ? q + tok * a.q_st + hd * a.q_sh + piece * 8 : a.q;
+      uint8_t* to = sQ + (x >> 7) * kTileBytes + (piece >> 3) * kHalfBytes + (x & 127) * 128 + (((piece & 7) ^ (x & 7)) << 4);
+      if constexpr (kMode == kCodes) {
+        uint4 v = real ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
+        const float scale = query_to_f16(v);
+        *reinterpret_cast<uint4*>(to) = v;
+        if (piece == 0) ctl->q_scale[x] = scale;
+      } else {
+        cp_async16(smem_u32(to), from, real);
+      }
+    }
+    cp_async_wait<0>();
+    fence_proxy_async_smem();
+    mbar_arrive(&ctl->q_full);
+  }
+
+  // Positions in the ring of K and V tiles: K0 K1 V0 K2 V1 ...; the tile at position n, and whether it is V's
+  const int positions = 2 * total;
+  auto tile_of = [&](int n, int& which) {
+    which = n == positions - 1 || (n > 0 && (n & 1) == 0);
+    return n == positions - 1 ? total - 1 : which ? n / 2 - 1 : (n + 1) / 2;
+  };
+
   if (warp >= 12) {
     // ------------------------------------------------------------------ gather
-    give_registers<TileRegs<kFp8>::kOthers>();
+    give_registers<Shape::kOthers>();
     const int r = tid - 12 * 32;
     bool ok = true;  // (every thread goes through the same barriers, also after a wait ran out)
-    const int len = ctl->seq.len, hkv = ctl->h;
-    // queries: the rows' places, then the rows
-    {
-      const int rows = ctl->seq.n * a.group, row0 = ctl->block * 2 * kBM;
-      for (int i = 0; i < 2; ++i) {
-        const int row = row0 + i * kBM + r, tok = row / a.group, hd = row - tok * a.group;
-        ctl->off[i][r] = row < rows ? 2 * (ctl->b * a.q_sb + (long long)(ctl->seq.start + tok) * a.q_st +
-                                           (long long)(hkv * a.group + hd) * a.q_sh) : -1;
-      }
-      asm volatile("bar.sync 2, 128;" ::: "memory");
-      const int piece = r & 15;
-#pragma unroll 8
-      for (int i = 0; i < 32; ++i) {
-        const int row = (r >> 4) + 8 * (i & 15);
-        const long long from = ctl->off[i >> 4][row];
-        const uint32_t to = smem_u32(sQ) + (i >> 4) * kTileBytes + (piece >> 3) * kHalfBytes + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to),
-                     "l"(reinterpret_cast<const uint8_t*>(a.q) + (from >= 0 ? from + piece * 16 : 0)), "r"(from >= 0 ? 16 : 0) : "memory");
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      fence_proxy_async_smem();
-      mbar_arrive(&ctl->q_full);
-      asm volatile("bar.sync 2, 128;" ::: "memory");  // the places are free again
-    }
-    // page of this thread's key of tile j
-    auto page_of = [&](int j) {
-      const int pos = (first + j) * kBN + r;
-      if (j >= total || pos >= len) return -1;
-      const int id = a.c.table[ctl->b * a.c.table_stride + page_index(a.c, pos)];
-      if (id < 0 || id >= a.c.pages) {
-        paged_error(a.c);
-        return -1;
-      }
-      return id;
-    };
-    auto put_place = [&](int j, int page) {
-      const int pos = (first + j) * kBN + r, slot = pos - page_index(a.c, pos) * a.c.page_size;
-      ctl->off[j % 3][r] = page >= 0 ? paged_offset(a.c, page, slot, hkv) : -1;
-      if constexpr (kFp8) ctl->off_scale[j % 3][r] = page >= 0 ? scale_offset(a.c, page, slot, hkv) : 0;
-    };
-    // Positions in the ring: K0 K1 V0 K2 V1 ... (tile, K or V) of position n
-    const int positions = 2 * total;
-    auto tile_of = [&](int n, int& which) {
-      if (n == 0) { which = 0; return 0; }
-      if (n == positions - 1) { which = 1; return total - 1; }
-      which = (n & 1) ^ 1;
-      return which ? n / 2 - 1 : (n + 1) / 2;
-    };
-    int page = page_of(0);
-    if constexpr (!kFp8) {
+    const int len = ctl->seq.len;
+    if constexpr (kMode == kRows) {
+      // the page table's entry for this thread's key of tile j
+      auto entry_of = [&](int j) {
+        const int pos = (first + j) * kBN + r;
+        return j < total && pos < len ? paged_entry(a.c, ctl->b, pos) : 0;
+      };
+      int entry = entry_of(0);
       const int piece = r & 15, row0 = r >> 4;
       const uint32_t col = (piece >> 3) * kHalfBytes;
-      int placed = 0;  // tiles whose places are in shared memory
       for (int n = 0; n < positions; ++n) {
         int which;
         const int j = tile_of(n, which);
-        if (j == placed) {
-          put_place(j, page);
-          page = page_of(j + 1);
-          ++placed;
+        if (!which) {  // where the tile's rows lie (three buffers: the values of the tile before are still to be fetched)
+          const int pos = (first + j) * kBN + r, slot = pos - page_index(a.c, pos) * a.c.page_size;
+          const int page = pos < len ? paged_id(a.c, entry, -1) : -1;
+          ctl->off[j % 3][r] = page >= 0 ? paged_offset(a.c, page, slot, ctl->h) : -1;
+          entry = entry_of(j + 1);
           asm volatile("bar.sync 2, 128;" ::: "memory");
         }
-        const int stage = n % kTileStages, round = n / kTileStages;
+        const int stage = n % kStages, round = n / kStages;
         if (ok && round > 0) ok = mbar_wait(&ctl->kv_empty[stage], (round - 1) & 1, abort_word, MB_ERR_TIMEOUT_KV_EMPTY);
         if (ok) {
           const uint8_t* base = which ? a.c.v : a.c.k;
           const uint32_t dst = smem_u32(sKV) + stage * kTileBytes + col;
           const long long* off = ctl->off[j % 3];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int row = row0 + 8 * i;
-            const long long from = off[row];
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + row * 128 + (((piece & 7) ^ (row & 7)) << 4)),
-                         "l"(from >= 0 ? base + from + piece * 16 : base), "r"(from >= 0 ? 16 : 0) : "memory");
+          for (int i = 0; i < 16; i += 8) {
+            long long from[8];  // (read before the first copy is issued: the compiler keeps their order)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) from[e] = off[row0 + 8 * (i + e)];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int row = row0 + 8 * (i + e);
+              cp_async16(dst + row * 128 + (((piece & 7) ^ (row & 7)) << 4),
+                         from[e] >= 0 ? base + from[e] + piece * 16 : base, from[e] >= 0);
+            }
           }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (n >= 1) {
-          asm volatile("cp.async.wait_group 1;" ::: "memory");
+        cp_async_commit();
+        if (n >= 2) {
+          cp_async_wait<2>();
           fence_proxy_async_smem();
-          mbar_arrive(&ctl->kv_full[(n - 1) % kTileStages]);
+          mbar_arrive(&ctl->kv_full[(n - 2) % kStages]);
         }
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
+      cp_async_wait<0>();
       fence_proxy_async_smem();
-      if (positions > 0) mbar_arrive(&ctl->kv_full[(positions - 1) % kTileStages]);
-    } else {
+      for (int n = max(positions - 2, 0); n < positions; ++n) mbar_arrive(&ctl->kv_full[n % kStages]);
+    } else if constexpr (kMode == kCodes) {
+      constexpr int kStride = Shape::kGather / 8;
       const int piece = r & 7, row0 = r >> 3;
-      uint4 x[8];
-      uint32_t sc[8];
-      auto fetch = [&](int n, int i) {  // piece i of position n
-        int which;
-        const int j = tile_of(n, which), row = row0 + 16 * i;
-        const long long from = ctl->off[j % 3][row];
-        x[i] = make_uint4(0, 0, 0, 0);
-        sc[i] = 127;
-        if (from >= 0) {
-          x[i] = __ldg(reinterpret_cast<const uint4*>((which ? a.c.v : a.c.k) + from) + piece);
-          sc[i] = __ldg((which ? a.c.v_scale : a.c.k_scale) + ctl->off_scale[j % 3][row] + (piece >> 1));
-        }
-      };
-      int placed = 0;
-      auto place_up_to = [&](int j) {  // uniform over the warpgroup
-        if (j == placed && j < total) {
-          put_place(j, page);
-          page = page_of(j + 1);
-          ++placed;
-          asm volatile("bar.sync 2, 128;" ::: "memory");
-        }
-      };
-      place_up_to(0);
-      if (positions > 0) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) fetch(0, i);
-      }
+#pragma unroll 1
       for (int n = 0; n < positions; ++n) {
-        const int stage = n % kTileStages, round = n / kTileStages;
+        const int stage = n % kStages, round = n / kStages, from = n % Shape::kCodeStages;
         int which;
-        if (n + 1 < positions) place_up_to(tile_of(n + 1, which));
+        const int j = tile_of(n, which);
+        if (ok) ok = mbar_wait(&ctl->codes_full[from], (n / Shape::kCodeStages) & 1, abort_word, MB_ERR_TIMEOUT_KV_FULL);
+        const int top = max(max(ctl->warp_top[j & 3][which][0], ctl->warp_top[j & 3][which][1]), kMinScale);
+        if (!which && r == 0) {  // for the softmax warps
+          ctl->top[j & 7][0] = top - 127;
+          ctl->top[j & 7][1] = max(max(ctl->warp_top[j & 3][1][0], ctl->warp_top[j & 3][1][1]), kMinScale) - 127;
+        }
         if (ok && round > 0) ok = mbar_wait(&ctl->kv_empty[stage], (round - 1) & 1, abort_word, MB_ERR_TIMEOUT_KV_EMPTY);
-        uint8_t* dst = sKV + stage * kTileBytes + (piece >> 2) * kHalfBytes;
+        if (ok) {
+          const uint8_t* codes = sCodes + from * Shape::kCodeStage + piece * 16;
+          uint8_t* dst = sKV + stage * kTileBytes + (piece >> 2) * kHalfBytes;
+          // the lanes of a row store even pieces of one half and odd pieces of the other at a time: different banks
+          const int c0 = (2 * piece) & 7, swap = (piece >> 2) & 1;
+          // four rows at a time: all loads before the first store, which the compiler would not pass
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = row0 + 16 * i;
-          const uint32_t mult = scale_mult(sc[i]);
-          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-          uint32_t y[8];
+          for (int i = 0; i < kBN / kStride; i += 4) {
+            uint2 x[4], y[4];
+            uint32_t w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            y[2 * e] = mul_bf16x2(e4m3_bits(__byte_perm(w[e], 0, 0x1404)), mult);
-            y[2 * e + 1] = mul_bf16x2(e4m3_bits(__byte_perm(w[e], 0, 0x3424)), mult);
-          }
-          if (n + 1 < positions) fetch(n + 1, i);
-          if (ok) {
-            // the lanes of a row store even pieces of one half and odd pieces of the other at a time: different banks
-            const int c0 = (2 * piece) & 7, swap = (piece >> 2) & 1;
-            uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
-            uint8_t* at = dst + row * 128;
-            *reinterpret_cast<uint4*>(at + (((c0 + swap) ^ (row & 7)) << 4)) = swap ? hi : lo;
-            *reinterpret_cast<uint4*>(at + (((c0 + 1 - swap) ^ (row & 7)) << 4)) = swap ? lo : hi;
+            for (int e = 0; e < 4; ++e) {
+              const int row = row0 + kStride * (i + e);
+              w[e] = ctl->scales[j & 3][which][row];
+              x[e] = *reinterpret_cast<const uint2*>(codes + row * kHeadDim + swap * 8);
+              y[e] = *reinterpret_cast<const uint2*>(codes + row * kHeadDim + 8 - swap * 8);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int row = row0 + kStride * (i + e);
+              const float f = scale_relative((w[e] >> (8 * (piece >> 1))) & 0xffu, top);
+              const uint32_t mult = pack_f16x2(f, f);
+              uint8_t* at = dst + row * 128;
+              *reinterpret_cast<uint4*>(at + (((c0 + swap) ^ (row & 7)) << 4)) =
+                  make_uint4(mul_f16x2(e4m3_f16(x[e].x), mult), mul_f16x2(e4m3_f16_high(x[e].x), mult),
+                             mul_f16x2(e4m3_f16(x[e].y), mult), mul_f16x2(e4m3_f16_high(x[e].y), mult));
+              *reinterpret_cast<uint4*>(at + (((c0 + 1 - swap) ^ (row & 7)) << 4)) =
+                  make_uint4(mul_f16x2(e4m3_f16(y[e].x), mult), mul_f16x2(e4m3_f16_high(y[e].x), mult),
+                             mul_f16x2(e4m3_f16(y[e].y), mult), mul_f16x2(e4m3_f16_high(y[e].y), mult));
+            }
           }
         }
         fence_proxy_async_smem();
         mbar_arrive(&ctl->kv_full[stage]);
+        mbar_arrive(&ctl->codes_empty[from]);
       }
     }
   } else if (warp == 9 || warp == 11) {
-    give_registers<TileRegs<kFp8>::kOthers>();
+    give_registers<Shape::kOthers>();
+    if constexpr (kMode == kCodes) {
+      // ---------------------------------------------------------------- codes: a thread places rows f and f + 64 of a tile
+      // and copies 16 codes of every eighth row
+      const int f = lane + (warp == 11 ? 32 : 0), len = ctl->seq.len, piece = f & 7;
+      bool ok = true;  // (both warps go through the same barriers, also after a wait ran out)
+      auto entry_of = [&](int j, int i) {
+        const int pos = (first + j) * kBN + f + 64 * i;
+        return j < total && pos < len ? paged_entry(a.c, ctl->b, pos) : 0;
+      };
+      long long off[2];     // of the tile to place next
+      uint32_t words[2][2]; // its scale bytes, [key, value][row]
+      int entry[2];         // of the tile behind it
+      auto look_up = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int pos = (first + j) * kBN + f + 64 * i, slot = pos - page_index(a.c, pos) * a.c.page_size;
+          const int page = j < total && pos < len ? paged_id(a.c, entry[i], -1) : -1;
+          off[i] = page >= 0 ? paged_offset(a.c, page, slot, ctl->h) : -1;
+          const long long at = page >= 0 ? scale_offset(a.c, page, slot, ctl->h) : 0;
+          words[0][i] = page >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(a.c.k_scale + at)) : 0;
+          words[1][i] = page >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(a.c.v_scale + at)) : 0;
+          entry[i] = entry_of(j + 1, i);
+        }
+      };
+      entry[0] = entry_of(0, 0);
+      entry[1] = entry_of(0, 1);
+      look_up(0);
+#pragma unroll 1
+      for (int n = 0; n < positions; ++n) {
+        int which;
+        const int j = tile_of(n, which), stage = n % Shape::kCodeStages, round = n / Shape::kCodeStages;
+        if (!which) {  // (three buffers: the values of the tile before are still to be fetched)
+          ctl->off[j % 3][f] = off[0];
+          ctl->off[j % 3][f + 64] = off[1];
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            ctl->scales[j & 3][kv][f] = words[kv][0];
+            ctl->scales[j & 3][kv][f + 64] = words[kv][1];
+            const int top = __reduce_max_sync(0xffffffffu, max(scale_top(words[kv][0]), scale_top(words[kv][1])));
+            if (lane == 0) ctl->warp_top[j & 3][kv][warp == 11] = top;
+          }
+          asm volatile("bar.sync 2, 64;" ::: "memory");
+          look_up(j + 1);
+        }
+        if (ok && round > 0) ok = mbar_wait(&ctl->codes_empty[stage], (round - 1) & 1, abort_word, MB_ERR_TIMEOUT_KV_EMPTY);
+        if (ok) {
+          const uint8_t* base = (which ? a.c.v : a.c.k) + piece * 16;
+          const uint32_t to = smem_u32(sCodes) + stage * Shape::kCodeStage + piece * 16;
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            long long from[4];  // (read before the first copy is issued: the compiler keeps their order)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) from[e] = ctl->off[j % 3][(f >> 3) + 8 * (i + e)];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              cp_async16(to + ((f >> 3) + 8 * (i + e)) * kHeadDim, from[e] >= 0 ? base + from[e] : a.c.k, from[e] >= 0);
+          }
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl->codes_full[stage])) : "memory");
+        mbar_arrive(&ctl->codes_full[stage]);
+      }
+      cp_async_wait<0>();
+    }
+    if constexpr (kMode == kBoxes) {
+      // ---------------------------------------------------------------- TMA: a lane has a box of a tile, a warp half of
+      // its columns (lanes issue one after the other, some 55 cycles each: small pages are bound by it)
+      const int half = warp == 11;
+      const int len = ctl->seq.len, boxes = kBN / maps.box;
+      bool ok = true;
+      auto page_of = [&](int j) {
+        const int pos = (first + j) * kBN + lane * maps.box;
+        if (j >= total || lane >= boxes || pos >= len) return a.c.pages;  // zeros
+        const int id = a.c.table[ctl->b * a.c.table_stride + page_index(a.c, pos)];
+        if (id < 0 || id >= a.c.pages) {
+          paged_error(a.c);
+          return a.c.pages;
+        }
+        return id;
+      };
+      if (lane == 0) tma_prefetch_desc(half ? &maps.v : &maps.k);
+      int page = page_of(0), page1 = page, page2 = page, n = 0;  // of the next keys, the last ones and those before
+      for (; n < positions && ok; ++n) {
+        int which;
+        const int j = tile_of(n, which);
+        const int stage = n % kStages, round = n / kStages;
+        const int id = !which ? page : n == positions - 1 ? page1 : page2;
+        const int pos = (first + j) * kBN + lane * maps.box;
+        const int slot = id < a.c.pages ? pos - page_index(a.c, pos) * a.c.page_size : 0;
+        if (round > 0) ok = mbar_wait_warp(&ctl->kv_empty[stage], (round - 1) & 1, abort_word, MB_ERR_TIMEOUT_KV_EMPTY);
+        if (!ok) break;
+        const int k0 = (first + j) * kBN;
+        const bool tail = which && k0 + kBN > len && len % maps.box != 0;  // a box holds rows behind the end
+        uint64_t* full = tail ? &ctl->tail : &ctl->kv_full[stage];
+        uint8_t* dst = sKV + stage * kTileBytes + lane * maps.box * 128;
+        if (lane == 0 && half == 0) mbar_expect_tx(full, kTileBytes);  // (of both warps)
+        __syncwarp();
+        if (lane < boxes) tma_load_4d(dst + half * kHalfBytes, which ? &maps.v : &maps.k, full, half * 64, ctl->h, slot, id);
+        if (tail && half == 0) {  // (the last position: no other tile reaches the end)
+          ok = mbar_wait_warp(&ctl->tail, 0, abort_word, MB_ERR_TIMEOUT_KV_FULL);
+          const int from = len - k0, to = (from + maps.box - 1) / maps.box * maps.box;
+          for (int i = from * 16 + lane; i < to * 16; i += 32)
+            *reinterpret_cast<uint4*>(sKV + stage * kTileBytes + ((i >> 3) & 1) * kHalfBytes + (i >> 4) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->kv_full[stage]);
+        }
+        if (!which) {
+          page2 = page1;
+          page1 = page;
+          page = page_of(j + 1);
+        }
+      }
+      if (!ok) {
+        // give copies already in flight a bounded chance to land before the CTA exits
+        for (int m = max(n - kStages, 0); m < n; ++m) {
+          const long long t0 = clock64();
+          while (!mbar_try_wait(&ctl->kv_full[m % kStages], (m / kStages) & 1) && clock64() - t0 < kWaitCycleLimit / 16) {
+          }
+        }
+      }
+    }
   } else if (warp == 8 || warp == 10) {
     // ------------------------------------------------------------------ tcgen05 issuers (see attn_fwd.cu)
-    give_registers<TileRegs<kFp8>::kOthers>();
+    give_registers<Shape::kOthers>();
     if (total > 0) {
       constexpr uint32_t kStageUnits = kTileBytes / 16;
       bool ok = true;
       if (warp == 8) {
-        constexpr uint32_t idesc_qk = umma_idesc_bf16(kBM, kBN, false, false);
+        constexpr uint32_t idesc_qk = tile_idesc<kMode>(kBN, false);
         const uint64_t q_desc = umma_smem_desc(smem_u32(sQ), 16, 1024);
         const uint64_t k_desc0 = umma_smem_desc(smem_u32(sKV), 16, 1024);
         int use = 0;
         ok = mbar_wait_warp(&ctl->q_full, 0, abort_word, MB_ERR_TIMEOUT_Q);
         for (int g = 0; g < total && ok; ++g) {
-          const int pos = g == 0 ? 0 : 2 * g - 1, stage = pos % kTileStages;
-          ok = mbar_wait_warp(&ctl->kv_full[stage], (pos / kTileStages) & 1, abort_word, MB_ERR_TIMEOUT_KV_FULL);
+          const int pos = g == 0 ? 0 : 2 * g - 1, stage = pos % kStages;
+          ok = mbar_wait_warp(&ctl->kv_full[stage], (pos / kStages) & 1, abort_word, MB_ERR_TIMEOUT_KV_FULL);
           if (!ok) break;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -366,12 +512,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
           umma_commit_elect(&ctl->kv_empty[stage]);
         }
       } else {
-        constexpr uint32_t idesc_pv = umma_idesc_bf16(kBM, kD, false, true);
+        constexpr uint32_t idesc_pv = tile_idesc<kMode>(kD, true);
         const uint64_t v_desc0 = umma_smem_desc(smem_u32(sKV), kHalfBytes, 1024);
         int cnt[2] = {0, 0};
         for (int g = 0; g < total && ok; ++g) {
-          const int pos = g == total - 1 ? 2 * total - 1 : 2 * g + 2, stage = pos % kTileStages;
-          ok = mbar_wait_warp(&ctl->kv_full[stage], (pos / kTileStages) & 1, abort_word, MB_ERR_TIMEOUT_KV_FULL);
+          const int pos = g == total - 1 ? 2 * total - 1 : 2 * g + 2, stage = pos % kStages;
+          ok = mbar_wait_warp(&ctl->kv_full[stage], (pos / kStages) & 1, abort_word, MB_ERR_TIMEOUT_KV_FULL);
           if (!ok) break;
           const uint64_t v_desc = v_desc0 + stage * kStageUnits;
 #pragma unroll
@@ -405,7 +551,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
     }
   } else {
     // ------------------------------------------------------------------ softmax + epilogue
-    take_registers<TileRegs<kFp8>::kSoftmax>();
+    take_registers<Shape::kSoftmax>();
     const int i = warp >> 2;                   // query tile
     const int row = ((warp & 3) << 5) | lane;  // row inside the tile == tensor-memory lane
     const uint32_t lane_field = static_cast<uint32_t>((warp & 3) << 5) << 16;
@@ -416,6 +562,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
     const int visible = visible_keys(a, ctl->seq, tile_row + row), visible_first = visible_keys(a, ctl->seq, tile_row);
     const int last = i ? n1 : n0;
 
+    // A row's reference m_ref is the exponent of its largest term exp2(score) * 2^value_exp (bf16: value_exp = 0)
     float m_ref = -INFINITY, l = 0.f;
     int cnt = 0;
     bool ok = true;
@@ -449,7 +596,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
         mx2 = max3(mx2, __uint_as_float(sr[2][e]), __uint_as_float(sr[2][e + 1]));
         mx3 = max3(mx3, __uint_as_float(sr[3][e]), __uint_as_float(sr[3][e + 1]));
       }
-      const float m_tile = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+      float c = a.scale_log2, value_exp = 0.f;
+      if constexpr (kMode == kCodes) {
+        const int* top = ctl->top[(jt - first) & 7];
+        c = fmaxf(c * exp2_int(top[0]) * ctl->q_scale[i * kBM + row], 1.2e-38f);  // (not zero: hidden scores are infinite)
+        value_exp = (float)top[1];
+      }
+      float m_tile = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+      m_tile = m_tile == -INFINITY ? -INFINITY : fmaf(m_tile, c, value_exp);
       if (cnt == 0) {
         m_ref = m_tile;
       } else {
@@ -458,9 +612,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
         if (!ok) break;
         tc_fence_after();
         const float m_new = fmaxf(m_ref, m_tile);
-        const bool need = (m_new - m_ref) * a.scale_log2 > kRescaleThreshold;
+        const bool need = m_new - m_ref > kRescaleThreshold;
         if (__any_sync(0xffffffffu, need)) {
-          const float f = need ? fast_exp2((m_ref - m_new) * a.scale_log2) : 1.f;
+          const float f = need ? fast_exp2(m_ref - m_new) : 1.f;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t orow[32];
@@ -477,9 +631,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
           }
         }
       }
-      const float m_scaled = (m_ref == -INFINITY) ? 0.f : m_ref * a.scale_log2;
-      const uint64_t c2 = pack2(a.scale_log2, a.scale_log2);
-      const uint64_t nm2 = pack2(-m_scaled, -m_scaled);
+      const float lift = value_exp - ((m_ref == -INFINITY) ? 0.f : m_ref);
+      const uint64_t c2 = pack2(c, c);
+      const uint64_t nm2 = pack2(lift, lift);
       uint64_t sum_a = pack2(0.f, 0.f), sum_b = pack2(0.f, 0.f);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -497,7 +651,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
             else sum_a = add2(sum_a, p2);
             float p0, p1;
             unpack2(p2, p0, p1);
-            pk[cc * 16 + (e >> 1)] = pack_bf16x2(p0, p1);
+            pk[cc * 16 + (e >> 1)] = kMode == kCodes ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
           }
         }
         tmem_st32(tPi + half * 32, pk);
@@ -507,7 +661,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
       }
       float s0, s1;
       unpack2(add2(sum_a, sum_b), s0, s1);
-      l += s0 + s1;
+      l = kMode == kCodes ? fmaf(s0 + s1, fast_exp2(-value_exp), l) : l + (s0 + s1);
       ++cnt;
     }
 
@@ -537,7 +691,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
           }
           a.tile_ml[(long long)blockIdx.x * (2 * kBM) + r] = make_float2(m_ref, l);
         } else {
-          const float inv = l == 0.f ? 0.f : a.out_scale / l;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
           const int tok = (tile_row + row) / a.group, hd = ctl->h * a.group + (tile_row + row) - tok * a.group;
           __nv_bfloat16* optr = a.o + ctl->b * a.o_sb + (long long)(ctl->seq.start + tok) * a.o_st + (long long)hd * a.o_sh;
 #pragma unroll
@@ -566,7 +720,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tiles_kernel(const __gr
             }
           }
           if (store)
-            a.lse[ctl->b * a.lse_sb + hd * a.lse_sh + ctl->seq.start + tok] = l == 0.f ? -INFINITY : m_ref * a.scale + __logf(l);
+            a.lse[ctl->b * a.lse_sb + hd * a.lse_sh + ctl->seq.start + tok] = l == 0.f ? -INFINITY : m_ref * kLn2 + __logf(l);
         }
       }
     }
@@ -605,36 +759,38 @@ __global__ void __launch_bounds__(256) paged_tiles_merge_kernel(const __grid_con
     const float2 s = ml[p * 2 * kBM];
     if (s.y == 0.f) continue;  // a share without visible keys has stored no rows, or products of hidden keys
     const float4 x = src[(long long)p * 32 * 2 * kBM];
-    const float w = s.x == -INFINITY ? 1.f : fast_exp2((s.x - m) * a.scale_log2);
+    const float w = s.x == -INFINITY ? 1.f : fast_exp2(s.x - m);
     l = fmaf(w, s.y, l);
     acc[0] = fmaf(w, x.x, acc[0]);
     acc[1] = fmaf(w, x.y, acc[1]);
     acc[2] = fmaf(w, x.z, acc[2]);
     acc[3] = fmaf(w, x.w, acc[3]);
   }
-  const float inv = l == 0.f ? 0.f : a.out_scale / l;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   const int tok = row / a.group, hd = unit.y * a.group + row - tok * a.group;
   const uint2 o = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
   *reinterpret_cast<uint2*>(a.o + unit.x * a.o_sb + (long long)(seq.start + tok) * a.o_st + (long long)hd * a.o_sh + chunk * 4) = o;
-  if (chunk == 0) a.lse[unit.x * a.lse_sb + hd * a.lse_sh + seq.start + tok] = l == 0.f ? -INFINITY : m * a.scale + __logf(l);
+  if (chunk == 0) a.lse[unit.x * a.lse_sb + hd * a.lse_sh + seq.start + tok] = l == 0.f ? -INFINITY : m * kLn2 + __logf(l);
 }
 
 long long paged_tiles_workspace(long long ctas) {
   return ctas * (2ll * kBM * (kHeadDim * (long long)sizeof(float) + (long long)sizeof(float2)) + (long long)sizeof(int4));
 }
 
-template <bool kFp8>
-static int launch_tiles(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
+template <int kMode>
+static int launch_tiles(const TileMaps& maps, const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   static bool attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MB_E_CUDA;
+  constexpr int bytes = tile_smem_bytes<kMode>();
   if (!attr_set[dev]) {
-    if (!cuda_ok(cudaFuncSetAttribute(paged_tiles_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmemBytes),
+    if (!cuda_ok(cudaFuncSetAttribute(paged_tiles_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
                  "paged_tiles_kernel shared memory"))
       return MB_E_CUDA;
     attr_set[dev] = true;
   }
-  if (!launch_overlapped("launch paged_tiles_kernel", paged_tiles_kernel<kFp8>, dim3(ctas), kTileThreads, kTileSmemBytes, stream, a))
+  if (!launch_overlapped("launch paged_tiles_kernel", paged_tiles_kernel<kMode>, dim3(ctas), TileShape<kMode>::kThreads, bytes,
+                         stream, maps, a))
     return MB_E_CUDA;
   if (a.tile_open != nullptr &&
       !launch_overlapped("launch paged_tiles_merge_kernel", paged_tiles_merge_kernel,
@@ -643,8 +799,23 @@ static int launch_tiles(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   return MB_SUCCESS;
 }
 
+static bool page_map(CUtensorMap* map, const void* ptr, const PagedView& c, int box) {
+  const cuuint64_t dims[4] = {(cuuint64_t)kHeadDim, (cuuint64_t)c.hkv, (cuuint64_t)c.page_size, (cuuint64_t)c.pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)c.head_sb, (cuuint64_t)c.slot_sb, (cuuint64_t)c.page_sb};
+  const cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1}, ones[4] = {1, 1, 1, 1};
+  return encode_tiled_bf16(map, const_cast<void*>(ptr), 4, dims, strides, boxes, ones) == 0;
+}
+
 int launch_paged_tiles(const PagedAttnArgs& a, bool fp8, int ctas, cudaStream_t stream) {
-  return fp8 ? launch_tiles<true>(a, ctas, stream) : launch_tiles<false>(a, ctas, stream);
+  TileMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  if (fp8) return launch_tiles<kCodes>(maps, a, ctas, stream);
+  maps.box = 1;
+  while (maps.box < kBN && a.c.page_size % (2 * maps.box) == 0) maps.box *= 2;
+  // (strides that no tensor map takes, as of a dimension of one entry, go row by row as well)
+  if (maps.box >= 8 && a.c.pages > 0 && page_map(&maps.k, a.c.k, a.c, maps.box) && page_map(&maps.v, a.c.v, a.c, maps.box))
+    return launch_tiles<kBoxes>(maps, a, ctas, stream);
+  return launch_tiles<kRows>(maps, a, ctas, stream);
 }
 
 }  // namespace mb

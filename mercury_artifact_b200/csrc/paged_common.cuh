@@ -65,6 +65,17 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedView& c, int b, int max
 __device__ __forceinline__ int page_index(const PagedView& c, int pos) {
   return c.page_shift >= 0 ? pos >> c.page_shift : pos / c.page_size;
 }
+// The table's entry for key `pos` of sequence b as it is; paged_id checks it.  (Entries are fetched ahead, and the check
+// would wait for them.)
+__device__ __forceinline__ int paged_entry(const PagedView& c, int b, int pos) {
+  return c.table[b * c.table_stride + page_index(c, pos)];
+}
+// `entry` if it is a page, else `none`, and an error.
+__device__ __forceinline__ int paged_id(const PagedView& c, int entry, int none) {
+  if (entry >= 0 && entry < c.pages) return entry;
+  paged_error(c);
+  return none;
+}
 // Byte offset of head `h` of the key in slot pos - p * page_size of page `id`, and of its scales (scale
 // blocks of one head lie slot by slot).
 __device__ __forceinline__ long long paged_offset(const PagedView& c, int id, int slot, int h) {
@@ -74,7 +85,7 @@ __device__ __forceinline__ long long scale_offset(const PagedView& c, int id, in
   return (((long long)id * c.hkv + h) * c.page_size + slot) * kScalesPerRow;
 }
 
-// ---- e4m3 codes as bf16 ------------------------------------------------------------------
+// ---- e4m3 codes as bf16 and f16 ------------------------------------------------------------
 // The bits of a code, put into the fraction and the low exponent bits of a bf16, stand for its value times 2^-120
 // (exponent biases 7 and 127; subnormal codes become subnormal bf16), so that one exact product gives code * 2^n.
 // x holds the codes in the high byte of each half.
@@ -84,13 +95,73 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// What the products work with is code * 2^(byte - 127 - kScaleBias): the bias keeps the multiplier 2^(byte - 7 -
-// kScaleBias) of e4m3_bits a finite bf16 up to kMaxScale, and is taken out of the fp32 results, where it is exact.
-constexpr int kScaleBias = 60;
-constexpr uint32_t kScaleAdd = 120 - kScaleBias;  // of the exponent field
-__device__ __forceinline__ uint32_t scale_mult(uint32_t byte) {  // the multiplier twice
-  const uint32_t m = byte > (uint32_t)kMaxScale ? 0x7fc0u : (byte + kScaleAdd) << 7;
-  return m | (m << 16);
+// The attention kernels multiply in f16, which holds a code as it is: code * 2^(n - N) with N the largest exponent of the
+// keys (or values) that one product takes, in units of 2^N.  That is exact down to n = N - 15 (f16 ends at 2^-24, a code at
+// 2^-9), off by less than bf16 would be down to N - 23, by less than e4m3's own rounding down to N - 27, and zero below N - 34.
+// (One conversion for two codes and one product, where the way through the bits above takes four integer instructions at
+// half rate: 64 tokens against up to 16 384 keys of 8 heads took 302 us with those and 189 without.)
+__device__ __forceinline__ uint32_t e4m3_f16(uint32_t two) {  // the two low bytes
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3_f16_high(uint32_t two) {  // the two high bytes
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(two));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// 2^(byte - top), top >= byte, as a float (0 below 2^-126); bytes beyond the written range: not a number.
+__device__ __forceinline__ float scale_relative(uint32_t byte, int top) {
+  return byte > (uint32_t)kMaxScale ? __int_as_float(0x7fc00000) : __int_as_float(max((int)byte - top + 127, 0) << 23);
+}
+__device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+// The largest of four scale bytes, those beyond the written range left out.
+__device__ __forceinline__ uint32_t scale_top(uint32_t w) {
+  const uint32_t beyond = w & (w << 1) & 0x80808080u;
+  w &= ~((beyond >> 7) * 0xffu);
+  const uint32_t m = __vmaxu2(w & 0x00ff00ffu, (w >> 8) & 0x00ff00ffu);
+  return max(m & 0xffffu, m >> 16);
+}
+
+// A row of 16 lanes' queries, eight bf16 values each, as f16 in [-2, 2) (or (-4, 4)) times a power of two, which is returned.
+__device__ __forceinline__ float query_to_f16(uint4& x) {
+  uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);  // |x| of bf16 orders like its bits
+  m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  const int e = m == 0 ? 0 : min(max((int)(m >> 7) - 127, -126), 126);
+  const float inv = exp2_int(-e);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = pack_f16x2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
+  x = make_uint4(w[0], w[1], w[2], w[3]);
+  return exp2_int(e);
+}
+
+// ---- 16 or 4 bytes into shared memory, zeros where they are not real --------------------------
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
 int paged_view(const mb_paged_kv* kv, PagedView* c);
