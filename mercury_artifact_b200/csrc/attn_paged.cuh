@@ -27,6 +27,9 @@ struct PagedAttnArgs {
   // [CTA][256]; tile_open: the split unit whose first share a CTA has (sequence, K/V head, row block, shares; 0: none).
   // All null where no unit is split.
   int share_tiles;
+  // tiles: keys and values of every sequence one after the other in bf16, [batch, packed_rows, hkv, 128] (null: in pages)
+  const __nv_bfloat16 *packed_k, *packed_v;
+  int packed_rows;
   int head_bytes;  // of a cached key and value of one head
   float4* tile_o;
   float2* tile_ml;
@@ -38,6 +41,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream);
 long long paged_rows_workspace(int rows, int ctas);
 int paged_rows_ctas();
+// The first `rows` keys and values of every sequence with at least min_new new tokens, in bf16 [batch, rows, hkv, 128].
+int launch_read_e4m3(const PagedView& c, void* k_out, void* v_out, int rows, int min_new, int max_new, cudaStream_t stream);
 int launch_paged_tiles(const PagedAttnArgs& a, bool fp8, int ctas, cudaStream_t stream);
 long long paged_tiles_workspace(long long ctas);
 

@@ -63,7 +63,9 @@ __host__ __device__ constexpr uint32_t tile_idesc(int n, bool b_mn_major) {
 
 struct TileMaps {
   CUtensorMap k, v;
-  int box;  // slots of a box
+  int box;     // slots of a box
+  int pages;   // behind the last one
+  int packed;  // a page is all of a sequence
 };
 
 struct TileSmem {
@@ -429,13 +431,8 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
       bool ok = true;
       auto page_of = [&](int j) {
         const int pos = (first + j) * kBN + lane * maps.box;
-        if (j >= total || lane >= boxes || pos >= len) return a.c.pages;  // zeros
-        const int id = a.c.table[ctl->b * a.c.table_stride + page_index(a.c, pos)];
-        if (id < 0 || id >= a.c.pages) {
-          paged_error(a.c);
-          return a.c.pages;
-        }
-        return id;
+        if (j >= total || lane >= boxes || pos >= len) return -1;
+        return maps.packed ? ctl->b : paged_entry(a.c, ctl->b, pos);
       };
       if (lane == 0) tma_prefetch_desc(half ? &maps.v : &maps.k);
       int page = page_of(0), page1 = page, page2 = page, n = 0;  // of the next keys, the last ones and those before
@@ -443,9 +440,11 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
         int which;
         const int j = tile_of(n, which);
         const int stage = n % kStages, round = n / kStages;
-        const int id = !which ? page : n == positions - 1 ? page1 : page2;
+        const int entry = !which ? page : n == positions - 1 ? page1 : page2;
         const int pos = (first + j) * kBN + lane * maps.box;
-        const int slot = id < a.c.pages ? pos - page_index(a.c, pos) * a.c.page_size : 0;
+        const bool real = lane < boxes && pos < len;  // else zeros: a page behind the last one
+        const int id = !real ? maps.pages : maps.packed ? entry : paged_id(a.c, entry, maps.pages);
+        const int slot = !real ? 0 : maps.packed ? pos : pos - page_index(a.c, pos) * a.c.page_size;
         if (round > 0) ok = mbar_wait_warp(&ctl->kv_empty[stage], (round - 1) & 1, abort_word, MB_ERR_TIMEOUT_KV_EMPTY);
         if (!ok) break;
         const int k0 = (first + j) * kBN;
@@ -799,9 +798,11 @@ static int launch_tiles(const TileMaps& maps, const PagedAttnArgs& a, int ctas, 
   return MB_SUCCESS;
 }
 
-static bool page_map(CUtensorMap* map, const void* ptr, const PagedView& c, int box) {
-  const cuuint64_t dims[4] = {(cuuint64_t)kHeadDim, (cuuint64_t)c.hkv, (cuuint64_t)c.page_size, (cuuint64_t)c.pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)c.head_sb, (cuuint64_t)c.slot_sb, (cuuint64_t)c.page_sb};
+// Boxes of `box` slots of 64 columns of a head, out of [pages, slots, heads, 128] with strides in bytes.
+static bool page_map(CUtensorMap* map, const void* ptr, int hkv, int slots, int pages, long long head_sb, long long slot_sb,
+                     long long page_sb, int box) {
+  const cuuint64_t dims[4] = {(cuuint64_t)kHeadDim, (cuuint64_t)hkv, (cuuint64_t)slots, (cuuint64_t)pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)head_sb, (cuuint64_t)slot_sb, (cuuint64_t)page_sb};
   const cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1}, ones[4] = {1, 1, 1, 1};
   return encode_tiled_bf16(map, const_cast<void*>(ptr), 4, dims, strides, boxes, ones) == 0;
 }
@@ -809,11 +810,24 @@ static bool page_map(CUtensorMap* map, const void* ptr, const PagedView& c, int 
 int launch_paged_tiles(const PagedAttnArgs& a, bool fp8, int ctas, cudaStream_t stream) {
   TileMaps maps;
   memset(&maps, 0, sizeof(maps));
+  const PagedView& c = a.c;
+  if (a.packed_k != nullptr) {
+    const long long row = (long long)c.hkv * kHeadDim * 2;
+    maps.box = kBN;
+    maps.pages = c.batch;
+    maps.packed = 1;
+    if (!page_map(&maps.k, a.packed_k, c.hkv, a.packed_rows, c.batch, kHeadDim * 2, row, row * a.packed_rows, kBN) ||
+        !page_map(&maps.v, a.packed_v, c.hkv, a.packed_rows, c.batch, kHeadDim * 2, row, row * a.packed_rows, kBN))
+      return MB_E_TENSORMAP;
+    return launch_tiles<kBoxes>(maps, a, ctas, stream);
+  }
   if (fp8) return launch_tiles<kCodes>(maps, a, ctas, stream);
   maps.box = 1;
-  while (maps.box < kBN && a.c.page_size % (2 * maps.box) == 0) maps.box *= 2;
+  maps.pages = c.pages;
+  while (maps.box < kBN && c.page_size % (2 * maps.box) == 0) maps.box *= 2;
   // (strides that no tensor map takes, as of a dimension of one entry, go row by row as well)
-  if (maps.box >= 8 && a.c.pages > 0 && page_map(&maps.k, a.c.k, a.c, maps.box) && page_map(&maps.v, a.c.v, a.c, maps.box))
+  if (maps.box >= 8 && c.pages > 0 && page_map(&maps.k, c.k, c.hkv, c.page_size, c.pages, c.head_sb, c.slot_sb, c.page_sb, maps.box) &&
+      page_map(&maps.v, c.v, c.hkv, c.page_size, c.pages, c.head_sb, c.slot_sb, c.page_sb, maps.box))
     return launch_tiles<kBoxes>(maps, a, ctas, stream);
   return launch_tiles<kRows>(maps, a, ctas, stream);
 }

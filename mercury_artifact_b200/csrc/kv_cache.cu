@@ -64,6 +64,7 @@ struct CacheMoveArgs {
   uint8_t* v;
   long long sb, st, sh;  // bytes
   int rows;              // read: rows per sequence
+  int min_new, max_new;  // read: sequences with at least min_new new tokens only
 };
 
 constexpr int kMoveThreads = 256;
@@ -208,11 +209,9 @@ __global__ void __launch_bounds__(kMoveThreads) kv_cache_read_kernel(const __gri
   const int b = blockIdx.y, p0 = blockIdx.x * kReadTokens;
   grid_dependents_launch();
   grid_dependency_wait();
-  int len = c.seq_lens[b];
-  if (len < 0 || len > c.max_pages * c.page_size) {
-    if (threadIdx.x == 0) paged_error(c);
-    len = min(max(len, 0), c.max_pages * c.page_size);
-  }
+  const PagedSeq seq = paged_seq(c, b, a.max_new, c.max_pages * c.page_size);
+  const int len = seq.len;
+  if (seq.n < a.min_new) return;
   const int n = min(min(len, a.rows) - p0, kReadTokens);
   if (n <= 0) return;
   if (threadIdx.x < n) {
@@ -268,7 +267,7 @@ int launch_kv_cache_write(const mb_paged_kv* kv, const void* k_new, const void* 
   a.k = static_cast<uint8_t*>(const_cast<void*>(k_new));
   a.v = static_cast<uint8_t*>(const_cast<void*>(v_new));
   a.sb = sb * 2; a.st = st * 2; a.sh = sh * 2;
-  a.rows = 0;
+  a.rows = a.min_new = a.max_new = 0;
   const long long rows = (long long)a.c.tokens * 2 * a.c.hkv;
   const bool fp8 = kv->dtype == MB_DTYPE_E4M3;
   const int groups = fp8 ? MoveShape<true>::kGroups : MoveShape<false>::kGroups;
@@ -279,6 +278,26 @@ int launch_kv_cache_write(const mb_paged_kv* kv, const void* k_new, const void* 
                           : (many ? kv_cache_write_kernel<false, 4> : kv_cache_write_kernel<false, 1>);
   return launch_overlapped("launch kv_cache_write_kernel", kernel, dim3((unsigned)blocks), kMoveThreads, 0, stream, a) ? MB_SUCCESS
                                                                                                                : MB_E_CUDA;
+}
+
+static int launch_read(const CacheMoveArgs& a, bool fp8, cudaStream_t stream) {
+  const dim3 grid((a.rows + kReadTokens - 1) / kReadTokens, a.c.batch);
+  const auto kernel = fp8 ? kv_cache_read_kernel<true> : kv_cache_read_kernel<false>;
+  return launch_overlapped("launch kv_cache_read_kernel", kernel, grid, kMoveThreads, 0, stream, a) ? MB_SUCCESS : MB_E_CUDA;
+}
+
+int launch_read_e4m3(const PagedView& c, void* k_out, void* v_out, int rows, int min_new, int max_new, cudaStream_t stream) {
+  CacheMoveArgs a;
+  a.c = c;
+  a.k = static_cast<uint8_t*>(k_out);
+  a.v = static_cast<uint8_t*>(v_out);
+  a.sh = kHeadDim * 2;
+  a.st = a.sh * c.hkv;
+  a.sb = a.st * rows;
+  a.rows = rows;
+  a.min_new = min_new;
+  a.max_new = max_new;
+  return launch_read(a, true, stream);
 }
 
 int launch_kv_cache_read(const mb_paged_kv* kv, void* k_out, void* v_out, long long sb, long long ss, long long sh,
@@ -294,9 +313,10 @@ int launch_kv_cache_read(const mb_paged_kv* kv, void* k_out, void* v_out, long l
   a.v = static_cast<uint8_t*>(v_out);
   a.sb = sb * 2; a.st = ss * 2; a.sh = sh * 2;
   a.rows = rows;
-  const dim3 grid((rows + kReadTokens - 1) / kReadTokens, a.c.batch);
-  const auto kernel = kv->dtype == MB_DTYPE_E4M3 ? kv_cache_read_kernel<true> : kv_cache_read_kernel<false>;
-  return launch_overlapped("launch kv_cache_read_kernel", kernel, grid, kMoveThreads, 0, stream, a) ? MB_SUCCESS : MB_E_CUDA;
+  a.min_new = 0;
+  a.max_new = 0;
+  a.c.cu = nullptr;
+  return launch_read(a, kv->dtype == MB_DTYPE_E4M3, stream);
 }
 
 }  // namespace mb
