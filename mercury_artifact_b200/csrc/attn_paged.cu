@@ -31,9 +31,11 @@ static int plan_paged(const mb_attn_paged_args* x, PagedPlan* p) {
   if (sms <= 0) return MB_E_CUDA;
   memset(p, 0, sizeof(*p));
   const bool padded = x->kv.cu_seqlens == nullptr;
-  p->few = kFewRows;
+  // Beside chunks the sequences with few rows are single tokens as a rule, which the kernel for 16 rows takes faster than
+  // that for 32 (11 of them against up to 8 192 e4m3 keys, 4 rows each: 24 us, 31 with room for 32 rows).
+  p->few = rows > kFewRows && group <= 16 ? 16 : kFewRows;
   if (rows <= kFewRows || !padded) {
-    p->rows = (int)min(rows, (long long)kFewRows);
+    p->rows = (int)min(rows, (long long)p->few);
     p->row_ctas = paged_rows_ctas();
     p->rows_bytes = paged_rows_workspace(p->rows, p->row_ctas);
   }

@@ -32,6 +32,7 @@ struct RowShape {
   static constexpr int kScaleBytes = kFp8 ? kKeys * kScalesPerRow : 0;
   static constexpr int kStage = 2 * kHalf + 2 * kScaleBytes;
   static constexpr int kStep = kKeys * kRowWarps;                  // keys of a CTA's step
+  static_assert(kStage % 256 == 0, "rows are aligned to their size");
   // pitch of the merge buffer, in floats: what the lanes of a warp store together falls into different banks
   static constexpr int kPitch = kFp8 ? 144 : 136;
 };
@@ -144,7 +145,7 @@ template <bool kFp8, int kTiles>
 __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
   using S = RowShape<kFp8>;
   constexpr int kStep = S::kStep, kKeys = S::kKeys, kBlocks = kKeys / 8;
-  extern __shared__ __align__(128) uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* stages = smem_raw + warp * (kRowStages * S::kStage);
   uint8_t* queries = smem_raw + kRowWarps * kRowStages * S::kStage;  // rows of 256 bytes, pieces swapped like the keys'
@@ -208,13 +209,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     const int slot = pos - page_index(a.c, pos) * a.c.page_size;
     const int page = pos < in.s.len ? paged_id(a.c, entry, -1) : -1;
     const long long off = page >= 0 ? paged_offset(a.c, page, slot, in.h) : -1;
+    // Piece p of row r lies at place p ^ (r & 7) of its row.  With r = i * n + r0 (n: rows of a pass, a power of two above
+    // r0) that is (p ^ r0) ^ (i * n & 7): one exclusive or with a constant, as rows are aligned to their size.
+    constexpr int kPass = 32 / S::kPieces;
     const uint32_t dst = stage0 + stage * S::kStage;
+    const uint32_t dst0 = dst + (lane / S::kPieces) * S::kRowBytes + (((lane % S::kPieces) ^ (lane / S::kPieces)) << 4);
+    const int piece = lane % S::kPieces;
 #pragma unroll
-    for (int i = 0; i < kKeys * S::kPieces / 32; ++i) {
-      const int key = i * (32 / S::kPieces) + lane / S::kPieces, piece = lane % S::kPieces;
-      const long long from = __shfl_sync(0xffffffffu, off, key);
+    for (int i = 0; i < kKeys / kPass; ++i) {
+      const long long from = __shfl_sync(0xffffffffu, off, i * kPass + lane / S::kPieces);
       const bool real = from >= 0;
-      const uint32_t to = dst + key * S::kRowBytes + ((piece ^ (key & 7)) << 4);
+      const uint32_t to = (dst0 ^ (((i * kPass) & 7) << 4)) + i * kPass * S::kRowBytes;
       cp_async16(to, real ? a.c.k + from + piece * 16 : a.c.k, real);
       cp_async16(to + S::kHalf, real ? a.c.v + from + piece * 16 : a.c.v, real);
     }
@@ -277,24 +282,24 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       }
     }
   };
-  const uint32_t q_addr = smem_u32(queries) + (lane & 15) * 2 * kHeadDim;
-  auto query = [&](uint32_t (&qf)[4], int m, int k) {
-    ldsm4(qf, q_addr + m * 16 * 2 * kHeadDim + (((2 * k + (lane >> 4)) ^ (lane & 7)) << 4));
-  };
+  const uint32_t q_addr = smem_u32(queries) + (lane & 15) * 2 * kHeadDim + (((lane >> 4) ^ (lane & 7)) << 4);
+  auto query = [&](uint32_t (&qf)[4], int m, int k) { ldsm4(qf, (q_addr ^ (k << 5)) + m * 16 * 2 * kHeadDim); };
 
-  float acc[kTiles][16][4], m_ref[kTiles][2], l[kTiles][2];
-  int limit[kTiles][2];        // keys that the row sees
-  float row_scale[kTiles][2];  // e4m3: power of two of the row's queries
-  auto row_scales = [&]() {
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) row_scale[m][half] = kFp8 ? sm->q_scale[m * 16 + half * 8 + g] : 1.f;
-  };
-  auto begin_unit = [&]() {
+  fetch_q();
+  int stage = 0;
+  for (int s = first; s < last;) {
+    // ---- a unit, or this CTA's part of it: steps [at.step, at.step + unit_end - s)
+    const bool from_start = at.step == 0;  // its earlier steps are not another CTA's
+    const int unit_end = min(last, s + at.steps - at.step);
+    const bool done = unit_end == s + at.steps - at.step;
     store_q();
     next_unit();
     fetch_q();
+    __syncthreads();  // the queries are there, and the buffers of the unit before are free again
+    float acc[kTiles][16][4], m_ref[kTiles][2], l[kTiles][2];
+    int limit[kTiles][2];        // keys that the row sees; the first of the unit's rows sees the fewest
+    float row_scale[kTiles][2];  // e4m3: power of two of the row's queries
+    const int seen_by_all = a.causal ? at.s.len - at.s.n + 1 : at.s.len;
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
 #pragma unroll
@@ -303,214 +308,205 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
+        const int r = m * 16 + half * 8 + g;
         m_ref[m][half] = -INFINITY;
         l[m][half] = 0.f;
-        limit[m][half] = at.s.len;
-        if (a.causal) limit[m][half] = min(at.s.len, at.s.len - at.s.n + (m * 16 + half * 8 + g) / a.group + 1);
+        limit[m][half] = a.causal ? min(at.s.len, at.s.len - at.s.n + r / a.group + 1) : at.s.len;
+        row_scale[m][half] = kFp8 ? sm->q_scale[r] : 1.f;
       }
     }
-  };
-  fetch_q();
-  begin_unit();
-  __syncthreads();
-  row_scales();
 
-  bool from_start = at.step == 0;  // the unit's earlier steps are not another CTA's
-  int stage = 0;
-  for (int s = first; s < last; ++s) {
-    // ---- keep the loads going
-    if (to_load > 0) {
-      load(stage == 0 ? kRowStages - 1 : stage - 1);
-      if (--to_load > 0) {
-        next_step<kStep>(a, in);
-        entry = entry_of(in);
-      }
-    }
-    cp_async_commit();
-    cp_async_wait<kRowStages - 1>();
-    __syncwarp();
-
-    // ---- one step
-    const uint32_t sk = stage0 + stage * S::kStage, sv = sk + S::kHalf;
-    const int key0 = at.step * kStep + warp * kKeys;
-    float sc[kTiles][kBlocks][4];
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m)
-#pragma unroll
-      for (int j = 0; j < kBlocks; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[m][j][e] = 0.f;
-    float step_scale = a.scale_log2;  // of the step's scores; e4m3: with the keys' power of two
-    int value_exp = 0;                // exponent of the power of two that the values were divided by
-    if constexpr (!kFp8) {
-      // four 8 x 8 matrices: keys 0-7 and 8-15 x two 16-byte pieces
-      const int row = (lane & 7) + ((lane >> 4) << 3), odd = (lane >> 3) & 1;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        uint32_t b[4];
-        ldsm4(b, sk + row * S::kRowBytes + (((2 * k + odd) ^ (row & 7)) << 4));
-#pragma unroll
-        for (int m = 0; m < kTiles; ++m) {
-          uint32_t qf[4];
-          query(qf, m, k);
-          mma16816<kFp8>(sc[m][0], qf, b[0], b[1]);
-          mma16816<kFp8>(sc[m][1], qf, b[2], b[3]);
+#pragma unroll 1
+    for (; s < unit_end; ++s, ++at.step) {
+      // ---- keep the loads going
+      if (to_load > 0) {
+        load(stage == 0 ? kRowStages - 1 : stage - 1);
+        if (--to_load > 0) {
+          next_step<kStep>(a, in);
+          entry = entry_of(in);
         }
       }
-    } else {
-      // The powers of two of this lane's key, relative to the largest of the step
-      const uint32_t* words = reinterpret_cast<const uint32_t*>(stages + stage * S::kStage + 2 * S::kHalf);
-      const uint32_t kw = words[lane], vw = words[kKeys + lane];
-      const int k_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(kw)), kMinScale);
-      const int v_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(vw)), kMinScale);
-      uint32_t ks[4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const float k2 = scale_relative((kw >> (8 * b)) & 0xffu, k_top);
-        ks[b] = pack_f16x2(k2, k2);
-        value_scale[b * kKeys + lane] = (uint16_t)pack_f16x2(scale_relative((vw >> (8 * b)) & 0xffu, v_top), 0.f);
-      }
-      *reinterpret_cast<uint4*>(key_scale + lane * 4) = make_uint4(ks[0], ks[1], ks[2], ks[3]);
+      cp_async_commit();
+      cp_async_wait<kRowStages - 1>();
       __syncwarp();
-      step_scale = a.scale_log2 * exp2_int(k_top - 127);
-      value_exp = v_top - 127;
-      // four matrices: the 32 keys x one piece of 16 values
-      uint32_t mult[kBlocks];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if ((k & 1) == 0) {
-#pragma unroll
-          for (int j = 0; j < kBlocks; ++j) mult[j] = key_scale[(j * 8 + g) * 4 + (k >> 1)];
-        }
-        uint32_t b[4];
-        ldsm4(b, sk + lane * S::kRowBytes + ((k ^ (lane & 7)) << 4));
-        uint32_t qf[kTiles][4];
-#pragma unroll
-        for (int m = 0; m < kTiles; ++m) query(qf[m], m, k);
-#pragma unroll
-        for (int j = 0; j < kBlocks; ++j) {
-          const uint32_t b0 = mul_f16x2(e4m3_f16(b[j]), mult[j]), b1 = mul_f16x2(e4m3_f16_high(b[j]), mult[j]);
-#pragma unroll
-          for (int m = 0; m < kTiles; ++m) mma16816<kFp8>(sc[m][j], qf[m], b0, b1);
-        }
-      }
-    }
 
-    // ---- softmax; a lane holds keys 8 j + 2 t + {0, 1} of rows g and g + 8 of a tile
-    uint32_t pf[kTiles][kBlocks / 2][4];
+      // ---- one step
+      const uint32_t sk = stage0 + stage * S::kStage, sv = sk + S::kHalf;
+      const int key0 = at.step * kStep + warp * kKeys;
+      float sc[kTiles][kBlocks][4];
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-      float top[2] = {-INFINITY, -INFINITY};
+      for (int m = 0; m < kTiles; ++m)
 #pragma unroll
-      for (int j = 0; j < kBlocks; ++j)
+        for (int j = 0; j < kBlocks; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (key0 + j * 8 + 2 * t + (e & 1) >= limit[m][e >> 1]) sc[m][j][e] = -INFINITY;
-          top[e >> 1] = fmaxf(top[e >> 1], sc[m][j][e]);
+          for (int e = 0; e < 4; ++e) sc[m][j][e] = 0.f;
+      float step_scale = a.scale_log2;  // of the step's scores; e4m3: with the keys' power of two
+      int value_exp = 0;                // exponent of the power of two that the values were divided by
+      if constexpr (!kFp8) {
+        // four 8 x 8 matrices: keys 0-7 and 8-15 x two 16-byte pieces
+        const uint32_t k_addr = sk + ((lane & 7) + ((lane >> 4) << 3)) * S::kRowBytes + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          uint32_t b[4];
+          ldsm4(b, k_addr ^ (k << 5));
+#pragma unroll
+          for (int m = 0; m < kTiles; ++m) {
+            uint32_t qf[4];
+            query(qf, m, k);
+            mma16816<kFp8>(sc[m][0], qf, b[0], b[1]);
+            mma16816<kFp8>(sc[m][1], qf, b[2], b[3]);
+          }
         }
+      } else {
+        // The powers of two of this lane's key, relative to the largest of the step
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(stages + stage * S::kStage + 2 * S::kHalf);
+        const uint32_t kw = words[lane], vw = words[kKeys + lane];
+        const int k_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(kw)), kMinScale);
+        const int v_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(vw)), kMinScale);
+        uint32_t ks[4];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
-        top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
-      }
-      // A row's reference is the exponent of its largest term exp2(score) * 2^value_exp; it only moves when a term
-      // exceeds it by 2^8.
-      float c[2], lift[2];
-      bool need[2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        // (not zero, with which hidden scores would make no number)
-        c[half] = kFp8 ? fmaxf(step_scale * row_scale[m][half], 1.2e-38f) : step_scale;
-        top[half] = top[half] == -INFINITY ? -INFINITY : fmaf(top[half], c[half], (float)value_exp);
-        need[half] = top[half] - m_ref[m][half] > 8.f;
-      }
-      if (__any_sync(0xffffffffu, need[0] || need[1])) {
-        float f[2];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          f[half] = need[half] ? fast_exp2(m_ref[m][half] - top[half]) : 1.f;
-          if (need[half]) m_ref[m][half] = top[half];
-          l[m][half] *= f[half];
+        for (int b = 0; b < 4; ++b) {
+          const float k2 = scale_relative((kw >> (8 * b)) & 0xffu, k_top);
+          ks[b] = pack_f16x2(k2, k2);
+          value_scale[b * kKeys + lane] = (uint16_t)pack_f16x2(scale_relative((vw >> (8 * b)) & 0xffu, v_top), 0.f);
         }
+        *reinterpret_cast<uint4*>(key_scale + lane * 4) = make_uint4(ks[0], ks[1], ks[2], ks[3]);
+        __syncwarp();
+        step_scale = a.scale_log2 * exp2_int(k_top - 127);
+        value_exp = v_top - 127;
+        // four matrices: the 32 keys x one piece of 16 values
+        const uint32_t k_addr = sk + lane * S::kRowBytes + ((lane & 7) << 4);
+        uint32_t mult[kBlocks];
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+        for (int k = 0; k < 8; ++k) {
+          if ((k & 1) == 0) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[m][j][e] *= f[e >> 1];
-      }
-      float sum[2] = {0.f, 0.f};
+            for (int j = 0; j < kBlocks; ++j) mult[j] = key_scale[(j * 8 + g) * 4 + (k >> 1)];
+          }
+          uint32_t b[4];
+          ldsm4(b, k_addr ^ (k << 4));
+          uint32_t qf[kTiles][4];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) lift[half] = (float)value_exp - (m_ref[m][half] == -INFINITY ? 0.f : m_ref[m][half]);
+          for (int m = 0; m < kTiles; ++m) query(qf[m], m, k);
 #pragma unroll
-      for (int j = 0; j < kBlocks; ++j) {
-        float p[4];
+          for (int j = 0; j < kBlocks; ++j) {
+            const uint32_t b0 = mul_f16x2(e4m3_f16(b[j]), mult[j]), b1 = mul_f16x2(e4m3_f16_high(b[j]), mult[j]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[e] = fast_exp2(fmaf(sc[m][j][e], c[e >> 1], lift[e >> 1]));
-          sum[e >> 1] += p[e];
-        }
-        if constexpr (kFp8) {
-          pf[m][j >> 1][(j & 1) * 2 + 0] = pack_f16x2(p[0], p[1]);
-          pf[m][j >> 1][(j & 1) * 2 + 1] = pack_f16x2(p[2], p[3]);
-        } else {
-          pf[m][j >> 1][(j & 1) * 2 + 0] = pack_bf16x2(p[0], p[1]);
-          pf[m][j >> 1][(j & 1) * 2 + 1] = pack_bf16x2(p[2], p[3]);
+            for (int m = 0; m < kTiles; ++m) mma16816<kFp8>(sc[m][j], qf[m], b0, b1);
+          }
         }
       }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) l[m][half] = kFp8 ? fmaf(sum[half], exp2_int(-value_exp), l[m][half]) : l[m][half] + sum[half];
-    }
 
-    // ---- values
-    if constexpr (!kFp8) {
-      const int row = lane & 15, odd = lane >> 4;  // keys 0-7, 8-15 x two pieces
+      // ---- softmax; a lane holds keys 8 j + 2 t + {0, 1} of rows g and g + 8 of a tile
+      if (key0 + kKeys > seen_by_all) {
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        uint32_t b[4];
-        ldsm4_t(b, sv + row * S::kRowBytes + (((j + odd) ^ (row & 7)) << 4));
-#pragma unroll
-        for (int m = 0; m < kTiles; ++m) {
-          mma16816<kFp8>(acc[m][j], pf[m][0], b[0], b[1]);
-          mma16816<kFp8>(acc[m][j + 1], pf[m][0], b[2], b[3]);
-        }
-      }
-    } else {
-      // Transposed 16-bit units are pairs of neighbouring values: a lane gets values (2 g, 2 g + 1) of keys (2 t, 2 t + 1) of
-      // each 8; the even ones make one 8-column block of the product and the odd ones the next.
-      uint32_t mult[kBlocks];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        if ((c & 1) == 0) {
+        for (int m = 0; m < kTiles; ++m)
 #pragma unroll
           for (int j = 0; j < kBlocks; ++j)
-            mult[j] = *reinterpret_cast<const uint32_t*>(value_scale + (c >> 1) * kKeys + j * 8 + 2 * t);
-        }
-        uint32_t b[4];
-        ldsm4_t(b, sv + lane * S::kRowBytes + ((c ^ (lane & 7)) << 4));
-        uint32_t even[4], odd[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t x = __byte_perm(b[j], 0, 0x3120);  // the even ones of both keys, then the odd ones
-          even[j] = mul_f16x2(e4m3_f16(x), mult[j]);
-          odd[j] = mul_f16x2(e4m3_f16_high(x), mult[j]);
-        }
+            for (int e = 0; e < 4; ++e)
+              if (key0 + j * 8 + 2 * t + (e & 1) >= limit[m][e >> 1]) sc[m][j][e] = -INFINITY;
+      }
+      // A row's reference is the exponent of its largest term exp2(score) * 2^value_exp; it only moves when a term exceeds
+      // it by 2^8.
+      float c[kTiles][2], top[kTiles][2];
+      bool need = false;
 #pragma unroll
-        for (int m = 0; m < kTiles; ++m) {
-          mma16816<kFp8>(acc[m][2 * c], pf[m][0], even[0], even[1]);
-          mma16816<kFp8>(acc[m][2 * c + 1], pf[m][0], odd[0], odd[1]);
-          mma16816<kFp8>(acc[m][2 * c], pf[m][1], even[2], even[3]);
-          mma16816<kFp8>(acc[m][2 * c + 1], pf[m][1], odd[2], odd[3]);
+      for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float x = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < kBlocks; ++j) x = max3(x, sc[m][j][2 * half], sc[m][j][2 * half + 1]);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          // (not zero, with which hidden scores would make no number)
+          c[m][half] = kFp8 ? fmaxf(step_scale * row_scale[m][half], 1.2e-38f) : step_scale;
+          top[m][half] = x == -INFINITY ? -INFINITY : fmaf(x, c[m][half], (float)value_exp);
+          need |= top[m][half] - m_ref[m][half] > 8.f;
+        }
+      if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const bool moves = top[m][half] - m_ref[m][half] > 8.f;
+            const float f = moves ? fast_exp2(m_ref[m][half] - top[m][half]) : 1.f;
+            if (moves) m_ref[m][half] = top[m][half];
+            l[m][half] *= f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              acc[m][j][2 * half] *= f;
+              acc[m][j][2 * half + 1] *= f;
+            }
+          }
+      }
+      uint32_t pf[kTiles][kBlocks / 2][4];
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float lift = (float)value_exp - (m_ref[m][half] == -INFINITY ? 0.f : m_ref[m][half]);
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < kBlocks; ++j) {
+            const float p0 = fast_exp2(fmaf(sc[m][j][2 * half], c[m][half], lift));
+            const float p1 = fast_exp2(fmaf(sc[m][j][2 * half + 1], c[m][half], lift));
+            sum += p0 + p1;
+            pf[m][j >> 1][(j & 1) * 2 + half] = kFp8 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
+          }
+          l[m][half] = kFp8 ? fmaf(sum, exp2_int(-value_exp), l[m][half]) : l[m][half] + sum;
+        }
+
+      // ---- values
+      if constexpr (!kFp8) {
+        const uint32_t v_addr = sv + (lane & 15) * S::kRowBytes + (((lane >> 4) ^ (lane & 7)) << 4);  // keys 0-7, 8-15 x two pieces
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          uint32_t b[4];
+          ldsm4_t(b, v_addr ^ (j << 4));
+#pragma unroll
+          for (int m = 0; m < kTiles; ++m) {
+            mma16816<kFp8>(acc[m][j], pf[m][0], b[0], b[1]);
+            mma16816<kFp8>(acc[m][j + 1], pf[m][0], b[2], b[3]);
+          }
+        }
+      } else {
+        // Transposed 16-bit units are pairs of neighbouring values: a lane gets values (2 g, 2 g + 1) of keys (2 t, 2 t + 1) of
+        // each 8; the even ones make one 8-column block of the product and the odd ones the next.
+        const uint32_t v_addr = sv + lane * S::kRowBytes + ((lane & 7) << 4);
+        uint32_t mult[kBlocks];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if ((c & 1) == 0) {
+#pragma unroll
+            for (int j = 0; j < kBlocks; ++j)
+              mult[j] = *reinterpret_cast<const uint32_t*>(value_scale + (c >> 1) * kKeys + j * 8 + 2 * t);
+          }
+          uint32_t b[4];
+          ldsm4_t(b, v_addr ^ (c << 4));
+          uint32_t even[4], odd[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t x = __byte_perm(b[j], 0, 0x3120);  // the even ones of both keys, then the odd ones
+            even[j] = mul_f16x2(e4m3_f16(x), mult[j]);
+            odd[j] = mul_f16x2(e4m3_f16_high(x), mult[j]);
+          }
+#pragma unroll
+          for (int m = 0; m < kTiles; ++m) {
+            mma16816<kFp8>(acc[m][2 * c], pf[m][0], even[0], even[1]);
+            mma16816<kFp8>(acc[m][2 * c + 1], pf[m][0], odd[0], odd[1]);
+            mma16816<kFp8>(acc[m][2 * c], pf[m][1], even[2], even[3]);
+            mma16816<kFp8>(acc[m][2 * c + 1], pf[m][1], odd[2], odd[3]);
+          }
         }
       }
-    }
-    __syncwarp();
-    stage = stage + 1 == kRowStages ? 0 : stage + 1;
+      __syncwarp();
+      stage = stage + 1 == kRowStages ? 0 : stage + 1;
 
-    // ---- end of the unit, or of this CTA's part of it
-    const bool done = at.step + 1 == at.steps;
-    if (!done && s + 1 < last) {
-      ++at.step;
-      continue;
     }
+
+    // ---- the warps' states become one
     const int rows = at.s.n * a.group;
 #pragma unroll
     for (int m = 0; m < kTiles; ++m)
@@ -557,6 +553,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
                     x.x += y.x; x.y += y.y;
                   }
                   *p = x;
+                  if ((j & 3) == 3) asm volatile("" ::: "memory");  // (else all of the row is loaded before the first sum)
                 }
               } else {
 #pragma unroll
@@ -570,6 +567,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
                     x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
                   }
                   *p = x;
+                  if ((c & 1) == 1) asm volatile("" ::: "memory");
                 }
               }
             }
@@ -612,13 +610,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       while (row_begin(total, blockIdx.x + n, ctas) < end) ++n;
       a.open[blockIdx.x] = make_int4(at.b, at.h, n, 0);
     }
-    if (s + 1 < last) {
-      at = nx;
-      from_start = true;
-      begin_unit();
-      __syncthreads();  // the buffers are free again, the queries there
-      row_scales();
-    }
+    at = nx;
   }
 }
 
