@@ -147,7 +147,7 @@ int launch_attn_paged(const mb_attn_paged_args* x, void* ws, unsigned long long 
   }
   if (p.row_ctas > 0) {
     // [partial rows | (maximum, sum) | open units]
-    const long long slots = 2ll * p.row_ctas * (p.rows <= 16 ? 16 : 32);
+    const long long slots = 2ll * p.row_ctas * paged_rows_padded(p.rows);
     a.part_o = static_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * kHeadDim);
     a.open = reinterpret_cast<int4*>(a.part_ml + slots);

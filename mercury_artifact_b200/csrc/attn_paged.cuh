@@ -41,6 +41,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream);
 long long paged_rows_workspace(int rows, int ctas);
 int paged_rows_ctas();
+int paged_rows_padded(int rows);
 // The first `rows` keys and values of every sequence with at least min_new new tokens, in bf16 [batch, rows, hkv, 128].
 int launch_read_e4m3(const PagedView& c, void* k_out, void* v_out, int rows, int min_new, int max_new, cudaStream_t stream);
 int launch_paged_tiles(const PagedAttnArgs& a, bool fp8, int ctas, cudaStream_t stream);

@@ -33,9 +33,9 @@ struct RowShape {
   static constexpr int kStage = 2 * kHalf + 2 * kScaleBytes;
   static constexpr int kStep = kKeys * kRowWarps;                  // keys of a CTA's step
   static_assert(kStage % 256 == 0, "rows are aligned to their size");
-  // pitch of the merge buffer, in floats: what the lanes of a warp store together falls into different banks
-  static constexpr int kPitch = kFp8 ? 144 : 136;
 };
+constexpr int kPitch = 132;  // of the merge buffers' rows, in floats: what the lanes of a warp store falls into different banks
+
 
 struct RowSmem {
   int total, warp_sum[kRowWarps];
@@ -46,13 +46,19 @@ struct RowSmem {
 
 template <bool kFp8>
 constexpr int row_smem_bytes() {
-  // merge buffers: two of 16 rows or one of 32
-  return kRowWarps * kRowStages * RowShape<kFp8>::kStage + 32 * 2 * kHeadDim + 32 * RowShape<kFp8>::kPitch * 4 + (int)sizeof(RowSmem);
+  // merge buffers: 32 rows, of as many warps as fit
+  return kRowWarps * kRowStages * RowShape<kFp8>::kStage + 32 * 2 * kHeadDim + 32 * kPitch * 4 + (int)sizeof(RowSmem);
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// An 8 x 8 matrix of 16-bit values, a row's pairs over four lanes, the other way round.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -144,13 +150,13 @@ __device__ __forceinline__ int row_begin(int total, int i, int n) { return (int)
 template <bool kFp8, int kTiles>
 __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
   using S = RowShape<kFp8>;
-  constexpr int kStep = S::kStep, kKeys = S::kKeys, kBlocks = kKeys / 8;
+  constexpr int kStep = S::kStep, kKeys = S::kKeys, kGroups = kKeys / 16;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* stages = smem_raw + warp * (kRowStages * S::kStage);
   uint8_t* queries = smem_raw + kRowWarps * kRowStages * S::kStage;  // rows of 256 bytes, pieces swapped like the keys'
   float* merge = reinterpret_cast<float*>(queries + 32 * 2 * kHeadDim);
-  RowSmem* sm = reinterpret_cast<RowSmem*>(merge + 32 * S::kPitch);
+  RowSmem* sm = reinterpret_cast<RowSmem*>(merge + 32 * kPitch);
   // e4m3: a step's powers of two in f16, twice [32 keys][4 blocks] for the keys, [4 blocks][32 keys] for the values; where
   // the states are merged at a unit's end
   uint32_t* key_scale = reinterpret_cast<uint32_t*>(merge) + warp * 192;
@@ -245,7 +251,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
 
   // Queries: the next unit's are fetched into registers while this one's are in use (from shared memory).
   RowIter nx = at;  // the unit behind this one
-  uint4 qx[kTiles];
+  constexpr int kPasses = (kTiles + 1) / 2;  // sixteen threads have a row, 16 rows at a time
+  uint4 qx[kPasses];
   auto next_unit = [&]() {
     nx.step = 0;
     if (++nx.h < a.c.hkv) return;
@@ -255,7 +262,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   };
   auto fetch_q = [&]() {
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
+    for (int m = 0; m < kPasses; ++m) {
       const int r = m * 16 + (tid >> 4), tok = r / a.group, hd = r - tok * a.group;
       qx[m] = make_uint4(0, 0, 0, 0);
       if (nx.b < a.c.batch && r < nx.s.n * a.group)
@@ -267,7 +274,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   // it gets four neighbouring values at once, so that its two pairs are 4 t .. 4 t + 3; the queries are put in that order.
   auto store_q = [&]() {
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
+    for (int m = 0; m < kPasses; ++m) {
       const int r = m * 16 + (tid >> 4), piece = tid & 15;
       uint8_t* row = queries + r * 2 * kHeadDim;
       if constexpr (kFp8) {
@@ -282,8 +289,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       }
     }
   };
-  const uint32_t q_addr = smem_u32(queries) + (lane & 15) * 2 * kHeadDim + (((lane >> 4) ^ (lane & 7)) << 4);
-  auto query = [&](uint32_t (&qf)[4], int m, int k) { ldsm4(qf, (q_addr ^ (k << 5)) + m * 16 * 2 * kHeadDim); };
+  // Queries of 8 rows as the second operand, for 32 elements along head_dim (two products)
+  const uint32_t q_addr = smem_u32(queries) + (lane & 7) * 2 * kHeadDim + (((lane >> 3) ^ (lane & 7)) << 4);
+  auto queries_of = [&](uint32_t (&qf)[4], int m, int k2) { ldsm4(qf, (q_addr ^ (k2 << 6)) + m * 8 * 2 * kHeadDim); };
+  constexpr bool kKeepQ = kTiles <= 2;  // in registers for the unit
 
   fetch_q();
   int stage = 0;
@@ -296,24 +305,28 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     next_unit();
     fetch_q();
     __syncthreads();  // the queries are there, and the buffers of the unit before are free again
-    float acc[kTiles][16][4], m_ref[kTiles][2], l[kTiles][2];
+    float acc[kTiles][8][4], m_ref[kTiles][2], l[kTiles][2];
     int limit[kTiles][2];        // keys that the row sees; the first of the unit's rows sees the fewest
     float row_scale[kTiles][2];  // e4m3: power of two of the row's queries
+    uint32_t qk[kKeepQ ? kTiles : 1][4][4];
     const int seen_by_all = a.causal ? at.s.len - at.s.n + 1 : at.s.len;
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
+      for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = m * 16 + half * 8 + g;
-        m_ref[m][half] = -INFINITY;
-        l[m][half] = 0.f;
-        limit[m][half] = a.causal ? min(at.s.len, at.s.len - at.s.n + r / a.group + 1) : at.s.len;
-        row_scale[m][half] = kFp8 ? sm->q_scale[r] : 1.f;
+      for (int e = 0; e < 2; ++e) {
+        const int r = m * 8 + 2 * t + e;
+        m_ref[m][e] = -INFINITY;
+        l[m][e] = 0.f;
+        limit[m][e] = a.causal ? min(at.s.len, at.s.len - at.s.n + r / a.group + 1) : at.s.len;
+        row_scale[m][e] = kFp8 ? sm->q_scale[r] : 1.f;
       }
+      if constexpr (kKeepQ)
+#pragma unroll
+        for (int k2 = 0; k2 < 4; ++k2) queries_of(qk[m][k2], m, k2);
     }
 
 #pragma unroll 1
@@ -333,28 +346,30 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       // ---- one step
       const uint32_t sk = stage0 + stage * S::kStage, sv = sk + S::kHalf;
       const int key0 = at.step * kStep + warp * kKeys;
-      float sc[kTiles][kBlocks][4];
+      float sc[kTiles][kGroups][4];  // of 16 keys each
 #pragma unroll
       for (int m = 0; m < kTiles; ++m)
 #pragma unroll
-        for (int j = 0; j < kBlocks; ++j)
+        for (int j = 0; j < kGroups; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[m][j][e] = 0.f;
       float step_scale = a.scale_log2;  // of the step's scores; e4m3: with the keys' power of two
       int value_exp = 0;                // exponent of the power of two that the values were divided by
       if constexpr (!kFp8) {
-        // four 8 x 8 matrices: keys 0-7 and 8-15 x two 16-byte pieces
-        const uint32_t k_addr = sk + ((lane & 7) + ((lane >> 4) << 3)) * S::kRowBytes + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+        // four 8 x 8 matrices: keys 0-7 and 8-15 of one 16-byte piece, then of the next
+        const uint32_t k_addr = sk + (lane & 15) * S::kRowBytes + (((lane >> 4) ^ (lane & 7)) << 4);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          uint32_t b[4];
-          ldsm4(b, k_addr ^ (k << 5));
+        for (int k2 = 0; k2 < 4; ++k2) {
+          uint32_t k0[4], k1[4];
+          ldsm4(k0, k_addr ^ (k2 << 6));
+          ldsm4(k1, k_addr ^ (k2 << 6) ^ 32);
 #pragma unroll
           for (int m = 0; m < kTiles; ++m) {
             uint32_t qf[4];
-            query(qf, m, k);
-            mma16816<kFp8>(sc[m][0], qf, b[0], b[1]);
-            mma16816<kFp8>(sc[m][1], qf, b[2], b[3]);
+            if constexpr (!kKeepQ) queries_of(qf, m, k2);
+            const uint32_t(&q)[4] = kKeepQ ? qk[kKeepQ ? m : 0][k2] : qf;
+            mma16816<kFp8>(sc[m][0], k0, q[0], q[1]);
+            mma16816<kFp8>(sc[m][0], k1, q[2], q[3]);
           }
         }
       } else {
@@ -374,130 +389,140 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         __syncwarp();
         step_scale = a.scale_log2 * exp2_int(k_top - 127);
         value_exp = v_top - 127;
-        // four matrices: the 32 keys x one piece of 16 values
+        // four matrices: the 32 keys x one piece of 16 values, which makes two operands of 16 keys x 16 values
         const uint32_t k_addr = sk + lane * S::kRowBytes + ((lane & 7) << 4);
-        uint32_t mult[kBlocks];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if ((k & 1) == 0) {
+        for (int k2 = 0; k2 < 4; ++k2) {
+          uint32_t mult[4];
 #pragma unroll
-            for (int j = 0; j < kBlocks; ++j) mult[j] = key_scale[(j * 8 + g) * 4 + (k >> 1)];
+          for (int j = 0; j < 4; ++j) mult[j] = key_scale[(j * 8 + g) * 4 + k2];
+          uint32_t kf[2][2][4];  // [piece][16 keys]
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t b[4];
+            ldsm4(b, k_addr ^ ((2 * k2 + i) << 4));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              kf[i][j][0] = mul_f16x2(e4m3_f16(b[2 * j]), mult[2 * j]);
+              kf[i][j][1] = mul_f16x2(e4m3_f16(b[2 * j + 1]), mult[2 * j + 1]);
+              kf[i][j][2] = mul_f16x2(e4m3_f16_high(b[2 * j]), mult[2 * j]);
+              kf[i][j][3] = mul_f16x2(e4m3_f16_high(b[2 * j + 1]), mult[2 * j + 1]);
+            }
           }
-          uint32_t b[4];
-          ldsm4(b, k_addr ^ (k << 4));
-          uint32_t qf[kTiles][4];
 #pragma unroll
-          for (int m = 0; m < kTiles; ++m) query(qf[m], m, k);
+          for (int m = 0; m < kTiles; ++m) {
+            uint32_t qf[4];
+            if constexpr (!kKeepQ) queries_of(qf, m, k2);
+            const uint32_t(&q)[4] = kKeepQ ? qk[kKeepQ ? m : 0][k2] : qf;
 #pragma unroll
-          for (int j = 0; j < kBlocks; ++j) {
-            const uint32_t b0 = mul_f16x2(e4m3_f16(b[j]), mult[j]), b1 = mul_f16x2(e4m3_f16_high(b[j]), mult[j]);
-#pragma unroll
-            for (int m = 0; m < kTiles; ++m) mma16816<kFp8>(sc[m][j], qf[m], b0, b1);
+            for (int j = 0; j < 2; ++j) {
+              mma16816<kFp8>(sc[m][j], kf[0][j], q[0], q[1]);
+              mma16816<kFp8>(sc[m][j], kf[1][j], q[2], q[3]);
+            }
           }
         }
       }
 
-      // ---- softmax; a lane holds keys 8 j + 2 t + {0, 1} of rows g and g + 8 of a tile
+      // ---- softmax; a lane holds keys 16 j + g and 16 j + 8 + g of rows 2 t and 2 t + 1 of a tile
       if (key0 + kKeys > seen_by_all) {
 #pragma unroll
         for (int m = 0; m < kTiles; ++m)
 #pragma unroll
-          for (int j = 0; j < kBlocks; ++j)
+          for (int j = 0; j < kGroups; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (key0 + j * 8 + 2 * t + (e & 1) >= limit[m][e >> 1]) sc[m][j][e] = -INFINITY;
+              if (key0 + j * 16 + (e >> 1) * 8 + g >= limit[m][e & 1]) sc[m][j][e] = -INFINITY;
       }
       // A row's reference is the exponent of its largest term exp2(score) * 2^value_exp; it only moves when a term exceeds
-      // it by 2^8.
+      // it by 2^8.  Each lane looks at its own keys, and the row's maximum is only taken when one of them does.
       float c[kTiles][2], top[kTiles][2];
       bool need = false;
 #pragma unroll
       for (int m = 0; m < kTiles; ++m)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float x = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < kBlocks; ++j) x = max3(x, sc[m][j][2 * half], sc[m][j][2 * half + 1]);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(sc[m][0][e], sc[m][0][2 + e]);
+          if constexpr (kGroups == 2) x = max3(x, sc[m][kGroups - 1][e], sc[m][kGroups - 1][2 + e]);
           // (not zero, with which hidden scores would make no number)
-          c[m][half] = kFp8 ? fmaxf(step_scale * row_scale[m][half], 1.2e-38f) : step_scale;
-          top[m][half] = x == -INFINITY ? -INFINITY : fmaf(x, c[m][half], (float)value_exp);
-          need |= top[m][half] - m_ref[m][half] > 8.f;
+          c[m][e] = kFp8 ? fmaxf(step_scale * row_scale[m][e], 1.2e-38f) : step_scale;
+          top[m][e] = x == -INFINITY ? -INFINITY : fmaf(x, c[m][e], (float)value_exp);
+          need |= top[m][e] - m_ref[m][e] > 8.f;
         }
       if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
         for (int m = 0; m < kTiles; ++m)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const bool moves = top[m][half] - m_ref[m][half] > 8.f;
-            const float f = moves ? fast_exp2(m_ref[m][half] - top[m][half]) : 1.f;
-            if (moves) m_ref[m][half] = top[m][half];
-            l[m][half] *= f;
+          for (int e = 0; e < 2; ++e) {
+            float x = top[m][e];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              acc[m][j][2 * half] *= f;
-              acc[m][j][2 * half + 1] *= f;
+            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            const bool moves = x - m_ref[m][e] > 8.f;
+            const float f = moves ? fast_exp2(m_ref[m][e] - x) : 1.f;
+            if (moves) m_ref[m][e] = x;
+            l[m][e] *= f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              acc[m][j][e] *= f;
+              acc[m][j][2 + e] *= f;
             }
           }
       }
-      uint32_t pf[kTiles][kBlocks / 2][4];
+      uint32_t pf[kTiles][kGroups][2];  // probabilities as the second operand: [16 keys][rows], keys 0-7 and 8-15
 #pragma unroll
-      for (int m = 0; m < kTiles; ++m)
+      for (int m = 0; m < kTiles; ++m) {
+        float lift[2], sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float lift = (float)value_exp - (m_ref[m][half] == -INFINITY ? 0.f : m_ref[m][half]);
-          float sum = 0.f;
+        for (int e = 0; e < 2; ++e) lift[e] = (float)value_exp - (m_ref[m][e] == -INFINITY ? 0.f : m_ref[m][e]);
 #pragma unroll
-          for (int j = 0; j < kBlocks; ++j) {
-            const float p0 = fast_exp2(fmaf(sc[m][j][2 * half], c[m][half], lift));
-            const float p1 = fast_exp2(fmaf(sc[m][j][2 * half + 1], c[m][half], lift));
-            sum += p0 + p1;
-            pf[m][j >> 1][(j & 1) * 2 + half] = kFp8 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
+        for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float p0 = fast_exp2(fmaf(sc[m][j][2 * i], c[m][0], lift[0]));
+            const float p1 = fast_exp2(fmaf(sc[m][j][2 * i + 1], c[m][1], lift[1]));
+            sum[0] += p0;
+            sum[1] += p1;
+            pf[m][j][i] = transpose8x8(kFp8 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1));
           }
-          l[m][half] = kFp8 ? fmaf(sum, exp2_int(-value_exp), l[m][half]) : l[m][half] + sum;
-        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[m][e] = kFp8 ? fmaf(sum[e], exp2_int(-value_exp), l[m][e]) : l[m][e] + sum[e];
+      }
 
-      // ---- values
+      // ---- values, transposed, as the first operand: 16 columns x 16 keys
       if constexpr (!kFp8) {
-        const uint32_t v_addr = sv + (lane & 15) * S::kRowBytes + (((lane >> 4) ^ (lane & 7)) << 4);  // keys 0-7, 8-15 x two pieces
+        // four matrices: two pieces of 8 values of keys 0-7, then of keys 8-15
+        const uint32_t v_addr = sv + ((lane & 7) + ((lane >> 4) << 3)) * S::kRowBytes + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          uint32_t b[4];
-          ldsm4_t(b, v_addr ^ (j << 4));
+        for (int j = 0; j < 8; ++j) {
+          uint32_t v[4];
+          ldsm4_t(v, v_addr ^ (j << 5));
 #pragma unroll
-          for (int m = 0; m < kTiles; ++m) {
-            mma16816<kFp8>(acc[m][j], pf[m][0], b[0], b[1]);
-            mma16816<kFp8>(acc[m][j + 1], pf[m][0], b[2], b[3]);
-          }
+          for (int m = 0; m < kTiles; ++m) mma16816<kFp8>(acc[m][j], v, pf[m][0][0], pf[m][0][1]);
         }
       } else {
         // Transposed 16-bit units are pairs of neighbouring values: a lane gets values (2 g, 2 g + 1) of keys (2 t, 2 t + 1) of
-        // each 8; the even ones make one 8-column block of the product and the odd ones the next.
+        // each 8; the even ones are the product's rows 0-7, the odd ones rows 8-15.
         const uint32_t v_addr = sv + lane * S::kRowBytes + ((lane & 7) << 4);
-        uint32_t mult[kBlocks];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          if ((c & 1) == 0) {
+        for (int j2 = 0; j2 < 4; ++j2) {
+          uint32_t mult[4];
 #pragma unroll
-            for (int j = 0; j < kBlocks; ++j)
-              mult[j] = *reinterpret_cast<const uint32_t*>(value_scale + (c >> 1) * kKeys + j * 8 + 2 * t);
-          }
-          uint32_t b[4];
-          ldsm4_t(b, v_addr ^ (c << 4));
-          uint32_t even[4], odd[4];
+          for (int i = 0; i < 4; ++i) mult[i] = *reinterpret_cast<const uint32_t*>(value_scale + j2 * kKeys + i * 8 + 2 * t);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t x = __byte_perm(b[j], 0, 0x3120);  // the even ones of both keys, then the odd ones
-            even[j] = mul_f16x2(e4m3_f16(x), mult[j]);
-            odd[j] = mul_f16x2(e4m3_f16_high(x), mult[j]);
-          }
+          for (int j = 2 * j2; j < 2 * j2 + 2; ++j) {
+            uint32_t b[4];
+            ldsm4_t(b, v_addr ^ (j << 4));
+            uint32_t v[2][4];
 #pragma unroll
-          for (int m = 0; m < kTiles; ++m) {
-            mma16816<kFp8>(acc[m][2 * c], pf[m][0], even[0], even[1]);
-            mma16816<kFp8>(acc[m][2 * c + 1], pf[m][0], odd[0], odd[1]);
-            mma16816<kFp8>(acc[m][2 * c], pf[m][1], even[2], even[3]);
-            mma16816<kFp8>(acc[m][2 * c + 1], pf[m][1], odd[2], odd[3]);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t x = __byte_perm(b[i], 0, 0x3120);  // the even ones of both keys, then the odd ones
+              v[i >> 1][(i & 1) * 2] = mul_f16x2(e4m3_f16(x), mult[i]);
+              v[i >> 1][(i & 1) * 2 + 1] = mul_f16x2(e4m3_f16_high(x), mult[i]);
+            }
+#pragma unroll
+            for (int m = 0; m < kTiles; ++m) {
+              mma16816<kFp8>(acc[m][j], v[0], pf[m][0][0], pf[m][0][1]);
+              mma16816<kFp8>(acc[m][j], v[1], pf[m][kGroups - 1][0], pf[m][kGroups - 1][1]);
+            }
           }
         }
       }
@@ -511,64 +536,51 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
 #pragma unroll
     for (int m = 0; m < kTiles; ++m)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float x = l[m][half];
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        x += __shfl_xor_sync(0xffffffffu, x, 2);
-        if (t == 0) sm->ml[warp][m * 16 + half * 8 + g] = make_float2(m_ref[m][half], x);
+      for (int e = 0; e < 2; ++e) {
+        float x = l[m][e];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+        if (g == 0) sm->ml[warp][m * 8 + 2 * t + e] = make_float2(m_ref[m][e], x);
       }
     __syncthreads();
     float f[kTiles][2];
 #pragma unroll
     for (int m = 0; m < kTiles; ++m)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int e = 0; e < 2; ++e) {
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm->ml[w][m * 16 + half * 8 + g].x);
-        f[m][half] = m_ref[m][half] == -INFINITY ? 0.f : fast_exp2(m_ref[m][half] - top);
+        for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm->ml[w][m * 8 + 2 * t + e].x);
+        f[m][e] = m_ref[m][e] == -INFINITY ? 0.f : fast_exp2(m_ref[m][e] - top);
         // a warp without a visible key has nothing, whatever its masked products gave
-        if (m_ref[m][half] == -INFINITY && !(l[m][half] != l[m][half])) {
+        const float mine = sm->ml[warp][m * 8 + 2 * t + e].y;
+        if (m_ref[m][e] == -INFINITY && mine == mine) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) acc[m][j][2 * half] = acc[m][j][2 * half + 1] = 0.f;
+          for (int j = 0; j < 8; ++j) acc[m][j][e] = acc[m][j][2 + e] = 0.f;
         }
       }
-    constexpr int kBuffers = 2 / kTiles;
+    constexpr int kBuffers = 4 / kTiles;
+#pragma unroll 1
     for (int round = 0; round < kRowWarps / kBuffers; ++round) {
       if (warp / kBuffers == round) {
-        float* buf = merge + (kTiles == 1 ? (warp & 1) * 16 * S::kPitch : 0);
+        float* buf = merge + (warp % kBuffers) * 8 * kTiles * kPitch;
 #pragma unroll
         for (int m = 0; m < kTiles; ++m)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int r = m * 16 + half * 8 + g;
+          for (int e = 0; e < 2; ++e) {
+            const int r = m * 8 + 2 * t + e;
             if (r < rows) {
-              if constexpr (!kFp8) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                  float2* p = reinterpret_cast<float2*>(buf + r * S::kPitch + j * 8 + t * 2);
-                  float2 x = make_float2(acc[m][j][2 * half] * f[m][half], acc[m][j][2 * half + 1] * f[m][half]);
-                  if (round > 0) {
-                    const float2 y = *p;
-                    x.x += y.x; x.y += y.y;
-                  }
-                  *p = x;
-                  if ((j & 3) == 3) asm volatile("" ::: "memory");  // (else all of the row is loaded before the first sum)
+              for (int j = 0; j < 8; ++j) {
+                // columns 16 j + g and 16 j + 8 + g; e4m3: 16 j + 2 g and the next
+                float* p = buf + r * kPitch + j * 16 + (kFp8 ? 2 * g : g);
+                float x0 = acc[m][j][e] * f[m][e], x1 = acc[m][j][2 + e] * f[m][e];
+                if (round > 0) {
+                  x0 += p[0];
+                  x1 += p[kFp8 ? 1 : 8];
                 }
-              } else {
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                  float4* p = reinterpret_cast<float4*>(buf + r * S::kPitch + c * 16 + t * 4);
-                  const float* ev = acc[m][2 * c] + 2 * half;
-                  const float* od = acc[m][2 * c + 1] + 2 * half;
-                  float4 x = make_float4(ev[0] * f[m][half], od[0] * f[m][half], ev[1] * f[m][half], od[1] * f[m][half]);
-                  if (round > 0) {
-                    const float4 y = *p;
-                    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-                  }
-                  *p = x;
-                  if ((c & 1) == 1) asm volatile("" ::: "memory");
-                }
+                p[0] = x0;
+                p[kFp8 ? 1 : 8] = x1;
               }
             }
           }
@@ -586,9 +598,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         const float2 x = sm->ml[w][r];
         sum += x.x == -INFINITY ? x.y : x.y * fast_exp2(x.x - top);
       }
-      float4 x = *reinterpret_cast<const float4*>(merge + r * S::kPitch + lane * 4);
-      if constexpr (kTiles == 1) {
-        const float4 y = *reinterpret_cast<const float4*>(merge + (16 + r) * S::kPitch + lane * 4);
+      float4 x = *reinterpret_cast<const float4*>(merge + r * kPitch + lane * 4);
+#pragma unroll
+      for (int i = 1; i < kBuffers; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(merge + (i * 8 * kTiles + r) * kPitch + lane * 4);
         x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
       }
       if (whole) {
@@ -599,8 +612,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         if (lane == 0)
           a.lse[at.b * a.lse_sb + hd * a.lse_sh + at.s.start + tok] = sum == 0.f ? -INFINITY : top * kLn2 + __logf(sum);
       } else {
-        *reinterpret_cast<float4*>(a.part_o + ((long long)slot * (16 * kTiles) + r) * kHeadDim + lane * 4) = x;
-        if (lane == 0) a.part_ml[slot * (16 * kTiles) + r] = make_float2(top, sum);
+        *reinterpret_cast<float4*>(a.part_o + ((long long)slot * (8 * kTiles) + r) * kHeadDim + lane * 4) = x;
+        if (lane == 0) a.part_ml[slot * (8 * kTiles) + r] = make_float2(top, sum);
       }
     }
     if (from_start && !done && tid == 0) {
@@ -667,9 +680,11 @@ __global__ void __launch_bounds__(kRowThreads) paged_merge_kernel(const __grid_c
 
 int paged_rows_ctas() { return sm_count(); }
 
+// Rows that the kernel is compiled for
+int paged_rows_padded(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+
 long long paged_rows_workspace(int rows, int ctas) {
-  const int padded = rows <= 16 ? 16 : 32;
-  return 2ll * ctas * padded * (kHeadDim * (long long)sizeof(float) + (long long)sizeof(float2)) + ctas * (long long)sizeof(int4);
+  return 2ll * ctas * paged_rows_padded(rows) * (kHeadDim * (long long)sizeof(float) + (long long)sizeof(float2)) + ctas * (long long)sizeof(int4);
 }
 
 template <bool kFp8, int kTiles>
@@ -687,15 +702,18 @@ static int launch_rows(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   }
   if (!launch_overlapped("launch paged_rows_kernel", paged_rows_kernel<kFp8, kTiles>, dim3(ctas), kRowThreads, bytes, stream, a))
     return MB_E_CUDA;
-  if (!launch_overlapped("launch paged_merge_kernel", paged_merge_kernel<16 * kTiles>,
+  if (!launch_overlapped("launch paged_merge_kernel", paged_merge_kernel<8 * kTiles>,
                          dim3(ctas, min(a.few, a.max_queries * a.group)), kRowThreads, 0, stream, a))
     return MB_E_CUDA;
   return MB_SUCCESS;
 }
 
 int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream) {
-  if (rows <= 16) return fp8 ? launch_rows<true, 1>(a, ctas, stream) : launch_rows<false, 1>(a, ctas, stream);
-  return fp8 ? launch_rows<true, 2>(a, ctas, stream) : launch_rows<false, 2>(a, ctas, stream);
+  switch (paged_rows_padded(rows)) {
+    case 8: return fp8 ? launch_rows<true, 1>(a, ctas, stream) : launch_rows<false, 1>(a, ctas, stream);
+    case 16: return fp8 ? launch_rows<true, 2>(a, ctas, stream) : launch_rows<false, 2>(a, ctas, stream);
+    default: return fp8 ? launch_rows<true, 4>(a, ctas, stream) : launch_rows<false, 4>(a, ctas, stream);
+  }
 }
 
 }  // namespace mb
