@@ -19,7 +19,6 @@ status 110, and raised by PagedKV.check().  Sequences may share pages that are o
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional, Tuple
 
 import torch
@@ -75,13 +74,11 @@ class PagedKV:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.device, self.dtype = k.device, k.dtype
         self.pages, self.page_size, self.heads = pages, page_size, heads
-        a = _lib.PagedKVArgs()
-        a.k, a.v = k.data_ptr(), v.data_ptr()
-        a.stride_page, a.stride_slot, a.stride_h = k.stride()[:3]
-        if k_scale is not None:
-            a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-        a.pages, a.page_size, a.hkv, a.head_dim, a.dtype = pages, page_size, heads, d, _DTYPES[k.dtype]
-        self._args = a
+        # the first fields of the calls' argument block
+        self._head = (k.data_ptr(), v.data_ptr(), *k.stride()[:3], k_scale.data_ptr() if k_scale is not None else 0,
+                      v_scale.data_ptr() if v_scale is not None else 0)
+        self._tail = (pages, page_size)
+        self._kind = (heads, d, _DTYPES[k.dtype], 0)
 
     @classmethod
     def empty(cls, pages: int, page_size: int, heads: int, dtype: torch.dtype = torch.bfloat16,
@@ -102,48 +99,51 @@ class PagedKV:
         with _on(self.device):
             _lib.raise_on_status(_stream_ptr())
 
-    def _fill(self, a, page_table, seq_lens, cu_seqlens, tokens) -> None:
-        """The batch's part of the arguments."""
-        if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    def _batch(self, page_table, seq_lens, cu_seqlens, tokens: int) -> tuple:
+        """The argument block of a call on this batch (_lib.PagedKVArgs), as values to pack."""
+        dev = self.device
+        shape = page_table.shape
+        if len(shape) != 2 or page_table.dtype != torch.int32 or (shape[1] > 1 and page_table.stride(1) != 1):
             raise ValueError("page_table must be int32 [batch, max_pages] with contiguous rows")
-        b = page_table.shape[0]
-        if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or seq_lens.shape[0] != b or not seq_lens.is_contiguous():
+        b, columns = shape
+        if seq_lens.dtype != torch.int32 or seq_lens.shape != (b,) or not seq_lens.is_contiguous():
             raise ValueError(f"seq_lens must be contiguous int32 [{b}]")
+        if page_table.device != dev or seq_lens.device != dev:
+            raise ValueError(f"page_table and seq_lens must be on {dev}, where the cache is")
+        cu = 0
         if cu_seqlens is not None:
-            if (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] != b + 1
-                    or not cu_seqlens.is_contiguous()):
+            if cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (b + 1,) or not cu_seqlens.is_contiguous():
                 raise ValueError(f"cu_seqlens must be contiguous int32 [{b + 1}]")
-            if cu_seqlens.device != self.device:
-                raise ValueError(f"cu_seqlens must be on {self.device}, where the cache is")
-            a.cu_seqlens = cu_seqlens.data_ptr()
-        if page_table.device != self.device or seq_lens.device != self.device:
-            raise ValueError(f"page_table and seq_lens must be on {self.device}, where the cache is")
-        if page_table.shape[1] * self.page_size > 0x7fffff00:
+            if cu_seqlens.device != dev:
+                raise ValueError(f"cu_seqlens must be on {dev}, where the cache is")
+            cu = cu_seqlens.data_ptr()
+        if columns * self.page_size > 0x7fffff00:
             raise ValueError("a page table may cover at most 2147483392 keys")
-        a.page_table, a.page_table_stride = page_table.data_ptr(), page_table.stride(0)
-        a.seq_lens = seq_lens.data_ptr()
-        a.batch, a.max_pages, a.tokens = b, page_table.shape[1], tokens
+        if tokens > 0x7fffffff:
+            raise ValueError("at most 2147483647 new tokens per call")
+        return (*self._head, page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr(), cu, b, tokens, *self._tail,
+                columns, *self._kind)
 
 
-def _check_rows(t: torch.Tensor, name: str, cache: PagedKV, dims: int) -> None:
-    if t.dim() != dims:
+def _rows(t: torch.Tensor, name: str, cache: PagedKV, dims: int) -> tuple:
+    """(address, batch stride, token stride, head stride) of [(batch,) tokens, heads, head_dim] rows, checked."""
+    shape, stride, ptr = t.shape, t.stride(), t.data_ptr()
+    if len(shape) != dims:
         want = "[tokens, heads, head_dim]" if dims == 3 else "[batch, tokens, heads, head_dim]"
-        raise ValueError(f"{name} must be {want}, got {tuple(t.shape)}")
+        raise ValueError(f"{name} must be {want}, got {tuple(shape)}")
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
     if t.device != cache.device:
         raise ValueError(f"{name} must be on {cache.device}, where the cache is")
-    if t.shape[-1] != HEAD_DIM or t.stride(-1) != 1:
+    if shape[-1] != HEAD_DIM or stride[-1] != 1:
         raise ValueError(f"{name}: head_dim must be {HEAD_DIM} and contiguous")
     # (the stride of a dimension of one entry is never used)
-    if t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+    sh = stride[-2] if shape[-2] > 1 else 0
+    st = stride[-3] if shape[-3] > 1 else 0
+    sb = stride[0] if dims == 4 and shape[0] > 1 else 0
+    if (ptr | sb * 2 | st * 2 | sh * 2) & 15:
         raise ValueError(f"{name}: address and strides must be multiples of 16 bytes")
-
-
-def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
-    """(batch, token, head) strides of a tensor that _check_rows has seen."""
-    s = [x if n > 1 else 0 for x, n in zip(t.stride()[:-1], t.shape)]
-    return (s[0], s[1], s[2]) if len(s) == 3 else (0, s[0], s[1])
+    return ptr, sb, st, sh
 
 
 def kv_cache_write(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -156,19 +156,18 @@ def kv_cache_write(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table:
     last ones of the seq_lens[b] keys; where a sequence has more of them than keys, the first ones are not stored.  No
     two new tokens may lie in the same slot."""
     dims = 3 if cu_seqlens is not None else 4
-    _check_rows(k, "k", cache, dims)
-    _check_rows(v, "v", cache, dims)
-    if k.shape != v.shape or _strides(k) != _strides(v):
+    shape = k.shape
+    k_ptr, *strides = _rows(k, "k", cache, dims)
+    v_ptr, *v_strides = _rows(v, "v", cache, dims)
+    if shape != v.shape or strides != v_strides:
         raise ValueError("k and v must share shape and strides")
-    if k.shape[-2] != cache.heads:
-        raise ValueError(f"k, v have {k.shape[-2]} heads, the cache {cache.heads}")
-    a = _lib.PagedKVArgs.from_buffer_copy(cache._args)
-    cache._fill(a, page_table, seq_lens, cu_seqlens, k.shape[0] if dims == 3 else k.shape[0] * k.shape[1])
-    if dims == 4 and k.shape[0] != a.batch:
-        raise ValueError(f"k, v have batch {k.shape[0]}, page_table {a.batch}")
+    if shape[-2] != cache.heads:
+        raise ValueError(f"k, v have {shape[-2]} heads, the cache {cache.heads}")
+    if dims == 4 and shape[0] != page_table.shape[0]:
+        raise ValueError(f"k, v have batch {shape[0]}, page_table {page_table.shape[0]}")
+    args = _lib.PAGED_KV.pack(*cache._batch(page_table, seq_lens, cu_seqlens, shape[0] if dims == 3 else shape[0] * shape[1]))
     with _on(cache.device):
-        _lib.check(_lib.lib.mb_kv_cache_write(C.byref(a), k.data_ptr(), v.data_ptr(), *_strides(k), _stream_ptr()),
-                   "mb_kv_cache_write")
+        _lib.check(_lib.lib.mb_kv_cache_write(args, k_ptr, v_ptr, *strides, _stream_ptr()), "mb_kv_cache_write")
 
 
 def kv_cache_read(cache: PagedKV, page_table: torch.Tensor, seq_lens: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -178,23 +177,25 @@ def kv_cache_read(cache: PagedKV, page_table: torch.Tensor, seq_lens: torch.Tens
     out: the buffer to write to; rows behind a sequence's last key are left as they are, keys beyond its rows are left out.
     Without it a zero-filled one of max_keys rows is made (default: what the page table covers).  Values of a
     float8_e4m3fn cache are exact: the code times its power of two."""
-    a = _lib.PagedKVArgs.from_buffer_copy(cache._args)
-    cache._fill(a, page_table, seq_lens, None, 0)
+    args = cache._batch(page_table, seq_lens, None, 0)
+    b, columns = page_table.shape
     if out is None:
-        rows = a.max_pages * cache.page_size if max_keys is None else int(max_keys)
+        rows = columns * cache.page_size if max_keys is None else int(max_keys)
         if rows < 0:
             raise ValueError("max_keys must not be negative")
-        out = torch.zeros((2, a.batch, rows, cache.heads, HEAD_DIM), dtype=torch.bfloat16, device=cache.device)
-    elif max_keys is not None and (out.dim() != 5 or out.shape[2] != max_keys):
+        out = torch.zeros((2, b, rows, cache.heads, HEAD_DIM), dtype=torch.bfloat16, device=cache.device)
+    shape = out.shape
+    if len(shape) != 5 or shape[0] != 2 or shape[1] != b or shape[3] != cache.heads:
+        raise ValueError(f"out must be [2, {b}, rows, {cache.heads}, {HEAD_DIM}], got {tuple(shape)}")
+    if max_keys is not None and shape[2] != max_keys:
         raise ValueError("out must have max_keys rows")
-    if out.dim() != 5 or out.shape[0] != 2 or out.shape[1] != a.batch or out.shape[3] != cache.heads:
-        raise ValueError(f"out must be [2, {a.batch}, rows, {cache.heads}, {HEAD_DIM}], got {tuple(out.shape)}")
-    k, v = out[0], out[1]
-    _check_rows(k, "out", cache, 4)
-    _check_rows(v, "out", cache, 4)
+    ptr, *strides = _rows(out[0], "out", cache, 4)
+    half = out.stride(0) * 2
+    if half % 16:
+        raise ValueError("out: address and strides must be multiples of 16 bytes")
     with _on(cache.device):
-        _lib.check(_lib.lib.mb_kv_cache_read(C.byref(a), k.data_ptr(), v.data_ptr(), *_strides(k), out.shape[2],
-                                             _stream_ptr()), "mb_kv_cache_read")
+        _lib.check(_lib.lib.mb_kv_cache_read(_lib.PAGED_KV.pack(*args), ptr, ptr + half, *strides, shape[2], _stream_ptr()),
+                   "mb_kv_cache_read")
     return out
 
 
@@ -227,50 +228,47 @@ def attn_fwd_paged(
     Rows of a sequence may be split over several SMs: the same call repeats bit for bit, but a row's bits may
     differ between calls of other shapes."""
     dims = 3 if cu_seqlens is not None else 4
-    _check_rows(q, "q", cache, dims)
-    hq = q.shape[-2]
+    q_rows = _rows(q, "q", cache, dims)
+    shape = q.shape
+    hq = shape[-2]
     if hq == 0 or hq % cache.heads:
         raise ValueError(f"q has {hq} heads, not a multiple of the cache's {cache.heads}")
     if not 0 < softmax_scale < float("inf"):
         raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
-    a = _lib.AttnPagedArgs()
-    a.kv = cache._args
-    tokens = q.shape[0] if dims == 3 else q.shape[0] * q.shape[1]
-    cache._fill(a.kv, page_table, seq_lens, cu_seqlens, tokens)
-    if dims == 4:
-        if q.shape[0] != a.kv.batch:
-            raise ValueError(f"q has batch {q.shape[0]}, page_table {a.kv.batch}")
-        if max_queries is not None and max_queries < q.shape[1]:
-            raise ValueError(f"max_queries is {max_queries}, q has {q.shape[1]} tokens per sequence")
-        max_queries = q.shape[1]
-    elif max_queries is None:
-        max_queries = tokens
-    covered = page_table.shape[1] * cache.page_size
+    covered = page_table.shape[-1] * cache.page_size
     max_keys = covered if max_keys is None else min(int(max_keys), covered)
+    if dims == 4:
+        n = shape[1]
+        tokens = shape[0] * n
+        if shape[0] != page_table.shape[0]:
+            raise ValueError(f"q has batch {shape[0]}, page_table {page_table.shape[0]}")
+        if max_queries is not None and max_queries < n:
+            raise ValueError(f"max_queries is {max_queries}, q has {n} tokens per sequence")
+        max_queries = n
+        lse_shape = (shape[0], hq, n)
+    else:
+        tokens = shape[0]
+        max_queries = tokens if max_queries is None else min(int(max_queries), tokens)
+        lse_shape = (hq, tokens)
     if max_queries < 0 or max_keys < 0:
         raise ValueError("max_queries and max_keys must not be negative")
+    batch = cache._batch(page_table, seq_lens, cu_seqlens, tokens)
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    else:
-        _check_rows(out, "out", cache, dims)
-        if out.shape != q.shape:
-            raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
-    shape = (hq, tokens) if dims == 3 else (q.shape[0], hq, q.shape[1])
+        out = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+    elif out.shape != shape:
+        raise ValueError(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
     if lse is None:
-        lse = torch.empty(shape, dtype=torch.float32, device=q.device)
-    elif lse.dtype != torch.float32 or tuple(lse.shape) != shape or lse.device != cache.device or \
-            (shape[-1] > 1 and lse.stride(-1) != 1):
-        raise ValueError(f"lse must be fp32 {shape} with contiguous rows on {cache.device}")
-    a.q, a.o, a.lse = q.data_ptr(), out.data_ptr(), lse.data_ptr()
-    a.q_stride_b, a.q_stride_t, a.q_stride_h = _strides(q)
-    a.o_stride_b, a.o_stride_t, a.o_stride_h = _strides(out)
-    a.lse_stride_b, a.lse_stride_h = (0, lse.stride(0)) if dims == 3 else lse.stride()[:2]
-    a.hq, a.max_queries, a.max_keys = hq, min(max_queries, tokens), max_keys
-    a.causal, a.softmax_scale = 1 if causal else 0, float(softmax_scale)
+        lse = torch.empty(lse_shape, dtype=torch.float32, device=cache.device)
+    elif (lse.dtype != torch.float32 or lse.shape != lse_shape or lse.device != cache.device
+          or (lse_shape[-1] > 1 and lse.stride(-1) != 1)):
+        raise ValueError(f"lse must be fp32 {lse_shape} with contiguous rows on {cache.device}")
+    lse_strides = lse.stride()
+    args = _lib.ATTN_PAGED.pack(*batch, *q_rows, *_rows(out, "out", cache, dims), lse.data_ptr(),
+                                lse_strides[0] if dims == 4 else 0, lse_strides[-2], hq, max_queries, max_keys,
+                                1 if causal else 0, softmax_scale)
     with _on(cache.device):
         # scratch of units that several SMs share; freed in stream order by the caching allocator
-        need = _lib.lib.mb_attn_paged_workspace(C.byref(a))
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        _lib.check(_lib.lib.mb_attn_paged(C.byref(a), ws.data_ptr() if need > 0 else None, need, _stream_ptr()),
-                   "mb_attn_paged")
+        need = _lib.lib.mb_attn_paged_workspace(args)
+        ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need > 0 else None
+        _lib.check(_lib.lib.mb_attn_paged(args, ws.data_ptr() if need > 0 else None, need, _stream_ptr()), "mb_attn_paged")
     return out, lse
