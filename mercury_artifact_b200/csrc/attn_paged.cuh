@@ -23,14 +23,16 @@ struct PagedAttnArgs {
   float* part_o;
   float2* part_ml;
   int4* open;
+  int whole;  // few rows: CTA i has unit i, and nothing is joined
   // tiles: keys (in tiles of 128) of a share of a unit; partial results [CTA][32 column groups][256 rows], (maximum, sum)
   // [CTA][256]; tile_open: the split unit whose first share a CTA has (sequence, K/V head, row block, shares; 0: none).
   // All null where no unit is split.
   int share_tiles;
-  // tiles: keys and values of every sequence one after the other in bf16, [batch, packed_rows, hkv, 128] (null: in pages)
+  // tiles: the sequences [b_begin, b_end); where their keys and values lie one after the other in bf16, [b_end - b_begin,
+  // packed_rows, hkv, 128] (null: in pages)
+  int b_begin, b_end;
   const __nv_bfloat16 *packed_k, *packed_v;
   int packed_rows;
-  int head_bytes;  // of a cached key and value of one head
   float4* tile_o;
   float2* tile_ml;
   int4* tile_open;
@@ -40,11 +42,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream);
 long long paged_rows_workspace(int rows, int ctas);
-int paged_rows_ctas();
 int paged_rows_padded(int rows);
-// The first `rows` keys and values of every sequence with at least min_new new tokens, in bf16 [batch, rows, hkv, 128].
-int launch_read_e4m3(const PagedView& c, void* k_out, void* v_out, int rows, int min_new, int max_new, cudaStream_t stream);
-int launch_paged_tiles(const PagedAttnArgs& a, bool fp8, int ctas, cudaStream_t stream);
+int paged_rows_step(bool fp8);  // keys
+// The first a.packed_rows keys and values of the sequences [a.b_begin, a.b_end) with at least min_new new tokens, in bf16.
+int launch_read_e4m3(const PagedAttnArgs& a, int min_new, cudaStream_t stream);
+int launch_paged_tiles(const PagedAttnArgs& a, int ctas, cudaStream_t stream);
 long long paged_tiles_workspace(long long ctas);
 
 }  // namespace mb

@@ -178,29 +178,39 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   }
 
   // this CTA's part of the list
-  const int total = row_total<kStep>(a, sm);
-  const int ctas = row_ctas(total, gridDim.x);
-  if (tid == 0) a.open[blockIdx.x] = make_int4(0, 0, 0, 0);
-  if ((int)blockIdx.x >= ctas || total == 0) return;
-  const int first = row_begin(total, blockIdx.x, ctas), last = row_begin(total, blockIdx.x + 1, ctas);
-  int before = 0;
-  for (int b0 = 0; b0 < a.c.batch; b0 += kRowThreads) {
-    const int b = b0 + tid;
-    const int mine = b < a.c.batch ? unit_steps<kStep>(a, paged_seq(a.c, b, a.max_queries, a.max_keys)) * a.c.hkv : 0;
-    const int incl = row_scan(mine, before, sm->warp_sum, before);
-    if (first >= incl - mine && first < incl) {
-      sm->b = b;
-      sm->step = first - (incl - mine);
-    }
-  }
-  __syncthreads();
-
   RowIter in;  // what is loaded next
-  in.b = sm->b;
-  in.s = paged_seq(a.c, in.b, a.max_queries, a.max_keys);
-  in.steps = unit_steps<kStep>(a, in.s);
-  in.h = sm->step / in.steps;
-  in.step = sm->step - in.h * in.steps;
+  int total, ctas = 1, first = 0, last;
+  if (a.whole) {
+    in.b = blockIdx.x / a.c.hkv;
+    in.h = blockIdx.x - in.b * a.c.hkv;
+    in.step = 0;
+    in.s = paged_seq(a.c, in.b, a.max_queries, a.max_keys);
+    in.steps = total = last = unit_steps<kStep>(a, in.s);
+    if (total == 0) return;
+  } else {
+    total = row_total<kStep>(a, sm);
+    ctas = row_ctas(total, gridDim.x);
+    if (tid == 0) a.open[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if ((int)blockIdx.x >= ctas || total == 0) return;
+    first = row_begin(total, blockIdx.x, ctas);
+    last = row_begin(total, blockIdx.x + 1, ctas);
+    int before = 0;
+    for (int b0 = 0; b0 < a.c.batch; b0 += kRowThreads) {
+      const int b = b0 + tid;
+      const int mine = b < a.c.batch ? unit_steps<kStep>(a, paged_seq(a.c, b, a.max_queries, a.max_keys)) * a.c.hkv : 0;
+      const int incl = row_scan(mine, before, sm->warp_sum, before);
+      if (first >= incl - mine && first < incl) {
+        sm->b = b;
+        sm->step = first - (incl - mine);
+      }
+    }
+    __syncthreads();
+    in.b = sm->b;
+    in.s = paged_seq(a.c, in.b, a.max_queries, a.max_keys);
+    in.steps = unit_steps<kStep>(a, in.s);
+    in.h = sm->step / in.steps;
+    in.step = sm->step - in.h * in.steps;
+  }
   RowIter at = in;  // what is computed next
 
   // the page table's entry for this lane's key of the step to load, fetched one step ahead
@@ -678,7 +688,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_merge_kernel(const __grid_c
   if (lane == 0) a.lse[unit.x * a.lse_sb + hd * a.lse_sh + tok] = sum == 0.f ? -INFINITY : top * kLn2 + __logf(sum);
 }
 
-int paged_rows_ctas() { return sm_count(); }
+int paged_rows_step(bool fp8) { return fp8 ? RowShape<true>::kStep : RowShape<false>::kStep; }
 
 // Rows that the kernel is compiled for
 int paged_rows_padded(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
@@ -702,7 +712,7 @@ static int launch_rows(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   }
   if (!launch_overlapped("launch paged_rows_kernel", paged_rows_kernel<kFp8, kTiles>, dim3(ctas), kRowThreads, bytes, stream, a))
     return MB_E_CUDA;
-  if (!launch_overlapped("launch paged_merge_kernel", paged_merge_kernel<8 * kTiles>,
+  if (!a.whole && !launch_overlapped("launch paged_merge_kernel", paged_merge_kernel<8 * kTiles>,
                          dim3(ctas, min(a.few, a.max_queries * a.group)), kRowThreads, 0, stream, a))
     return MB_E_CUDA;
   return MB_SUCCESS;

@@ -13,15 +13,15 @@
 //            last box that lie behind the end are cleared before the values are used (hidden scores are replaced anyway).
 //   kRows    bf16, other pages: four more warps gather row by row with cp.async, 16 bytes a piece, straight into the
 //            swizzled layout that tcgen05 reads.
-//   kCodes   e4m3: two warps gather codes row by row with cp.async, up to three tiles ahead, and those four turn them into
-//            f16 (see paged_common.cuh) on their way from one place in shared memory to another.  Scores and
-//            probabilities of a tile are then in units of the tile's largest power of two, which goes into the scale of
-//            the scores and into the exponents.
+// Codes (e4m3) are brought into bf16 before, into a buffer where every sequence is one page (launch_read_e4m3).  Turning them
+// on their way into shared memory instead, by four more warps, was built and measured: it took 1.35 ms where the copy
+// (35 us) and these tiles take 0.86 (2 048 tokens, 32 768 keys, 32/8 heads), because the tiles then stall on the
+// conversion's instructions, and no less time with one block of rows per sequence (64 tokens: 88 us, 85).
 //
 //   warps 0-3   softmax + epilogue of query tile 0 (one thread per row)
 //   warps 4-7   softmax + epilogue of query tile 1; warps 0-7 also gather the queries
-//   warp  8     issues Q K^T, owns tensor memory;  warp 10 issues P V;  warps 9 and 11 issue TMA (kBoxes) or gather codes
-//   warps 12-15 gather keys and values (kRows), turn codes into f16 (kCodes)
+//   warp  8     issues Q K^T, owns tensor memory;  warp 10 issues P V;  warps 9 and 11 issue TMA (kBoxes)
+//   warps 12-15 gather keys and values (kRows)
 //
 // A launch has one CTA per (sequence, 256 rows, K/V head, share of the keys), found on the device from the lengths that
 // are there; CTAs beyond the last of them return.  Shares leave their unnormalised rows, maxima and sums in
@@ -31,21 +31,18 @@
 
 namespace mb {
 
-enum TileMode { kBoxes, kRows, kCodes };
+enum TileMode { kBoxes, kRows };
 
 // Threads; registers at launch, of the softmax warps and of the others (an increase beyond what the CTA was launched with
-// would block forever, hence the check).  Stages of 32 KiB in bf16; of codes, 16 KiB.
+// would block forever, hence the check).  
 template <int kMode>
 struct TileShape {
-  static constexpr int kGather = kMode == kBoxes ? 0 : 128;  // threads of warps 12-15
-  static constexpr int kThreads = 384 + kGather;
+  static constexpr int kThreads = kMode == kBoxes ? 384 : 512;
   static constexpr int kLaunch = kMode == kBoxes ? 160 : 128;
   static constexpr int kSoftmax = kMode == kBoxes ? 216 : 208, kOthers = 48;
   static_assert(256 * kSoftmax + (kThreads - 256) * kOthers <= kThreads * kLaunch, "more registers than the CTA is launched with");
-  static constexpr int kStages = kMode == kCodes ? 3 : 4;
-  static constexpr int kCodeStages = kMode == kCodes ? 3 : 0;
-  static constexpr int kCodeStage = kBN * kHeadDim;
 };
+constexpr int kTileStages = 4;  // of 32 KiB: a tile of keys or values
 template <int kRegs>
 __device__ __forceinline__ void give_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
@@ -53,12 +50,6 @@ __device__ __forceinline__ void give_registers() {
 template <int kRegs>
 __device__ __forceinline__ void take_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
-}
-
-// Instruction descriptor of a product of 128 rows: bf16, or f16 (both operands alike), fp32 sums.
-template <int kMode>
-__host__ __device__ constexpr uint32_t tile_idesc(int n, bool b_mn_major) {
-  return umma_idesc_bf16(kBM, n, false, b_mn_major) & ~(kMode == kCodes ? (1u << 7) | (1u << 10) : 0u);
 }
 
 struct TileMaps {
@@ -69,27 +60,20 @@ struct TileMaps {
 };
 
 struct TileSmem {
-  uint64_t q_full, kv_full[4], kv_empty[4], s_full[2], s_free, p_full[2][2], o_full[2], drain, tail, codes_full[3], codes_empty[3];
+  uint64_t q_full, kv_full[4], kv_empty[4], s_full[2], s_free, p_full[2][2], o_full[2], drain, tail;
   uint32_t tmem_base;
   int abort_word;
   int valid;                // this CTA has an item
   int b, h, block, part, parts;
   PagedSeq seq;
   int first, last[2];       // tiles of 128 keys: [first, last[i]) of query tile i
-  long long off[3][kBN];       // byte offsets of a tile's rows in k and v (-1: zeros)
-  // e4m3: scale bytes of the keys and values of a tile; exponents of their largest; power of two of a row of queries
-  uint32_t scales[4][2][kBN];
-  int warp_top[4][2][2];  // largest scale byte of half of the rows
-  int top[8][2];
-  float q_scale[2 * kBM];
+  alignas(16) long long off[3][kBN];       // byte offsets of a tile's rows in k and v (-1: zeros)
 };
 
-template <int kMode>
 constexpr int tile_smem_bytes() {
-  return (2 + TileShape<kMode>::kStages) * kTileBytes + TileShape<kMode>::kCodeStages * TileShape<kMode>::kCodeStage +
-         1024 /* alignment */ + (int)sizeof(TileSmem);
+  return (2 + kTileStages) * kTileBytes + 1024 /* alignment */ + (int)sizeof(TileSmem);
 }
-static_assert(tile_smem_bytes<kRows>() <= 232448 && tile_smem_bytes<kCodes>() <= 232448, "shared memory budget of one CTA");
+static_assert(tile_smem_bytes() <= 232448, "shared memory budget of one CTA");
 
 __device__ __forceinline__ int tiles_of(int keys) { return (keys + kBN - 1) / kBN; }
 
@@ -111,11 +95,11 @@ __device__ __forceinline__ int key_shares(const PagedAttnArgs& a, const PagedSeq
 __device__ __forceinline__ void find_item(const PagedAttnArgs& a, TileSmem* ctl, int lane) {
   int before = 0, found = 0;
   const int want = blockIdx.x;
-  for (int b0 = 0; b0 < a.c.batch && !found; b0 += 32) {
+  for (int b0 = a.b_begin; b0 < a.b_end && !found; b0 += 32) {
     const int b = b0 + lane;
     PagedSeq s{0, 0, 0};
     int items = 0;
-    if (b < a.c.batch) {
+    if (b < a.b_end) {
       s = paged_seq(a.c, b, a.max_queries, a.max_keys);
       items = row_blocks(a, s) * a.c.hkv * key_shares(a, s);
     }
@@ -132,7 +116,7 @@ __device__ __forceinline__ void find_item(const PagedAttnArgs& a, TileSmem* ctl,
       int i = want - (incl - items);
       ctl->part = i % shares;
       i /= shares;
-      const long long head_bytes = max(1ll, (long long)s.len * a.head_bytes);
+      const long long head_bytes = max(1ll, (long long)s.len * (4 * kHeadDim));
       const int fit = (int)min((long long)a.c.hkv, max(1ll, (48ll << 20) / head_bytes));
       const int hb = (a.c.hkv + (a.c.hkv + fit - 1) / fit - 1) / ((a.c.hkv + fit - 1) / fit);  // equal blocks
       const int group = i / (hb * blocks), rem = i - group * hb * blocks;
@@ -153,13 +137,12 @@ template <int kMode>
 __global__ void __maxnreg__(TileShape<kMode>::kLaunch)
 paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ PagedAttnArgs a) {
   using Shape = TileShape<kMode>;
-  constexpr int kStages = Shape::kStages;
+  constexpr int kStages = kTileStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sKV = smem + 2 * kTileBytes;
-  uint8_t* sCodes = sKV + kStages * kTileBytes;
-  TileSmem* ctl = reinterpret_cast<TileSmem*>(sCodes + Shape::kCodeStages * Shape::kCodeStage);
+  TileSmem* ctl = reinterpret_cast<TileSmem*>(sKV + kStages * kTileBytes);
   volatile int* abort_word = &ctl->abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -189,12 +172,8 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
   } else if (warp == 1 && lane == 0) {
     mbar_init(&ctl->q_full, 256);
     mbar_init(&ctl->tail, 1);
-    for (int s = 0; s < Shape::kCodeStages; ++s) {
-      mbar_init(&ctl->codes_full[s], 128);  // of 64 threads, when their copies are there and when their other stores are
-      mbar_init(&ctl->codes_empty[s], 128);
-    }
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&ctl->kv_full[s], kMode == kBoxes ? 1 : Shape::kGather);
+      mbar_init(&ctl->kv_full[s], kMode == kBoxes ? 1 : 128);
       mbar_init(&ctl->kv_empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -229,18 +208,10 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
     for (int i = 0; i < 16; ++i) {
       const int x = (tid >> 4) + 16 * i, row = row0 + x, tok = row / a.group, hd = row - tok * a.group;
       const bool real = row < rows;
-      const __nv_bfloat16* from = real ? q + tok * a.q_st + hd * a.q_sh + piece * 8 : a.q;
-      uint8_t* to = sQ + (x >> 7) * kTileBytes + (piece >> 3) * kHalfBytes + (x & 127) * 128 + (((piece & 7) ^ (x & 7)) << 4);
-      if constexpr (kMode == kCodes) {
-        uint4 v = real ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
-        const float scale = query_to_f16(v);
-        *reinterpret_cast<uint4*>(to) = v;
-        if (piece == 0) ctl->q_scale[x] = scale;
-      } else {
-        cp_async16(smem_u32(to), from, real);
-      }
+      cp_async16(smem_u32(sQ) + (x >> 7) * kTileBytes + (piece >> 3) * kHalfBytes + (x & 127) * 128 + (((piece & 7) ^ (x & 7)) << 4),
+                 real ? q + tok * a.q_st + hd * a.q_sh + piece * 8 : a.q, real);
     }
-    cp_async_wait<0>();
+    cp_async_wait_all();
     fence_proxy_async_smem();
     mbar_arrive(&ctl->q_full);
   }
@@ -303,126 +274,12 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
           mbar_arrive(&ctl->kv_full[(n - 2) % kStages]);
         }
       }
-      cp_async_wait<0>();
+      cp_async_wait_all();
       fence_proxy_async_smem();
       for (int n = max(positions - 2, 0); n < positions; ++n) mbar_arrive(&ctl->kv_full[n % kStages]);
-    } else if constexpr (kMode == kCodes) {
-      constexpr int kStride = Shape::kGather / 8;
-      const int piece = r & 7, row0 = r >> 3;
-#pragma unroll 1
-      for (int n = 0; n < positions; ++n) {
-        const int stage = n % kStages, round = n / kStages, from = n % Shape::kCodeStages;
-        int which;
-        const int j = tile_of(n, which);
-        if (ok) ok = mbar_wait(&ctl->codes_full[from], (n / Shape::kCodeStages) & 1, abort_word, MB_ERR_TIMEOUT_KV_FULL);
-        const int top = max(max(ctl->warp_top[j & 3][which][0], ctl->warp_top[j & 3][which][1]), kMinScale);
-        if (!which && r == 0) {  // for the softmax warps
-          ctl->top[j & 7][0] = top - 127;
-          ctl->top[j & 7][1] = max(max(ctl->warp_top[j & 3][1][0], ctl->warp_top[j & 3][1][1]), kMinScale) - 127;
-        }
-        if (ok && round > 0) ok = mbar_wait(&ctl->kv_empty[stage], (round - 1) & 1, abort_word, MB_ERR_TIMEOUT_KV_EMPTY);
-        if (ok) {
-          const uint8_t* codes = sCodes + from * Shape::kCodeStage + piece * 16;
-          uint8_t* dst = sKV + stage * kTileBytes + (piece >> 2) * kHalfBytes;
-          // the lanes of a row store even pieces of one half and odd pieces of the other at a time: different banks
-          const int c0 = (2 * piece) & 7, swap = (piece >> 2) & 1;
-          // four rows at a time: all loads before the first store, which the compiler would not pass
-#pragma unroll
-          for (int i = 0; i < kBN / kStride; i += 4) {
-            uint2 x[4], y[4];
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int row = row0 + kStride * (i + e);
-              w[e] = ctl->scales[j & 3][which][row];
-              x[e] = *reinterpret_cast<const uint2*>(codes + row * kHeadDim + swap * 8);
-              y[e] = *reinterpret_cast<const uint2*>(codes + row * kHeadDim + 8 - swap * 8);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int row = row0 + kStride * (i + e);
-              const float f = scale_relative((w[e] >> (8 * (piece >> 1))) & 0xffu, top);
-              const uint32_t mult = pack_f16x2(f, f);
-              uint8_t* at = dst + row * 128;
-              *reinterpret_cast<uint4*>(at + (((c0 + swap) ^ (row & 7)) << 4)) =
-                  make_uint4(mul_f16x2(e4m3_f16(x[e].x), mult), mul_f16x2(e4m3_f16_high(x[e].x), mult),
-                             mul_f16x2(e4m3_f16(x[e].y), mult), mul_f16x2(e4m3_f16_high(x[e].y), mult));
-              *reinterpret_cast<uint4*>(at + (((c0 + 1 - swap) ^ (row & 7)) << 4)) =
-                  make_uint4(mul_f16x2(e4m3_f16(y[e].x), mult), mul_f16x2(e4m3_f16_high(y[e].x), mult),
-                             mul_f16x2(e4m3_f16(y[e].y), mult), mul_f16x2(e4m3_f16_high(y[e].y), mult));
-            }
-          }
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(&ctl->kv_full[stage]);
-        mbar_arrive(&ctl->codes_empty[from]);
-      }
     }
   } else if (warp == 9 || warp == 11) {
     give_registers<Shape::kOthers>();
-    if constexpr (kMode == kCodes) {
-      // ---------------------------------------------------------------- codes: a thread places rows f and f + 64 of a tile
-      // and copies 16 codes of every eighth row
-      const int f = lane + (warp == 11 ? 32 : 0), len = ctl->seq.len, piece = f & 7;
-      bool ok = true;  // (both warps go through the same barriers, also after a wait ran out)
-      auto entry_of = [&](int j, int i) {
-        const int pos = (first + j) * kBN + f + 64 * i;
-        return j < total && pos < len ? paged_entry(a.c, ctl->b, pos) : 0;
-      };
-      long long off[2];     // of the tile to place next
-      uint32_t words[2][2]; // its scale bytes, [key, value][row]
-      int entry[2];         // of the tile behind it
-      auto look_up = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int pos = (first + j) * kBN + f + 64 * i, slot = pos - page_index(a.c, pos) * a.c.page_size;
-          const int page = j < total && pos < len ? paged_id(a.c, entry[i], -1) : -1;
-          off[i] = page >= 0 ? paged_offset(a.c, page, slot, ctl->h) : -1;
-          const long long at = page >= 0 ? scale_offset(a.c, page, slot, ctl->h) : 0;
-          words[0][i] = page >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(a.c.k_scale + at)) : 0;
-          words[1][i] = page >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(a.c.v_scale + at)) : 0;
-          entry[i] = entry_of(j + 1, i);
-        }
-      };
-      entry[0] = entry_of(0, 0);
-      entry[1] = entry_of(0, 1);
-      look_up(0);
-#pragma unroll 1
-      for (int n = 0; n < positions; ++n) {
-        int which;
-        const int j = tile_of(n, which), stage = n % Shape::kCodeStages, round = n / Shape::kCodeStages;
-        if (!which) {  // (three buffers: the values of the tile before are still to be fetched)
-          ctl->off[j % 3][f] = off[0];
-          ctl->off[j % 3][f + 64] = off[1];
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            ctl->scales[j & 3][kv][f] = words[kv][0];
-            ctl->scales[j & 3][kv][f + 64] = words[kv][1];
-            const int top = __reduce_max_sync(0xffffffffu, max(scale_top(words[kv][0]), scale_top(words[kv][1])));
-            if (lane == 0) ctl->warp_top[j & 3][kv][warp == 11] = top;
-          }
-          asm volatile("bar.sync 2, 64;" ::: "memory");
-          look_up(j + 1);
-        }
-        if (ok && round > 0) ok = mbar_wait(&ctl->codes_empty[stage], (round - 1) & 1, abort_word, MB_ERR_TIMEOUT_KV_EMPTY);
-        if (ok) {
-          const uint8_t* base = (which ? a.c.v : a.c.k) + piece * 16;
-          const uint32_t to = smem_u32(sCodes) + stage * Shape::kCodeStage + piece * 16;
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            long long from[4];  // (read before the first copy is issued: the compiler keeps their order)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) from[e] = ctl->off[j % 3][(f >> 3) + 8 * (i + e)];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              cp_async16(to + ((f >> 3) + 8 * (i + e)) * kHeadDim, from[e] >= 0 ? base + from[e] : a.c.k, from[e] >= 0);
-          }
-        }
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl->codes_full[stage])) : "memory");
-        mbar_arrive(&ctl->codes_full[stage]);
-      }
-      cp_async_wait<0>();
-    }
     if constexpr (kMode == kBoxes) {
       // ---------------------------------------------------------------- TMA: a lane has a box of a tile, a warp half of
       // its columns (lanes issue one after the other, some 55 cycles each: small pages are bound by it)
@@ -432,7 +289,7 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
       auto page_of = [&](int j) {
         const int pos = (first + j) * kBN + lane * maps.box;
         if (j >= total || lane >= boxes || pos >= len) return -1;
-        return maps.packed ? ctl->b : paged_entry(a.c, ctl->b, pos);
+        return maps.packed ? ctl->b - a.b_begin : paged_entry(a.c, ctl->b, pos);
       };
       if (lane == 0) tma_prefetch_desc(half ? &maps.v : &maps.k);
       int page = page_of(0), page1 = page, page2 = page, n = 0;  // of the next keys, the last ones and those before
@@ -485,7 +342,7 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
       constexpr uint32_t kStageUnits = kTileBytes / 16;
       bool ok = true;
       if (warp == 8) {
-        constexpr uint32_t idesc_qk = tile_idesc<kMode>(kBN, false);
+        constexpr uint32_t idesc_qk = umma_idesc_bf16(kBM, kBN, false, false);
         const uint64_t q_desc = umma_smem_desc(smem_u32(sQ), 16, 1024);
         const uint64_t k_desc0 = umma_smem_desc(smem_u32(sKV), 16, 1024);
         int use = 0;
@@ -511,7 +368,7 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
           umma_commit_elect(&ctl->kv_empty[stage]);
         }
       } else {
-        constexpr uint32_t idesc_pv = tile_idesc<kMode>(kD, true);
+        constexpr uint32_t idesc_pv = umma_idesc_bf16(kBM, kD, false, true);
         const uint64_t v_desc0 = umma_smem_desc(smem_u32(sKV), kHalfBytes, 1024);
         int cnt[2] = {0, 0};
         for (int g = 0; g < total && ok; ++g) {
@@ -561,7 +418,6 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
     const int visible = visible_keys(a, ctl->seq, tile_row + row), visible_first = visible_keys(a, ctl->seq, tile_row);
     const int last = i ? n1 : n0;
 
-    // A row's reference m_ref is the exponent of its largest term exp2(score) * 2^value_exp (bf16: value_exp = 0)
     float m_ref = -INFINITY, l = 0.f;
     int cnt = 0;
     bool ok = true;
@@ -595,14 +451,8 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
         mx2 = max3(mx2, __uint_as_float(sr[2][e]), __uint_as_float(sr[2][e + 1]));
         mx3 = max3(mx3, __uint_as_float(sr[3][e]), __uint_as_float(sr[3][e + 1]));
       }
-      float c = a.scale_log2, value_exp = 0.f;
-      if constexpr (kMode == kCodes) {
-        const int* top = ctl->top[(jt - first) & 7];
-        c = fmaxf(c * exp2_int(top[0]) * ctl->q_scale[i * kBM + row], 1.2e-38f);  // (not zero: hidden scores are infinite)
-        value_exp = (float)top[1];
-      }
       float m_tile = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
-      m_tile = m_tile == -INFINITY ? -INFINITY : fmaf(m_tile, c, value_exp);
+      m_tile *= a.scale_log2;
       if (cnt == 0) {
         m_ref = m_tile;
       } else {
@@ -630,8 +480,8 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
           }
         }
       }
-      const float lift = value_exp - ((m_ref == -INFINITY) ? 0.f : m_ref);
-      const uint64_t c2 = pack2(c, c);
+      const float lift = m_ref == -INFINITY ? 0.f : -m_ref;
+      const uint64_t c2 = pack2(a.scale_log2, a.scale_log2);
       const uint64_t nm2 = pack2(lift, lift);
       uint64_t sum_a = pack2(0.f, 0.f), sum_b = pack2(0.f, 0.f);
 #pragma unroll
@@ -650,7 +500,7 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
             else sum_a = add2(sum_a, p2);
             float p0, p1;
             unpack2(p2, p0, p1);
-            pk[cc * 16 + (e >> 1)] = kMode == kCodes ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
+            pk[cc * 16 + (e >> 1)] = pack_bf16x2(p0, p1);
           }
         }
         tmem_st32(tPi + half * 32, pk);
@@ -660,7 +510,7 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
       }
       float s0, s1;
       unpack2(add2(sum_a, sum_b), s0, s1);
-      l = kMode == kCodes ? fmaf(s0 + s1, fast_exp2(-value_exp), l) : l + (s0 + s1);
+      l += s0 + s1;
       ++cnt;
     }
 
@@ -781,7 +631,7 @@ static int launch_tiles(const TileMaps& maps, const PagedAttnArgs& a, int ctas, 
   static bool attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MB_E_CUDA;
-  constexpr int bytes = tile_smem_bytes<kMode>();
+  constexpr int bytes = tile_smem_bytes();
   if (!attr_set[dev]) {
     if (!cuda_ok(cudaFuncSetAttribute(paged_tiles_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
                  "paged_tiles_kernel shared memory"))
@@ -807,29 +657,29 @@ static bool page_map(CUtensorMap* map, const void* ptr, int hkv, int slots, int 
   return encode_tiled_bf16(map, const_cast<void*>(ptr), 4, dims, strides, boxes, ones) == 0;
 }
 
-int launch_paged_tiles(const PagedAttnArgs& a, bool fp8, int ctas, cudaStream_t stream) {
+int launch_paged_tiles(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   TileMaps maps;
   memset(&maps, 0, sizeof(maps));
   const PagedView& c = a.c;
   if (a.packed_k != nullptr) {
     const long long row = (long long)c.hkv * kHeadDim * 2;
     maps.box = kBN;
-    maps.pages = c.batch;
+    maps.pages = a.b_end - a.b_begin;
     maps.packed = 1;
-    if (!page_map(&maps.k, a.packed_k, c.hkv, a.packed_rows, c.batch, kHeadDim * 2, row, row * a.packed_rows, kBN) ||
-        !page_map(&maps.v, a.packed_v, c.hkv, a.packed_rows, c.batch, kHeadDim * 2, row, row * a.packed_rows, kBN))
+    if (!page_map(&maps.k, a.packed_k, c.hkv, a.packed_rows, maps.pages, kHeadDim * 2, row, row * a.packed_rows, kBN) ||
+        !page_map(&maps.v, a.packed_v, c.hkv, a.packed_rows, maps.pages, kHeadDim * 2, row, row * a.packed_rows, kBN))
       return MB_E_TENSORMAP;
     return launch_tiles<kBoxes>(maps, a, ctas, stream);
   }
-  if (fp8) return launch_tiles<kCodes>(maps, a, ctas, stream);
   maps.box = 1;
   maps.pages = c.pages;
   while (maps.box < kBN && c.page_size % (2 * maps.box) == 0) maps.box *= 2;
-  // (strides that no tensor map takes, as of a dimension of one entry, go row by row as well)
-  if (maps.box >= 8 && c.pages > 0 && page_map(&maps.k, c.k, c.hkv, c.page_size, c.pages, c.head_sb, c.slot_sb, c.page_sb, maps.box) &&
-      page_map(&maps.v, c.v, c.hkv, c.page_size, c.pages, c.head_sb, c.slot_sb, c.page_sb, maps.box))
-    return launch_tiles<kBoxes>(maps, a, ctas, stream);
-  return launch_tiles<kRows>(maps, a, ctas, stream);
+  // (rows of the swizzled layout go in groups of 8; without a page there is nothing to map, and nothing to fetch)
+  if (maps.box < 8 || c.pages == 0) return launch_tiles<kRows>(maps, a, ctas, stream);
+  if (!page_map(&maps.k, c.k, c.hkv, c.page_size, c.pages, c.head_sb, c.slot_sb, c.page_sb, maps.box) ||
+      !page_map(&maps.v, c.v, c.hkv, c.page_size, c.pages, c.head_sb, c.slot_sb, c.page_sb, maps.box))
+    return MB_E_TENSORMAP;
+  return launch_tiles<kBoxes>(maps, a, ctas, stream);
 }
 
 }  // namespace mb

@@ -9,7 +9,7 @@
 // Why powers of two: a code has 4 significant bits, so code * 2^e is exact in bf16.  What is read back, and what the
 // attention kernels multiply, is the stored value itself with no second rounding; a factor of amax / 448 would use
 // the top of the range a little better (at most one binade), but e4m3's step is relative, so that nothing is gained.
-#include "paged_common.cuh"
+#include "attn_paged.cuh"
 
 namespace mb {
 
@@ -38,6 +38,10 @@ int paged_view(const mb_paged_kv* x, PagedView* c) {
   c->page_sb = x->stride_page * size;
   c->slot_sb = x->stride_slot * size;
   c->head_sb = x->stride_h * size;
+  // the stride of a dimension of one entry is never used; tensor maps want one that makes sense
+  if (x->hkv == 1) c->head_sb = kHeadDim * size;
+  if (x->page_size == 1) c->slot_sb = c->head_sb * x->hkv;
+  if (x->pages == 1) c->page_sb = c->slot_sb * x->page_size;
   c->k_scale = x->k_scale;
   c->v_scale = x->v_scale;
   c->table = x->page_table;
@@ -64,7 +68,8 @@ struct CacheMoveArgs {
   uint8_t* v;
   long long sb, st, sh;  // bytes
   int rows;              // read: rows per sequence
-  int min_new, max_new;  // read: sequences with at least min_new new tokens only
+  int first_seq;         // read: sequences from this one on, the first one's rows at k, v
+  int min_new, max_new;  // read: those with at least min_new new tokens only
 };
 
 constexpr int kMoveThreads = 256;
@@ -206,7 +211,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_cache_read_kernel(const __gri
   using S = MoveShape<kFp8>;
   __shared__ long long place[kReadTokens], place_scale[kFp8 ? kReadTokens : 1];
   const PagedView& c = a.c;
-  const int b = blockIdx.y, p0 = blockIdx.x * kReadTokens;
+  const int b = a.first_seq + blockIdx.y, p0 = blockIdx.x * kReadTokens;
   grid_dependents_launch();
   grid_dependency_wait();
   const PagedSeq seq = paged_seq(c, b, a.max_new, c.max_pages * c.page_size);
@@ -231,7 +236,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_cache_read_kernel(const __gri
     const int which = rem >= c.hkv, h = rem - which * c.hkv;
     if (place[t] < 0) continue;
     const uint4 x = __ldg(reinterpret_cast<const uint4*>((which ? c.v : c.k) + place[t] + h * c.head_sb) + lane);
-    uint4* dst = reinterpret_cast<uint4*>((which ? a.v : a.k) + b * a.sb + (p0 + t) * a.st + h * a.sh) + lane * (kFp8 ? 2 : 1);
+    uint4* dst = reinterpret_cast<uint4*>((which ? a.v : a.k) + blockIdx.y * a.sb + (p0 + t) * a.st + h * a.sh) + lane * (kFp8 ? 2 : 1);
     if constexpr (kFp8) {
       const uint32_t byte = __ldg((which ? c.v_scale : c.k_scale) + place_scale[t] + (long long)h * c.page_size * kScalesPerRow + lane / 2);
       // code * 2^-120 from the bits, then two exact factors: 2^120 and the block's own
@@ -267,7 +272,7 @@ int launch_kv_cache_write(const mb_paged_kv* kv, const void* k_new, const void* 
   a.k = static_cast<uint8_t*>(const_cast<void*>(k_new));
   a.v = static_cast<uint8_t*>(const_cast<void*>(v_new));
   a.sb = sb * 2; a.st = st * 2; a.sh = sh * 2;
-  a.rows = a.min_new = a.max_new = 0;
+  a.rows = a.first_seq = a.min_new = a.max_new = 0;
   const long long rows = (long long)a.c.tokens * 2 * a.c.hkv;
   const bool fp8 = kv->dtype == MB_DTYPE_E4M3;
   const int groups = fp8 ? MoveShape<true>::kGroups : MoveShape<false>::kGroups;
@@ -280,24 +285,25 @@ int launch_kv_cache_write(const mb_paged_kv* kv, const void* k_new, const void* 
                                                                                                                : MB_E_CUDA;
 }
 
-static int launch_read(const CacheMoveArgs& a, bool fp8, cudaStream_t stream) {
-  const dim3 grid((a.rows + kReadTokens - 1) / kReadTokens, a.c.batch);
+static int launch_read(const CacheMoveArgs& a, bool fp8, int sequences, cudaStream_t stream) {
+  const dim3 grid((a.rows + kReadTokens - 1) / kReadTokens, sequences);
   const auto kernel = fp8 ? kv_cache_read_kernel<true> : kv_cache_read_kernel<false>;
   return launch_overlapped("launch kv_cache_read_kernel", kernel, grid, kMoveThreads, 0, stream, a) ? MB_SUCCESS : MB_E_CUDA;
 }
 
-int launch_read_e4m3(const PagedView& c, void* k_out, void* v_out, int rows, int min_new, int max_new, cudaStream_t stream) {
+int launch_read_e4m3(const PagedAttnArgs& x, int min_new, cudaStream_t stream) {
   CacheMoveArgs a;
-  a.c = c;
-  a.k = static_cast<uint8_t*>(k_out);
-  a.v = static_cast<uint8_t*>(v_out);
+  a.c = x.c;
+  a.k = reinterpret_cast<uint8_t*>(const_cast<__nv_bfloat16*>(x.packed_k));
+  a.v = reinterpret_cast<uint8_t*>(const_cast<__nv_bfloat16*>(x.packed_v));
   a.sh = kHeadDim * 2;
-  a.st = a.sh * c.hkv;
-  a.sb = a.st * rows;
-  a.rows = rows;
+  a.st = a.sh * x.c.hkv;
+  a.sb = a.st * x.packed_rows;
+  a.rows = x.packed_rows;
+  a.first_seq = x.b_begin;
   a.min_new = min_new;
-  a.max_new = max_new;
-  return launch_read(a, true, stream);
+  a.max_new = x.max_queries;
+  return launch_read(a, true, x.b_end - x.b_begin, stream);
 }
 
 int launch_kv_cache_read(const mb_paged_kv* kv, void* k_out, void* v_out, long long sb, long long ss, long long sh,
@@ -313,10 +319,9 @@ int launch_kv_cache_read(const mb_paged_kv* kv, void* k_out, void* v_out, long l
   a.v = static_cast<uint8_t*>(v_out);
   a.sb = sb * 2; a.st = ss * 2; a.sh = sh * 2;
   a.rows = rows;
-  a.min_new = 0;
-  a.max_new = 0;
+  a.first_seq = a.min_new = a.max_new = 0;
   a.c.cu = nullptr;
-  return launch_read(a, kv->dtype == MB_DTYPE_E4M3, stream);
+  return launch_read(a, kv->dtype == MB_DTYPE_E4M3, a.c.batch, stream);
 }
 
 }  // namespace mb

@@ -254,11 +254,11 @@ def attn_fwd_paged(
         raise ValueError("max_queries and max_keys must not be negative")
     batch = cache._batch(page_table, seq_lens, cu_seqlens, tokens)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+        out = torch.empty_like(q)
     elif out.shape != shape:
         raise ValueError(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
     if lse is None:
-        lse = torch.empty(lse_shape, dtype=torch.float32, device=cache.device)
+        lse = q.new_empty(lse_shape, dtype=torch.float32)
     elif (lse.dtype != torch.float32 or lse.shape != lse_shape or lse.device != cache.device
           or (lse_shape[-1] > 1 and lse.stride(-1) != 1)):
         raise ValueError(f"lse must be fp32 {lse_shape} with contiguous rows on {cache.device}")
@@ -269,6 +269,6 @@ def attn_fwd_paged(
     with _on(cache.device):
         # scratch of units that several SMs share; freed in stream order by the caching allocator
         need = _lib.lib.mb_attn_paged_workspace(args)
-        ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need > 0 else None
+        ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
         _lib.check(_lib.lib.mb_attn_paged(args, ws.data_ptr() if need > 0 else None, need, _stream_ptr()), "mb_attn_paged")
     return out, lse
