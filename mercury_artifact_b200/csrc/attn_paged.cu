@@ -40,10 +40,12 @@ static int plan_paged(const mb_attn_paged_args* x, PagedPlan* p) {
   memset(p, 0, sizeof(*p));
   const bool padded = kv.cu_seqlens == nullptr, e4m3 = kv.dtype == MB_DTYPE_E4M3;
   // Beside chunks the sequences with few rows are single tokens as a rule, which the kernels for fewer rows take faster.
-  p->few = e4m3 && rows <= kFewRowsE4m3 ? kFewRowsE4m3 : kFewRows;
+  p->few = rows > kFewRows && heads <= 8 ? 8 : kFewRows;
+  if (e4m3 && rows <= kFewRowsE4m3) p->few = kFewRowsE4m3;
   if (rows <= p->few || !padded) {
     p->rows = (int)min(rows, (long long)p->few);
-    const long long units = (long long)kv.batch * kv.hkv;
+    const int block = paged_rows_padded(p->rows);
+    const long long units = (long long)kv.batch * kv.hkv * ((p->few + block - 1) / block);
     const int step = paged_rows_step(e4m3);
     // Few short units are not split over SMs: the launch that joins the parts would take longer than the steps it saves.
     p->whole = units <= sms && x->max_keys <= kWholeSteps * step;

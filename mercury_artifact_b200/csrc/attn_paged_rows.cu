@@ -40,14 +40,15 @@ constexpr int kPitch = 132;  // of the merge buffers' rows, in floats: what the 
 struct RowSmem {
   int total, warp_sum[kRowWarps];
   int b, step;                               // where this CTA's part starts: sequence, and step inside it
-  float2 ml[kRowWarps][32];
-  float q_scale[32];  // e4m3: power of two that a row of queries was divided by
+  float2 ml[kRowWarps][16];                  // of a unit: every warp's maximum and sum,
+  float part_l[kRowWarps][16], row_top[16];  // its sum relative to the rows' maxima, these
+  float q_scale[16];  // e4m3: power of two that a row of queries was divided by
 };
 
 template <bool kFp8>
 constexpr int row_smem_bytes() {
-  // merge buffers: 32 rows, of as many warps as fit
-  return kRowWarps * kRowStages * RowShape<kFp8>::kStage + 32 * 2 * kHeadDim + 32 * kPitch * 4 + (int)sizeof(RowSmem);
+  // queries of 16 rows; merge buffers: 32 rows, of as many warps as fit
+  return kRowWarps * kRowStages * RowShape<kFp8>::kStage + 16 * 2 * kHeadDim + 32 * kPitch * 4 + (int)sizeof(RowSmem);
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -76,9 +77,10 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A place in the list of steps.
+// A place in the list of steps.  A sequence's units: K/V heads, and blocks of kRows rows of each.
 struct RowIter {
-  int b, h, step, steps;  // steps: of the unit
+  int b, h, block, blocks;  // block of rows, how many the sequence has
+  int step, steps;          // of the unit
   PagedSeq s;
 };
 
@@ -86,43 +88,36 @@ template <int kStep>
 __device__ __forceinline__ int unit_steps(const PagedAttnArgs& a, const PagedSeq& s) {
   return s.n > 0 && s.n * a.group <= a.few ? (s.len + kStep - 1) / kStep : 0;
 }
-template <int kStep>
-__device__ __forceinline__ void next_sequence(const PagedAttnArgs& a, RowIter& it) {
-  it.steps = 0;
-  while (it.b < a.c.batch) {
-    it.s = paged_seq(a.c, it.b, a.max_queries, a.max_keys);
-    it.steps = unit_steps<kStep>(a, it.s);
-    if (it.steps > 0) return;
-    ++it.b;
-  }
+template <int kRows>
+__device__ __forceinline__ int rows_blocks(const PagedAttnArgs& a, const PagedSeq& s) {
+  return (s.n * a.group + kRows - 1) / kRows;
 }
-template <int kStep>
-__device__ __forceinline__ void next_step(const PagedAttnArgs& a, RowIter& it) {
-  if (++it.step < it.steps) return;
+template <int kStep, int kRows>
+__device__ __forceinline__ int sequence_steps(const PagedAttnArgs& a, const PagedSeq& s) {
+  const int steps = unit_steps<kStep>(a, s);
+  return steps == 0 ? 0 : steps * rows_blocks<kRows>(a, s) * a.c.hkv;
+}
+template <int kStep, int kRows>
+__device__ __forceinline__ void next_unit(const PagedAttnArgs& a, RowIter& it) {
   it.step = 0;
+  if (++it.block < it.blocks) return;
+  it.block = 0;
   if (++it.h < a.c.hkv) return;
   it.h = 0;
-  ++it.b;
-  next_sequence<kStep>(a, it);
+  it.steps = 0;
+  while (++it.b < a.c.batch) {
+    it.s = paged_seq(a.c, it.b, a.max_queries, a.max_keys);
+    it.steps = unit_steps<kStep>(a, it.s);
+    it.blocks = rows_blocks<kRows>(a, it.s);
+    if (it.steps > 0) return;
+  }
+}
+template <int kStep, int kRows>
+__device__ __forceinline__ void next_step(const PagedAttnArgs& a, RowIter& it) {
+  if (++it.step >= it.steps) next_unit<kStep, kRows>(a, it);
 }
 
-// Steps of all sequences, and where step `first` lies (all threads take part; two barriers per 256 sequences).
-template <int kStep>
-__device__ __forceinline__ int row_total(const PagedAttnArgs& a, RowSmem* sm) {
-  int mine = 0;
-  for (int b = threadIdx.x; b < a.c.batch; b += kRowThreads)
-    mine += unit_steps<kStep>(a, paged_seq(a.c, b, a.max_queries, a.max_keys)) * a.c.hkv;
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-  if ((threadIdx.x & 31) == 0) sm->warp_sum[threadIdx.x >> 5] = mine;
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < kRowWarps; ++w) total += sm->warp_sum[w];
-  __syncthreads();
-  return total;
-}
-// Inclusive scan over the block of one value per thread, plus `before`.
+// Inclusive scan over the block of one value per thread, plus `before`; `all`: the last one's.
 __device__ __forceinline__ int row_scan(int mine, int before, int* warp_sum, int& all) {
   int incl = mine;
 #pragma unroll
@@ -134,7 +129,8 @@ __device__ __forceinline__ int row_scan(int mine, int before, int* warp_sum, int
   __syncthreads();
   int add = before;
   all = before;
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
+#pragma unroll
+  for (int w = 0; w < kRowWarps; ++w) {
     if (w < (int)(threadIdx.x >> 5)) add += warp_sum[w];
     all += warp_sum[w];
   }
@@ -150,12 +146,12 @@ __device__ __forceinline__ int row_begin(int total, int i, int n) { return (int)
 template <bool kFp8, int kTiles>
 __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
   using S = RowShape<kFp8>;
-  constexpr int kStep = S::kStep, kKeys = S::kKeys, kGroups = kKeys / 16;
+  constexpr int kStep = S::kStep, kKeys = S::kKeys, kGroups = kKeys / 16, kRows = 8 * kTiles;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* stages = smem_raw + warp * (kRowStages * S::kStage);
   uint8_t* queries = smem_raw + kRowWarps * kRowStages * S::kStage;  // rows of 256 bytes, pieces swapped like the keys'
-  float* merge = reinterpret_cast<float*>(queries + 32 * 2 * kHeadDim);
+  float* merge = reinterpret_cast<float*>(queries + 16 * 2 * kHeadDim);
   RowSmem* sm = reinterpret_cast<RowSmem*>(merge + 32 * kPitch);
   // e4m3: a step's powers of two in f16, twice [32 keys][4 blocks] for the keys, [4 blocks][32 keys] for the values; where
   // the states are merged at a unit's end
@@ -166,8 +162,56 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   grid_dependents_launch();
   grid_dependency_wait();
 
-  // sequences without keys: their rows see nothing
-  for (int b = blockIdx.x; b < a.c.batch; b += gridDim.x) {
+  // This CTA's part of the list.  A thread looks at every 256th sequence; up to 256 of them are looked at once.
+  RowIter in;  // what is loaded next
+  int total = 0, ctas = 1, first = 0, last;
+  bool empty = false;  // there is a sequence without keys
+  if (a.whole) {
+    const int most = (a.few + kRows - 1) / kRows;  // blocks of a sequence, at most
+    int i = blockIdx.x;
+    in.b = i / (a.c.hkv * most);
+    i -= in.b * a.c.hkv * most;
+    in.h = i / most;
+    in.block = i - in.h * most;
+    in.step = 0;
+    in.s = paged_seq(a.c, in.b, a.max_queries, a.max_keys);
+    in.blocks = rows_blocks<kRows>(a, in.s);
+    in.steps = unit_steps<kStep>(a, in.s);
+    last = total = in.block < in.blocks ? in.steps : 0;
+    empty = in.steps == 0 && in.h == 0 && in.block == 0;
+  } else {
+    int mine = 0, incl = 0;
+    for (int b0 = 0; b0 < a.c.batch; b0 += kRowThreads) {
+      const int b = b0 + tid;
+      mine = 0;
+      if (b < a.c.batch) {
+        const PagedSeq s = paged_seq(a.c, b, a.max_queries, a.max_keys);
+        mine = sequence_steps<kStep, kRows>(a, s);
+        empty |= s.len == 0;
+      }
+      incl = row_scan(mine, total, sm->warp_sum, total);
+    }
+    ctas = row_ctas(total, gridDim.x);
+    if (tid == 0) a.open[blockIdx.x] = make_int4(0, 0, 0, 0);
+    first = row_begin(total, blockIdx.x, ctas);
+    last = row_begin(total, blockIdx.x + 1, ctas);
+    int before = 0;
+    for (int b0 = 0; b0 < a.c.batch; b0 += kRowThreads) {
+      const int b = b0 + tid;
+      if (a.c.batch > kRowThreads) {
+        mine = b < a.c.batch ? sequence_steps<kStep, kRows>(a, paged_seq(a.c, b, a.max_queries, a.max_keys)) : 0;
+        incl = row_scan(mine, before, sm->warp_sum, before);
+      }
+      if (first >= incl - mine && first < incl) {
+        sm->b = b;
+        sm->step = first - (incl - mine);
+      }
+    }
+    empty = __syncthreads_or(empty);
+    if ((int)blockIdx.x >= ctas) total = 0;
+  }
+  // rows of sequences without keys see nothing
+  for (int b = a.whole ? in.b : blockIdx.x; empty && b < a.c.batch; b += a.whole ? a.c.batch : gridDim.x) {
     const PagedSeq seq = paged_seq(a.c, b, a.max_queries, a.max_keys);
     if (seq.len > 0 || seq.n * a.group > a.few) continue;
     for (int i = warp; i < seq.n * a.hq; i += kRowWarps) {
@@ -176,40 +220,16 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       if (lane == 0) a.lse[b * a.lse_sb + hd * a.lse_sh + tok] = -INFINITY;
     }
   }
-
-  // this CTA's part of the list
-  RowIter in;  // what is loaded next
-  int total, ctas = 1, first = 0, last;
-  if (a.whole) {
-    in.b = blockIdx.x / a.c.hkv;
-    in.h = blockIdx.x - in.b * a.c.hkv;
-    in.step = 0;
-    in.s = paged_seq(a.c, in.b, a.max_queries, a.max_keys);
-    in.steps = total = last = unit_steps<kStep>(a, in.s);
-    if (total == 0) return;
-  } else {
-    total = row_total<kStep>(a, sm);
-    ctas = row_ctas(total, gridDim.x);
-    if (tid == 0) a.open[blockIdx.x] = make_int4(0, 0, 0, 0);
-    if ((int)blockIdx.x >= ctas || total == 0) return;
-    first = row_begin(total, blockIdx.x, ctas);
-    last = row_begin(total, blockIdx.x + 1, ctas);
-    int before = 0;
-    for (int b0 = 0; b0 < a.c.batch; b0 += kRowThreads) {
-      const int b = b0 + tid;
-      const int mine = b < a.c.batch ? unit_steps<kStep>(a, paged_seq(a.c, b, a.max_queries, a.max_keys)) * a.c.hkv : 0;
-      const int incl = row_scan(mine, before, sm->warp_sum, before);
-      if (first >= incl - mine && first < incl) {
-        sm->b = b;
-        sm->step = first - (incl - mine);
-      }
-    }
-    __syncthreads();
+  if (total == 0) return;
+  if (!a.whole) {
     in.b = sm->b;
     in.s = paged_seq(a.c, in.b, a.max_queries, a.max_keys);
     in.steps = unit_steps<kStep>(a, in.s);
-    in.h = sm->step / in.steps;
-    in.step = sm->step - in.h * in.steps;
+    in.blocks = rows_blocks<kRows>(a, in.s);
+    const int unit = sm->step / in.steps;
+    in.step = sm->step - unit * in.steps;
+    in.h = unit / in.blocks;
+    in.block = unit - in.h * in.blocks;
   }
   RowIter at = in;  // what is computed next
 
@@ -252,7 +272,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     if (to_load > 0) {
       load(i);
       if (--to_load > 0) {
-        next_step<kStep>(a, in);
+        next_step<kStep, kRows>(a, in);
         entry = entry_of(in);
       }
     }
@@ -263,19 +283,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   RowIter nx = at;  // the unit behind this one
   constexpr int kPasses = (kTiles + 1) / 2;  // sixteen threads have a row, 16 rows at a time
   uint4 qx[kPasses];
-  auto next_unit = [&]() {
-    nx.step = 0;
-    if (++nx.h < a.c.hkv) return;
-    nx.h = 0;
-    ++nx.b;
-    next_sequence<kStep>(a, nx);
-  };
   auto fetch_q = [&]() {
 #pragma unroll
     for (int m = 0; m < kPasses; ++m) {
-      const int r = m * 16 + (tid >> 4), tok = r / a.group, hd = r - tok * a.group;
+      const int r = m * 16 + (tid >> 4), row = nx.block * kRows + r, tok = row / a.group, hd = row - tok * a.group;
       qx[m] = make_uint4(0, 0, 0, 0);
-      if (nx.b < a.c.batch && r < nx.s.n * a.group)
+      if (nx.b < a.c.batch && r < kRows && row < nx.s.n * a.group)
         qx[m] = __ldg(reinterpret_cast<const uint4*>(a.q + nx.b * a.q_sb + (long long)(nx.s.start + tok) * a.q_st +
                                                      (long long)(nx.h * a.group + hd) * a.q_sh) + (tid & 15));
     }
@@ -302,7 +315,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   // Queries of 8 rows as the second operand, for 32 elements along head_dim (two products)
   const uint32_t q_addr = smem_u32(queries) + (lane & 7) * 2 * kHeadDim + (((lane >> 3) ^ (lane & 7)) << 4);
   auto queries_of = [&](uint32_t (&qf)[4], int m, int k2) { ldsm4(qf, (q_addr ^ (k2 << 6)) + m * 8 * 2 * kHeadDim); };
-  constexpr bool kKeepQ = kTiles <= 2;  // in registers for the unit
 
   fetch_q();
   int stage = 0;
@@ -312,14 +324,15 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     const int unit_end = min(last, s + at.steps - at.step);
     const bool done = unit_end == s + at.steps - at.step;
     store_q();
-    next_unit();
+    next_unit<kStep, kRows>(a, nx);
     fetch_q();
     __syncthreads();  // the queries are there, and the buffers of the unit before are free again
     float acc[kTiles][8][4], m_ref[kTiles][2], l[kTiles][2];
     int limit[kTiles][2];        // keys that the row sees; the first of the unit's rows sees the fewest
     float row_scale[kTiles][2];  // e4m3: power of two of the row's queries
-    uint32_t qk[kKeepQ ? kTiles : 1][4][4];
-    const int seen_by_all = a.causal ? at.s.len - at.s.n + 1 : at.s.len;
+    uint32_t qk[kTiles][4][4];
+    const int row0 = at.block * kRows, rows = min(at.s.n * a.group - row0, kRows);
+    const int seen_by_all = a.causal ? at.s.len - at.s.n + row0 / a.group + 1 : at.s.len;
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
 #pragma unroll
@@ -331,10 +344,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         const int r = m * 8 + 2 * t + e;
         m_ref[m][e] = -INFINITY;
         l[m][e] = 0.f;
-        limit[m][e] = a.causal ? min(at.s.len, at.s.len - at.s.n + r / a.group + 1) : at.s.len;
+        limit[m][e] = a.causal ? min(at.s.len, at.s.len - at.s.n + (row0 + r) / a.group + 1) : at.s.len;
         row_scale[m][e] = kFp8 ? sm->q_scale[r] : 1.f;
       }
-      if constexpr (kKeepQ)
 #pragma unroll
         for (int k2 = 0; k2 < 4; ++k2) queries_of(qk[m][k2], m, k2);
     }
@@ -345,7 +357,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       if (to_load > 0) {
         load(stage == 0 ? kRowStages - 1 : stage - 1);
         if (--to_load > 0) {
-          next_step<kStep>(a, in);
+          next_step<kStep, kRows>(a, in);
           entry = entry_of(in);
         }
       }
@@ -375,9 +387,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
           ldsm4(k1, k_addr ^ (k2 << 6) ^ 32);
 #pragma unroll
           for (int m = 0; m < kTiles; ++m) {
-            uint32_t qf[4];
-            if constexpr (!kKeepQ) queries_of(qf, m, k2);
-            const uint32_t(&q)[4] = kKeepQ ? qk[kKeepQ ? m : 0][k2] : qf;
+            const uint32_t(&q)[4] = qk[m][k2];
             mma16816<kFp8>(sc[m][0], k0, q[0], q[1]);
             mma16816<kFp8>(sc[m][0], k1, q[2], q[3]);
           }
@@ -421,9 +431,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
           }
 #pragma unroll
           for (int m = 0; m < kTiles; ++m) {
-            uint32_t qf[4];
-            if constexpr (!kKeepQ) queries_of(qf, m, k2);
-            const uint32_t(&q)[4] = kKeepQ ? qk[kKeepQ ? m : 0][k2] : qf;
+            const uint32_t(&q)[4] = qk[m][k2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               mma16816<kFp8>(sc[m][j], kf[0][j], q[0], q[1]);
@@ -541,8 +549,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
 
     }
 
-    // ---- the warps' states become one
-    const int rows = at.s.n * a.group;
+    // ---- the warps' states become one: through as many buffers as fit, in turns where these are fewer than warps
 #pragma unroll
     for (int m = 0; m < kTiles; ++m)
 #pragma unroll
@@ -558,22 +565,26 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     for (int m = 0; m < kTiles; ++m)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        const int r = m * 8 + 2 * t + e;
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm->ml[w][m * 8 + 2 * t + e].x);
+        for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm->ml[w][r].x);
         f[m][e] = m_ref[m][e] == -INFINITY ? 0.f : fast_exp2(m_ref[m][e] - top);
         // a warp without a visible key has nothing, whatever its masked products gave
-        const float mine = sm->ml[warp][m * 8 + 2 * t + e].y;
+        const float mine = sm->ml[warp][r].y;
         if (m_ref[m][e] == -INFINITY && mine == mine) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) acc[m][j][e] = acc[m][j][2 + e] = 0.f;
         }
+        // (from here on: the row's maximum, and the warp's sum relative to it)
+        if (g == 0) sm->part_l[warp][r] = m_ref[m][e] == -INFINITY ? mine : mine * f[m][e];
+        if (g == 0 && warp == 0) sm->row_top[r] = top;
       }
-    constexpr int kBuffers = 4 / kTiles;
+    const int buffers = rows <= 4 ? 8 : 4 / kTiles, pitch = rows <= 4 ? 4 * kPitch : kRows * kPitch;
 #pragma unroll 1
-    for (int round = 0; round < kRowWarps / kBuffers; ++round) {
-      if (warp / kBuffers == round) {
-        float* buf = merge + (warp % kBuffers) * 8 * kTiles * kPitch;
+    for (int round = 0; round < kRowWarps; round += buffers) {
+      if (warp >= round && warp < round + buffers) {
+        float* buf = merge + (warp - round) * pitch;
 #pragma unroll
         for (int m = 0; m < kTiles; ++m)
 #pragma unroll
@@ -600,30 +611,25 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     const bool whole = from_start && done;
     const int slot = 2 * blockIdx.x + (from_start ? 1 : 0);
     for (int r = warp; r < rows; r += kRowWarps) {
-      float top = -INFINITY, sum = 0.f;
+      float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm->ml[w][r].x);
-#pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) {
-        const float2 x = sm->ml[w][r];
-        sum += x.x == -INFINITY ? x.y : x.y * fast_exp2(x.x - top);
-      }
+      for (int w = 0; w < kRowWarps; ++w) sum += sm->part_l[w][r];
+      const float top = sm->row_top[r];
       float4 x = *reinterpret_cast<const float4*>(merge + r * kPitch + lane * 4);
-#pragma unroll
-      for (int i = 1; i < kBuffers; ++i) {
-        const float4 y = *reinterpret_cast<const float4*>(merge + (i * 8 * kTiles + r) * kPitch + lane * 4);
+      for (int i = 1; i < buffers; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(merge + i * pitch + r * kPitch + lane * 4);
         x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
       }
       if (whole) {
-        const int tok = r / a.group, hd = at.h * a.group + r - tok * a.group;
+        const int tok = (row0 + r) / a.group, hd = at.h * a.group + row0 + r - tok * a.group;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const uint2 w = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
         *reinterpret_cast<uint2*>(a.o + at.b * a.o_sb + (long long)(at.s.start + tok) * a.o_st + (long long)hd * a.o_sh + lane * 4) = w;
         if (lane == 0)
           a.lse[at.b * a.lse_sb + hd * a.lse_sh + at.s.start + tok] = sum == 0.f ? -INFINITY : top * kLn2 + __logf(sum);
       } else {
-        *reinterpret_cast<float4*>(a.part_o + ((long long)slot * (8 * kTiles) + r) * kHeadDim + lane * 4) = x;
-        if (lane == 0) a.part_ml[slot * (8 * kTiles) + r] = make_float2(top, sum);
+        *reinterpret_cast<float4*>(a.part_o + ((long long)slot * kRows + r) * kHeadDim + lane * 4) = x;
+        if (lane == 0) a.part_ml[slot * kRows + r] = make_float2(top, sum);
       }
     }
     if (from_start && !done && tid == 0) {
@@ -631,67 +637,75 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       const int end = s + at.steps - at.step;  // behind its last step
       int n = 1;
       while (row_begin(total, blockIdx.x + n, ctas) < end) ++n;
-      a.open[blockIdx.x] = make_int4(at.b, at.h, n, 0);
+      a.open[blockIdx.x] = make_int4(at.b, at.h, n, at.block);
     }
     at = nx;
   }
 }
 
-// Joins the partial states of the unit that CTA blockIdx.x of the launch before began and did not finish (if there is one):
-// row blockIdx.y.  A warp takes every eighth of the parts, four columns a lane; the warps' sums are added in order.
+// Joins the partial states of the unit that CTA blockIdx.x of the launch before began and did not finish (if there is one).
+// Of few parts a warp joins a row; of many, all warps join row after row, each an eighth of the parts.  A lane has four columns.
+// The parts are added in order.
 template <int kRows>
 __global__ void __launch_bounds__(kRowThreads) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
   __shared__ float4 part[kRowWarps][32];
   __shared__ float part_l[kRowWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependents_launch();
   grid_dependency_wait();
   const int4 unit = a.open[blockIdx.x];
   if (unit.z == 0) return;
   const PagedSeq seq = paged_seq(a.c, unit.x, a.max_queries, a.max_keys);
-  if (r >= seq.n * a.group) return;
-  const int n = unit.z;
-  // slot of the unit's p-th CTA: it ends the list of the first one and starts those of the others
-  auto slot = [&](int p) { return (long long)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * kRows + r; };
-  float top = -INFINITY;
-  for (int p = lane; p < n; p += 32) top = fmaxf(top, a.part_ml[slot(p)].x);
+  const int n = unit.z, row0 = unit.w * kRows, rows = min(seq.n * a.group - row0, kRows);
+  const bool many = n > 16;
+  for (int r = many ? 0 : warp; r < rows; r += many ? 1 : kRowWarps) {
+    // slot of the unit's p-th CTA: it ends the list of the first one and starts those of the others
+    auto slot = [&](int p) { return (long long)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * kRows + r; };
+    float top = -INFINITY;
+    for (int p = lane; p < n; p += 32) top = fmaxf(top, a.part_ml[slot(p)].x);
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  float sum = 0.f;
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    float sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int p = warp; p < n; p += kRowWarps) {
-    const float2 ml = a.part_ml[slot(p)];
-    const float4 y = *reinterpret_cast<const float4*>(a.part_o + slot(p) * kHeadDim + lane * 4);
-    // (a part without visible keys holds zeros, or what is not a number)
-    const float w = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top);
-    sum = fmaf(w, ml.y, sum);
-    x.x = fmaf(w, y.x, x.x);
-    x.y = fmaf(w, y.y, x.y);
-    x.z = fmaf(w, y.z, x.z);
-    x.w = fmaf(w, y.w, x.w);
-  }
-  part[warp][lane] = x;
-  if (lane == 0) part_l[warp] = sum;
-  __syncthreads();
-  if (warp != 0) return;
+    for (int p = many ? warp : 0; p < n; p += many ? kRowWarps : 1) {
+      const float2 ml = a.part_ml[slot(p)];
+      const float4 y = *reinterpret_cast<const float4*>(a.part_o + slot(p) * kHeadDim + lane * 4);
+      // (a part without visible keys holds zeros, or what is not a number)
+      const float w = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top);
+      sum = fmaf(w, ml.y, sum);
+      x.x = fmaf(w, y.x, x.x);
+      x.y = fmaf(w, y.y, x.y);
+      x.z = fmaf(w, y.z, x.z);
+      x.w = fmaf(w, y.w, x.w);
+    }
+    if (many) {
+      part[warp][lane] = x;
+      if (lane == 0) part_l[warp] = sum;
+      __syncthreads();
+      if (warp == 0) {
 #pragma unroll
-  for (int w = 1; w < kRowWarps; ++w) {
-    const float4 y = part[w][lane];
-    sum += part_l[w];
-    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+        for (int w = 1; w < kRowWarps; ++w) {
+          const float4 y = part[w][lane];
+          sum += part_l[w];
+          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+        }
+      }
+      __syncthreads();
+      if (warp != 0) continue;
+    }
+    const int tok = (row0 + r) / a.group, hd = unit.y * a.group + row0 + r - tok * a.group;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const uint2 w = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+    *reinterpret_cast<uint2*>(a.o + unit.x * a.o_sb + (long long)(seq.start + tok) * a.o_st + (long long)hd * a.o_sh + lane * 4) = w;
+    if (lane == 0) a.lse[unit.x * a.lse_sb + hd * a.lse_sh + seq.start + tok] = sum == 0.f ? -INFINITY : top * kLn2 + __logf(sum);
   }
-  const int tok = seq.start + r / a.group, hd = unit.y * a.group + r % a.group;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const uint2 w = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
-  *reinterpret_cast<uint2*>(a.o + unit.x * a.o_sb + (long long)tok * a.o_st + (long long)hd * a.o_sh + lane * 4) = w;
-  if (lane == 0) a.lse[unit.x * a.lse_sb + hd * a.lse_sh + tok] = sum == 0.f ? -INFINITY : top * kLn2 + __logf(sum);
 }
 
 int paged_rows_step(bool fp8) { return fp8 ? RowShape<true>::kStep : RowShape<false>::kStep; }
 
-// Rows that the kernel is compiled for
-int paged_rows_padded(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+// Rows of a block, for which the kernel is compiled
+int paged_rows_padded(int rows) { return rows <= 8 ? 8 : 16; }
 
 long long paged_rows_workspace(int rows, int ctas) {
   return 2ll * ctas * paged_rows_padded(rows) * (kHeadDim * (long long)sizeof(float) + (long long)sizeof(float2)) + ctas * (long long)sizeof(int4);
@@ -713,17 +727,14 @@ static int launch_rows(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   if (!launch_overlapped("launch paged_rows_kernel", paged_rows_kernel<kFp8, kTiles>, dim3(ctas), kRowThreads, bytes, stream, a))
     return MB_E_CUDA;
   if (!a.whole && !launch_overlapped("launch paged_merge_kernel", paged_merge_kernel<8 * kTiles>,
-                         dim3(ctas, min(a.few, a.max_queries * a.group)), kRowThreads, 0, stream, a))
+                         dim3(ctas), kRowThreads, 0, stream, a))
     return MB_E_CUDA;
   return MB_SUCCESS;
 }
 
 int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream) {
-  switch (paged_rows_padded(rows)) {
-    case 8: return fp8 ? launch_rows<true, 1>(a, ctas, stream) : launch_rows<false, 1>(a, ctas, stream);
-    case 16: return fp8 ? launch_rows<true, 2>(a, ctas, stream) : launch_rows<false, 2>(a, ctas, stream);
-    default: return fp8 ? launch_rows<true, 4>(a, ctas, stream) : launch_rows<false, 4>(a, ctas, stream);
-  }
+  if (paged_rows_padded(rows) == 8) return fp8 ? launch_rows<true, 1>(a, ctas, stream) : launch_rows<false, 1>(a, ctas, stream);
+  return fp8 ? launch_rows<true, 2>(a, ctas, stream) : launch_rows<false, 2>(a, ctas, stream);
 }
 
 }  // namespace mb
