@@ -163,26 +163,29 @@ __global__ void __launch_bounds__(kMoveThreads) kv_cache_write_kernel(const __gr
   __syncthreads();
 
   const int group = threadIdx.x / S::kLanes, lane = threadIdx.x % S::kLanes;
+  // a group's i-th row and the end, counted from the first row of token t0 (divisions in 32 bits)
+  const int row_in = (int)(row0 - (long long)t0 * per_token) + group;
+  const int rows = (int)min(total - (long long)t0 * per_token, (long long)(kRows + per_token));
   uint4 x[kIters][kFp8 ? 2 : 1];
   uint8_t* dst[kIters];
   uint8_t* dst_scale[kIters];
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
-    const long long r = row0 + i * S::kGroups + group;
+    const int r = row_in + i * S::kGroups;
     dst[i] = nullptr;
     dst_scale[i] = nullptr;
 #pragma unroll
     for (int j = 0; j < (kFp8 ? 2 : 1); ++j) x[i][j] = make_uint4(0, 0, 0, 0);
-    if (r < total) {
-      const int t = (int)(r / per_token), rem = (int)(r - (long long)t * per_token);
+    if (r < rows) {
+      const int in = r / per_token, rem = r - in * per_token;
       const int which = rem >= c.hkv, h = rem - which * c.hkv;
-      if (place[t - t0] >= 0) {
-        const uint4* src = reinterpret_cast<const uint4*>((which ? a.v : a.k) + source[t - t0] + h * a.sh);
+      if (place[in] >= 0) {
+        const uint4* src = reinterpret_cast<const uint4*>((which ? a.v : a.k) + source[in] + h * a.sh);
 #pragma unroll
-        for (int j = 0; j < (kFp8 ? 2 : 1); ++j) x[i][j] = __ldg(src + lane * (kFp8 ? 2 : 1) + j);
-        dst[i] = (which ? c.v : c.k) + place[t - t0] + h * c.head_sb + lane * 16;
+        for (int j = 0; j < (kFp8 ? 2 : 1); ++j) x[i][j] = __ldcs(src + lane * (kFp8 ? 2 : 1) + j);
+        dst[i] = (which ? c.v : c.k) + place[in] + h * c.head_sb + lane * 16;
         if constexpr (kFp8)
-          dst_scale[i] = (which ? c.v_scale : c.k_scale) + place_scale[t - t0] + (long long)h * c.page_size * kScalesPerRow;
+          dst_scale[i] = (which ? c.v_scale : c.k_scale) + place_scale[in] + (long long)h * c.page_size * kScalesPerRow;
       }
     }
   }
@@ -195,11 +198,11 @@ __global__ void __launch_bounds__(kMoveThreads) kv_cache_write_kernel(const __gr
       byte |= __shfl_down_sync(0xffffffffu, byte, 2, 8) << 8;
       byte |= __shfl_down_sync(0xffffffffu, byte, 4, 8) << 16;
       if (dst[i] != nullptr) {
-        *reinterpret_cast<uint4*>(dst[i]) = q;
+        __stcs(reinterpret_cast<uint4*>(dst[i]), q);
         if (lane == 0) *reinterpret_cast<uint32_t*>(dst_scale[i]) = byte;
       }
     } else {
-      if (dst[i] != nullptr) *reinterpret_cast<uint4*>(dst[i]) = x[i][0];
+      if (dst[i] != nullptr) __stcs(reinterpret_cast<uint4*>(dst[i]), x[i][0]);
     }
   }
 }
