@@ -220,3 +220,364 @@ def test_chunks_split_over_keys(fp8, lens, new, heads):
     assert _status() == 0
     assert torch.equal(o, o2) and torch.equal(lse, lse2)
     check(batch, o, lse, batch.expected(tensors, True))
+
+
+# -- what calls may find -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("new", [[1, 3, 2], [40, 1, 90]])
+def test_rows_behind_the_last_sequence_and_given_buffers(fp8, new):
+    """q, out and lse are views of wider buffers with rows behind the last sequence; these stay as they were."""
+    batch = Batch([200, 31, 300], new, (8, 2), 16, fp8, seed=11)
+    tensors = batch.cache_tensors()
+    t = batch.tokens
+    wide = torch.full((t + 7, 10, D + 8), 3.0, dtype=torch.bfloat16, device="cuda")
+    wide[:t, 1:9, :D] = batch.q.cuda()
+    out = torch.full((t + 7, 9, D), 5.0, dtype=torch.bfloat16, device="cuda")
+    lse = torch.full((8, t + 20), 6.0, device="cuda")
+    o, l = _mb().attn_fwd_paged(wide[:, 1:9, :D], _cache(batch, tensors), batch.on(batch.table), batch.on(batch.seq_lens), SCALE,
+                                cu_seqlens=batch.on(batch.cu), max_queries=max(new), out=out[:, :8], lse=lse[:, 3:3 + t + 7])
+    assert _status() == 0
+    check(batch, o[:t], l[:, :t], batch.expected(tensors, True))
+    assert (out[t:] == 5).all() and (out[:, 8] == 5).all()
+    assert (lse[:, :3] == 6).all() and (lse[:, 3 + t:] == 6).all()
+
+
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("new", [1, 60])
+def test_cache_layouts(fp8, new):
+    """Heads before slots, and keys and values as the halves of one packed tensor with pages between them unused."""
+    batch = Batch([333, 70], [new, new], (8, 4), 16, fp8, ragged=False, seed=12)
+    k, v, ks, vs = batch.cache_tensors()
+    want = batch.expected((k, v, ks, vs), True)
+    bits = torch.uint8 if fp8 else torch.int16
+    shape = (2, batch.pages * 2, 4, 16, D)  # every other page, heads first
+    packed = torch.zeros(shape, dtype=bits, device="cuda")
+    packed[0, ::2], packed[1, ::2] = (x.view(bits).transpose(1, 2).cuda() for x in (k, v))
+    packed = packed.view(k.dtype)[:, ::2].transpose(2, 3)
+    cache = _mb().PagedKV(packed[0], packed[1], batch.on(ks), batch.on(vs))
+    o, lse = _attend(batch, cache)
+    assert _status() == 0
+    check(batch, o, lse, want)
+    back = _mb().kv_cache_read(cache, batch.on(batch.table), batch.on(batch.seq_lens), max_keys=333)
+    for c, (x, s) in enumerate(((k, ks), (v, vs))):
+        assert torch.equal(back[c, 0].double().cpu(), oracle.gather(x, s, batch.table[0], 333, 16))
+
+
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("sequences", [300, 1100])
+def test_many_sequences(fp8, sequences):
+    """More sequences than threads of a block, some of them empty, some without new tokens."""
+    lens = [(7 * i) % 61 for i in range(sequences)]
+    new = [min(n, (i % 4)) for i, n in enumerate(lens)]
+    new[5], lens[5] = 30, 40  # one chunk for the tiles
+    batch = Batch(lens, new, (4, 1), 16, fp8, seed=13)
+    tensors = batch.cache_tensors()
+    cache = _cache(batch, tensors)
+    o, lse = _attend(batch, cache)
+    assert _status() == 0
+    check(batch, o, lse, batch.expected(tensors, True))
+    k, v = (torch.cat([batch.kv[i][c][lens[i] - n:] for i, n in enumerate(new)]) for c in range(2))
+    cache.k.view(torch.uint8).zero_()
+    _mb().kv_cache_write(cache, batch.on(k), batch.on(v), batch.on(batch.table), batch.on(batch.seq_lens), batch.on(batch.cu))
+    assert _status() == 0
+    for i in (0, 5, 63, 255, 256, 257, sequences - 1):
+        for j in range(lens[i] - new[i], lens[i]):
+            page, slot = batch.table[i, j // 16].item(), j % 16
+            assert torch.equal(cache.k[page, slot].cpu().view(torch.uint8), tensors[0][page, slot].view(torch.uint8))
+
+
+def test_offsets_beyond_32_bits():
+    """Pages whose addresses lie more than 2^32 bytes (and 2^31 elements) behind the cache's."""
+    pages, page, heads = 300000, 16, 8
+    need = 2 * pages * page * heads * D * 2
+    if torch.cuda.mem_get_info()[0] < need + (8 << 30):
+        pytest.skip("needs 20 GB of device memory")
+    cache = _mb().PagedKV.empty(pages, page, heads)
+    g = torch.Generator().manual_seed(0)
+    for new in (1, 40):
+        k, v, q = ((torch.randn(2, 100, heads, D, generator=g)).to(torch.bfloat16) for _ in range(3))
+        q = q[:, :new]
+        table = torch.tensor([[pages - 1 - i for i in range(7)], [pages // 2 + 131 * i for i in range(7)]], dtype=torch.int32, device="cuda")
+        lens = torch.tensor([100, 100], dtype=torch.int32, device="cuda")
+        _mb().kv_cache_write(cache, k.cuda(), v.cuda(), table, lens)
+        o, lse = _mb().attn_fwd_paged(q.cuda(), cache, table, lens, SCALE)
+        back = _mb().kv_cache_read(cache, table, lens, max_keys=100)
+        assert _status() == 0
+        assert torch.equal(back[0].cpu(), k) and torch.equal(back[1].cpu(), v)
+        from tests.paged_cases import bounds
+
+        for b in range(2):
+            want, l, mass, size = oracle.attend(q[b], k[b].double(), v[b].double(), SCALE, True)
+            tol, tol_l = bounds(want, mass, size)
+            assert ((o[b].double().cpu() - want).abs() <= tol).all()
+            assert ((lse[b].double().cpu() - l).abs() <= tol_l).all()
+
+
+def test_empty_calls():
+    mb = _mb()
+    cache = mb.PagedKV.empty(4, 16, 2)
+    table = torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(3, dtype=torch.int32, device="cuda")
+
+    def rows(*shape):
+        return torch.zeros(*shape, D, dtype=torch.bfloat16, device="cuda")
+
+    o, lse = mb.attn_fwd_paged(rows(3, 0, 4), cache, table, lens, SCALE)
+    assert o.shape == (3, 0, 4, D) and lse.shape == (3, 4, 0)
+    o, lse = mb.attn_fwd_paged(rows(0, 2, 4), cache, table[:0], lens[:0], SCALE)
+    assert o.shape == (0, 2, 4, D)
+    for n in (1, 40):  # nothing cached, by length, by bound, and by a table without columns
+        for kw in ({}, {"max_keys": 0}):
+            o, lse = mb.attn_fwd_paged(rows(3, n, 4) + 1, cache, table, lens, SCALE, **kw)
+            assert (o == 0).all() and (lse == float("-inf")).all()
+        o, lse = mb.attn_fwd_paged(rows(3, n, 4) + 1, cache, table[:, :0], lens, SCALE)
+        assert (o == 0).all() and (lse == float("-inf")).all()
+    mb.kv_cache_write(cache, rows(3, 0, 2), rows(3, 0, 2), table, lens)
+    mb.kv_cache_write(cache, rows(3, 2, 2), rows(3, 2, 2), table, lens)  # more new tokens than keys: none is stored
+    assert mb.kv_cache_read(cache, table, lens, max_keys=0).shape == (2, 3, 0, 2, D)
+    assert (mb.kv_cache_read(cache, table, lens) == 0).all()
+    none = mb.PagedKV.empty(0, 16, 2)
+    o, lse = mb.attn_fwd_paged(rows(3, 40, 4), none, table, lens, SCALE)
+    assert (lse == float("-inf")).all()
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("new", [1, 5, 50])
+def test_bad_pages_lengths_and_offsets_are_reported(fp8, new):
+    """What lies outside is skipped and reported; the other sequences and the next call are as they should be."""
+    from mercury_artifact_b200._lib import MercuryB200Error
+
+    mb = _mb()
+    batch = Batch([100, 120, 90], [new] * 3, (8, 2), 16, fp8, seed=14)
+    tensors = batch.cache_tensors()
+    cache = _cache(batch, tensors)
+    want = batch.expected(tensors, True)
+    q, cu = batch.on(batch.q), batch.on(batch.cu)
+    table, lens = batch.on(batch.table), batch.on(batch.seq_lens)
+    new_rows = torch.zeros(batch.tokens, 2, D, dtype=torch.bfloat16, device="cuda")
+
+    def damaged(t, at, value):
+        t = t.clone()
+        t[at] = value
+        return t
+
+    cases = [(damaged(table, (1, 3), batch.pages), lens, cu), (damaged(table, (1, 0), -1), lens, cu),
+             (table, damaged(lens, 1, -5), cu), (table, damaged(lens, 1, 2 ** 30), cu),
+             (table, lens, damaged(cu, 3, batch.tokens + 100)), (table, lens, damaged(cu, 1, -2 ** 31))]
+    for tb, ln, c in cases:
+        o, lse = mb.attn_fwd_paged(q, cache, tb, ln, SCALE, cu_seqlens=c, max_queries=new)
+        with pytest.raises(MercuryB200Error, match="page number"):
+            cache.check()
+        if c is cu:  # the sequences beside the damaged one
+            for i in (0, 2):
+                rows = slice(int(batch.cu[i]), int(batch.cu[i + 1]))
+                err = (o[rows].double().cpu() - want[0][rows]).abs().max().item()
+                assert err < 0.05
+        if new == 1:
+            mb.kv_cache_read(cache, tb, ln, max_keys=128)
+            if c is cu:
+                with pytest.raises(MercuryB200Error):
+                    cache.check()
+    # a write does not leave the pages
+    before = cache.k.view(torch.uint8).clone()
+    mb.kv_cache_write(cache, new_rows, new_rows, torch.full_like(table, batch.pages), lens, cu)
+    with pytest.raises(MercuryB200Error):
+        cache.check()
+    assert torch.equal(before, cache.k.view(torch.uint8))
+    o, lse = mb.attn_fwd_paged(q, cache, table, lens, SCALE, cu_seqlens=cu, max_queries=new)
+    cache.check()
+    check(batch, o, lse, want)
+
+
+@pytest.mark.parametrize("fp8", FP8)
+def test_captured_graph_replays_with_other_lengths(fp8):
+    """Write, attend and attend with a chunk, captured once; the lengths, pages and rows change between replays."""
+    mb = _mb()
+    a = Batch([100, 0, 517], [1, 1, 1], (8, 2), 16, fp8, ragged=False, seed=15)
+    b = Batch([17, 600, 33], [1, 1, 1], (8, 2), 16, fp8, ragged=False, seed=16)
+    pages = max(a.pages, b.pages)
+    cache = mb.PagedKV.empty(pages, 16, 2, torch.float8_e4m3fn if fp8 else torch.bfloat16)
+    table = torch.zeros(3, 40, dtype=torch.int32, device="cuda")
+    lens = torch.ones(3, dtype=torch.int32, device="cuda")
+    q = torch.zeros(3, 1, 8, D, dtype=torch.bfloat16, device="cuda")
+    kv = torch.zeros(2, 3, 1, 2, D, dtype=torch.bfloat16, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # warm up
+        mb.kv_cache_write(cache, kv[0], kv[1], table, lens)
+        mb.attn_fwd_paged(q, cache, table, lens, SCALE)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mb.kv_cache_write(cache, kv[0], kv[1], table, lens)
+        o, lse = mb.attn_fwd_paged(q, cache, table, lens, SCALE)
+        o2, lse2 = mb.attn_fwd_paged(q, cache, table, lens, SCALE, max_keys=640)
+    for batch in (a, b, a):
+        tensors = batch.cache_tensors()
+        for got, x in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), tensors):
+            if x is not None:
+                got[:batch.pages].view(torch.uint8).copy_(x.view(torch.uint8))
+        table[:, :batch.table.shape[1]] = batch.on(batch.table)
+        lens.copy_(batch.seq_lens)
+        q.copy_(batch.shaped(batch.q))
+        for i, n in enumerate(batch.lens):  # the last key arrives with the call
+            if n:
+                kv[:, i, 0] = batch.kv[i][:, n - 1].cuda()
+                cache.k[batch.table[i, (n - 1) // 16].item(), (n - 1) % 16].view(torch.uint8).fill_(0x7f)
+        graph.replay()
+        cache.check()
+        want = batch.expected(tensors, True)
+        check(batch, o, lse, want)
+        check(batch, o2, lse2, want)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams, each with scratch of its own, give what they give alone."""
+    mb = _mb()
+    work = []
+    for seed, fp8, lens, new in ((17, False, [9000], [1]), (18, True, [9000], [1]), (19, False, [5000], [40]), (20, True, [700, 9000], [9, 9])):
+        batch = Batch(lens, new, (4, 1), 16, fp8, ragged=False, seed=seed)
+        cache = _cache(batch, batch.cache_tensors())
+        args = (batch.on(batch.shaped(batch.q)), cache, batch.on(batch.table), batch.on(batch.seq_lens), SCALE)
+        work.append((args, mb.attn_fwd_paged(*args)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    results = [[] for _ in work]
+    for _ in range(20):
+        for (args, _), stream, got in zip(work, streams, results):
+            with torch.cuda.stream(stream):
+                got.append(mb.attn_fwd_paged(*args))
+    torch.cuda.synchronize()
+    for (_, want), got in zip(work, results):
+        for o, lse in got:
+            assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("lens,new,heads,page", [([3000], [100], (8, 2), 64), ([3000] * 4, [100] * 4, (8, 8), 16), ([500] * 3, [300] * 3, (8, 8), 7),
+                                                 ([2000] * 9, [3] * 9, (8, 2), 16)])
+def test_bits_repeat(fp8, lens, new, heads, page):
+    """With caches cold and warm: every value that is used was waited for."""
+    batch = Batch(lens, new, heads, page, fp8, ragged=False, seed=21)
+    cache = _cache(batch, batch.cache_tensors())
+    args = (batch.on(batch.shaped(batch.q)), cache, batch.on(batch.table), batch.on(batch.seq_lens), SCALE)
+    flush = torch.empty(64 << 20, dtype=torch.int32, device="cuda")
+    runs = []
+    for i in range(40):
+        if i % 4 == 0:
+            flush.fill_(i)
+        runs.append(_mb().attn_fwd_paged(*args))
+        if i % 3 == 0:
+            torch.cuda.synchronize()
+    assert _status() == 0
+    for o, lse in runs[1:]:
+        assert torch.equal(o, runs[0][0]) and torch.equal(lse, runs[0][1])
+
+
+# -- values ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new", [1, 6, 40])
+@pytest.mark.parametrize("k_size,v_size", [(1.0, 2.0 ** -40), (1.0, 2.0 ** 60), (2.0 ** -20, 1.0), (2.0 ** 12, 2.0 ** -12)])
+def test_magnitudes_of_a_quantised_cache(new, k_size, v_size):
+    """Keys and values far from one: the powers of two go into the scores' scale and the results, not into f16's range."""
+    batch = Batch([400, 129], [new, new], (8, 2), 16, True, ragged=False, seed=22, spread=0.5 / max(k_size, 1.0))
+    for kv in batch.kv:
+        kv[0] *= k_size
+        kv[1] *= v_size
+    tensors = batch.cache_tensors()
+    o, lse = _attend(batch, _cache(batch, tensors))
+    assert _status() == 0
+    o_, lse_, mass, size = batch.expected(tensors, True)
+    check(batch, o.double() / v_size, lse, (o_ / v_size, lse_, mass / v_size, size))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_blocks_that_are_not_numbers(new):
+    """A key or value block with a NaN makes the rows that see it NaN; sequences that do not hold it stay."""
+    for which in (0, 1):
+        batch = Batch([200, 90], [new, new], (4, 1), 16, True, ragged=False, seed=23)
+        batch.kv[0][which, 100, 0, 40] = float("inf")
+        tensors = batch.cache_tensors()
+        o, lse = _attend(batch, _cache(batch, tensors))
+        assert _status() == 0
+        assert torch.isnan(o[0].float()[..., 32:64]).all()
+        assert torch.isnan(o[0].float()).all() == (which == 0)
+        assert torch.isnan(lse[0]).all() == (which == 0)
+        assert not torch.isnan(o[1].float()).any()
+        second = Batch([90], [new], (4, 1), 16, True, ragged=False)
+        second.lens, second.new, second.tokens = [90], [new], new
+        second.table, second.seq_lens, second.q, second.cu = batch.table[1:], batch.seq_lens[1:], batch.q[new:], batch.cu[:2]
+        check(second, o[1:], lse[1:], second.expected(tensors, True))
+
+
+# -- together ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fp8", FP8)
+def test_serving_run(fp8):
+    """A prompt in chunks, then tokens one by one: each call sees what was written before it; sequences share a prefix."""
+    mb = _mb()
+    g = torch.Generator().manual_seed(31)
+    hq, hkv, page, total = 8, 2, 16, 150
+    cache = mb.PagedKV.empty(40, page, hkv, torch.float8_e4m3fn if fp8 else torch.bfloat16)
+    k, v = ((torch.randn(2, total, hkv, D, generator=g)).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(2, total, hq, D, generator=g).to(torch.bfloat16)
+    for x in (k, v, q):
+        x[1, :64] = x[0, :64]  # the second sequence begins like the first one, in the same four pages
+    table = torch.arange(20, dtype=torch.int32).reshape(2, 10)
+    table[1, :4] = table[0, :4]
+    table = table.cuda()
+    at = [0, 64]  # the shared prefix is written once
+    steps = [(64, 0), (33, 50), (1, 1), (1, 1), (3, 2), (20, 1), (1, 30)]
+    for n0, n1 in steps:
+        new = [n0, n1]
+        at = [at[0] + n0, at[1] + n1]
+        lens = torch.tensor(at, dtype=torch.int32)
+        cu = torch.tensor([0, n0, n0 + n1], dtype=torch.int32, device="cuda")
+        kn, vn, qn = (torch.cat([x[i, at[i] - new[i]:at[i]] for i in range(2)]).cuda() for x in (k, v, q))
+        mb.kv_cache_write(cache, kn, vn, table, lens.cuda(), cu)
+        o, lse = mb.attn_fwd_paged(qn, cache, table, lens.cuda(), SCALE, cu_seqlens=cu, max_queries=max(new))
+        cache.check()
+        row = 0
+        for i in range(2):
+            kk, vv = k[i, :at[i]].double(), v[i, :at[i]].double()
+            if fp8:
+                kk, vv = (oracle.values(*oracle.quantise(x[i, :at[i]])) for x in (k, v))
+            want, l, mass, size = oracle.attend(q[i, at[i] - new[i]:at[i]], kk, vv, SCALE, True)
+            from tests.paged_cases import bounds
+
+            tol, tol_l = bounds(want, mass, size)
+            got = o[row:row + new[i]].double().cpu()
+            assert ((got - want).abs() <= tol).all()
+            assert ((lse[:, row:row + new[i]].double().cpu() - l).abs() <= tol_l).all()
+            row += new[i]
+
+
+def test_cache_and_block_merge_and_ring_reads_back():
+    """A cached prefix and a block of fresh keys, merged like two blocks of a ring, are attention over both; what is read back
+    goes into the fused forward."""
+    from oracle import block
+    from mercury_artifact_b200.ring import RingAttention
+
+    mb = _mb()
+    g = torch.Generator().manual_seed(32)
+    b, prefix, n, hq, hkv = 2, 300, 128, 8, 2
+    k, v = ((torch.randn(b, prefix + n, hkv, D, generator=g) * 0.5).to(torch.bfloat16).cuda() for _ in range(2))
+    q = (torch.randn(b, n, hq, D, generator=g) * 0.5).to(torch.bfloat16).cuda()
+    cache = mb.PagedKV.empty(64, 16, hkv)
+    table = torch.randperm(64, generator=g)[:b * 20].reshape(b, 20).to(torch.int32).cuda()
+    lens = torch.full((b,), prefix, dtype=torch.int32, device="cuda")
+    mb.kv_cache_write(cache, k[:, :prefix], v[:, :prefix], table, lens)
+    o1, l1 = mb.attn_fwd_paged(q, cache, table, lens, SCALE, causal=False)
+    o2, l2, _, _ = mb._flash_attn_forward(q, k[:, prefix:], v[:, prefix:], 0.0, SCALE, True)
+    out, ls = mb.update_out_and_lse(None, None, o1, l1)
+    out, ls = mb.update_out_and_lse(out, ls, o2, l2)
+    ro, rl = block.block_attn_fwd(q.cpu(), k.cpu(), v.cpu(), SCALE, causal=True, q_off=prefix, k_off=0)
+    assert (out.cpu() - ro.float()).abs().max().item() <= 2e-2
+    assert (ls.squeeze(-1).permute(0, 2, 1).cpu() - rl).abs().max().item() <= 1e-3
+    kv = mb.kv_cache_read(cache, table, lens, max_keys=prefix)
+    op = RingAttention((1,), b, prefix, hq, hkv, D, causal=True)
+    qq = torch.randn(b, prefix, hq, D, generator=g).to(torch.bfloat16).cuda()
+    o3, l3 = op.forward(qq, kv)
+    o4, l4 = mb.attn_fwd_paged(qq, cache, table, lens, SCALE)
+    assert (o3.float() - o4.float()).abs().max().item() <= 2e-2 and (l3 - l4).abs().max().item() <= 1e-3
+    assert _status() == 0
