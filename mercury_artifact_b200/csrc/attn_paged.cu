@@ -79,13 +79,13 @@ static int plan_paged(const mb_attn_paged_args* x, PagedPlan* p) {
     if (ctas > 0x7fffff00ll) return MB_E_TOO_LARGE;
     p->tile_ctas = (int)ctas;
     p->split = best > 1;
-    if (p->split) p->split_bytes = paged_tiles_workspace(p->tile_ctas);
+    if (p->split) p->split_bytes = align_up(paged_tiles_workspace(p->tile_ctas));
   }
   return MB_SUCCESS;
 }
 
-// The two kernels run one after the other and use the workspace in turn.
-static long long workspace_of(const PagedPlan& p) { return max(p.rows_bytes, p.packed_bytes + p.split_bytes); }
+// The two kernels run side by side: [bf16 copy | shares of the tiles | parts of the rows]
+static long long workspace_of(const PagedPlan& p) { return p.packed_bytes + p.split_bytes + p.rows_bytes; }
 
 long long attn_paged_workspace(const mb_attn_paged_args* x) {
   PagedPlan p;
@@ -134,41 +134,53 @@ int launch_attn_paged(const mb_attn_paged_args* x, void* ws, unsigned long long 
   a.few = p.few;
   a.share_tiles = max(p.share_tiles, 1);
 
-  if (p.tile_ctas > 0) {
-    uint8_t* at = static_cast<uint8_t*>(ws);
-    if (e4m3) {  // [keys | values]
-      a.packed_rows = x->max_keys;
-      a.packed_k = reinterpret_cast<const __nv_bfloat16*>(at);
-      a.packed_v = a.packed_k + (long long)p.group * x->max_keys * a.c.hkv * kHeadDim;
-      at += p.packed_bytes;
+  uint8_t* at = static_cast<uint8_t*>(ws);
+  if (p.tile_ctas > 0 && e4m3) {  // [keys | values]
+    a.packed_rows = x->max_keys;
+    a.packed_k = reinterpret_cast<const __nv_bfloat16*>(at);
+    a.packed_v = a.packed_k + (long long)p.group * x->max_keys * a.c.hkv * kHeadDim;
+    at += p.packed_bytes;
+  }
+  if (p.split) {  // [rows | (maximum, sum) | split units]
+    a.tile_o = reinterpret_cast<float4*>(at);
+    a.tile_ml = reinterpret_cast<float2*>(a.tile_o + (long long)p.tile_ctas * (256 * kHeadDim / 4));
+    a.tile_open = reinterpret_cast<int4*>(a.tile_ml + (long long)p.tile_ctas * 256);
+    at += p.split_bytes;
+  }
+  a.whole = p.whole;
+  if (p.row_ctas > 0 && !p.whole) {  // [partial rows | (maximum, sum) | open units]
+    const long long slots = 2ll * p.row_ctas * paged_rows_padded(p.rows);
+    a.part_o = reinterpret_cast<float*>(at);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * kHeadDim);
+    a.open = reinterpret_cast<int4*>(a.part_ml + slots);
+  }
+
+  // Beside chunks, which are bound by the tensor cores and leave SMs idle at their end, single tokens cost little: 16
+  // sequences, 5 of them chunks, up to 8 192 e4m3 keys, 32/8 heads: 176 us one after the other, TODO side by side.
+  for (int b = 0; p.tile_ctas > 0 && b < a.c.batch; b += p.group) {
+    a.b_begin = b;
+    a.b_end = min(b + p.group, a.c.batch);
+    if (e4m3) {
+      rc = launch_read_e4m3(a, p.few / a.group + 1, stream);
+      if (rc != MB_SUCCESS) return rc;
     }
-    if (p.split) {  // [rows | (maximum, sum) | split units]
-      a.tile_o = reinterpret_cast<float4*>(at);
-      a.tile_ml = reinterpret_cast<float2*>(a.tile_o + (long long)p.tile_ctas * (256 * kHeadDim / 4));
-      a.tile_open = reinterpret_cast<int4*>(a.tile_ml + (long long)p.tile_ctas * 256);
+    rc = launch_paged_tiles(a, p.tile_ctas, stream);
+    if (rc != MB_SUCCESS) return rc;
+    if (a.b_end == a.c.batch && p.row_ctas > 0) {
+      a.beside = 1;
+      rc = launch_paged_rows(a, e4m3, p.rows, p.row_ctas, stream);
+      if (rc != MB_SUCCESS) return rc;
     }
-    for (int b = 0; b < a.c.batch; b += p.group) {
-      a.b_begin = b;
-      a.b_end = min(b + p.group, a.c.batch);
-      if (e4m3) {
-        rc = launch_read_e4m3(a, p.few / a.group + 1, stream);
-        if (rc != MB_SUCCESS) return rc;
-      }
-      rc = launch_paged_tiles(a, p.tile_ctas, stream);
+    if (p.split) {
+      rc = launch_paged_tiles_merge(a, p.tile_ctas, stream);
       if (rc != MB_SUCCESS) return rc;
     }
   }
-  if (p.row_ctas > 0) {
-    a.whole = p.whole;
-    if (!p.whole) {  // [partial rows | (maximum, sum) | open units]
-      const long long slots = 2ll * p.row_ctas * paged_rows_padded(p.rows);
-      a.part_o = static_cast<float*>(ws);
-      a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * kHeadDim);
-      a.open = reinterpret_cast<int4*>(a.part_ml + slots);
-    }
+  if (p.row_ctas > 0 && !a.beside) {
     rc = launch_paged_rows(a, e4m3, p.rows, p.row_ctas, stream);
+    if (rc != MB_SUCCESS) return rc;
   }
-  return rc;
+  return p.row_ctas > 0 && !p.whole ? launch_paged_rows_merge(a, p.rows, p.row_ctas, stream) : MB_SUCCESS;
 }
 
 }  // namespace mb

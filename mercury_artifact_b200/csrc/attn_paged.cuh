@@ -24,6 +24,9 @@ struct PagedAttnArgs {
   float2* part_ml;
   int4* open;
   int whole;  // few rows: CTA i has unit i, and nothing is joined
+  // The kernel for few rows comes right behind one for tiles and runs beside it: it starts as soon as all of that one's CTAs
+  // have (these wait for what came before them first), and does not end before it.
+  int beside;
   // tiles: keys (in tiles of 128) of a share of a unit; partial results [CTA][32 column groups][256 rows], (maximum, sum)
   // [CTA][256]; tile_open: the split unit whose first share a CTA has (sequence, K/V head, row block, shares; 0: none).
   // All null where no unit is split.
@@ -47,6 +50,8 @@ int paged_rows_step(bool fp8);  // keys
 // The first a.packed_rows keys and values of the sequences [a.b_begin, a.b_end) with at least min_new new tokens, in bf16.
 int launch_read_e4m3(const PagedAttnArgs& a, int min_new, cudaStream_t stream);
 int launch_paged_tiles(const PagedAttnArgs& a, int ctas, cudaStream_t stream);
+int launch_paged_tiles_merge(const PagedAttnArgs& a, int ctas, cudaStream_t stream);
+int launch_paged_rows_merge(const PagedAttnArgs& a, int rows, int ctas, cudaStream_t stream);
 long long paged_tiles_workspace(long long ctas);
 
 }  // namespace mb

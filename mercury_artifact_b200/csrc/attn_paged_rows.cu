@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   const uint32_t stage0 = smem_u32(stages);
 
   grid_dependents_launch();
-  grid_dependency_wait();
+  if (!a.beside) grid_dependency_wait();
 
   // This CTA's part of the list.  A thread looks at every 256th sequence; up to 256 of them are looked at once.
   RowIter in;  // what is loaded next
@@ -220,7 +220,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       if (lane == 0) a.lse[b * a.lse_sb + hd * a.lse_sh + tok] = -INFINITY;
     }
   }
-  if (total == 0) return;
+  if (total == 0) {
+    if (a.beside) grid_dependency_wait();
+    return;
+  }
   if (!a.whole) {
     in.b = sm->b;
     in.s = paged_seq(a.c, in.b, a.max_queries, a.max_keys);
@@ -641,6 +644,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     }
     at = nx;
   }
+  if (a.beside) grid_dependency_wait();
 }
 
 // Joins the partial states of the unit that CTA blockIdx.x of the launch before began and did not finish (if there is one).
@@ -726,15 +730,17 @@ static int launch_rows(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   }
   if (!launch_overlapped("launch paged_rows_kernel", paged_rows_kernel<kFp8, kTiles>, dim3(ctas), kRowThreads, bytes, stream, a))
     return MB_E_CUDA;
-  if (!a.whole && !launch_overlapped("launch paged_merge_kernel", paged_merge_kernel<8 * kTiles>,
-                         dim3(ctas), kRowThreads, 0, stream, a))
-    return MB_E_CUDA;
   return MB_SUCCESS;
 }
 
 int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream) {
   if (paged_rows_padded(rows) == 8) return fp8 ? launch_rows<true, 1>(a, ctas, stream) : launch_rows<false, 1>(a, ctas, stream);
   return fp8 ? launch_rows<true, 2>(a, ctas, stream) : launch_rows<false, 2>(a, ctas, stream);
+}
+
+int launch_paged_rows_merge(const PagedAttnArgs& a, int rows, int ctas, cudaStream_t stream) {
+  const auto kernel = paged_rows_padded(rows) == 8 ? paged_merge_kernel<8> : paged_merge_kernel<16>;
+  return launch_overlapped("launch paged_merge_kernel", kernel, dim3(ctas), kRowThreads, 0, stream, a) ? MB_SUCCESS : MB_E_CUDA;
 }
 
 }  // namespace mb

@@ -146,8 +146,8 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
   volatile int* abort_word = &ctl->abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  grid_dependents_launch();
   grid_dependency_wait();
+  grid_dependents_launch();
   if (warp == 0) {
     find_item(a, ctl, lane);
     __syncwarp();
@@ -641,11 +641,14 @@ static int launch_tiles(const TileMaps& maps, const PagedAttnArgs& a, int ctas, 
   if (!launch_overlapped("launch paged_tiles_kernel", paged_tiles_kernel<kMode>, dim3(ctas), TileShape<kMode>::kThreads, bytes,
                          stream, maps, a))
     return MB_E_CUDA;
-  if (a.tile_open != nullptr &&
-      !launch_overlapped("launch paged_tiles_merge_kernel", paged_tiles_merge_kernel,
-                         dim3(ctas, (2 * kBM) / kTileMergeRows), 256, 0, stream, a))
-    return MB_E_CUDA;
   return MB_SUCCESS;
+}
+
+int launch_paged_tiles_merge(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
+  return launch_overlapped("launch paged_tiles_merge_kernel", paged_tiles_merge_kernel, dim3(ctas, (2 * kBM) / kTileMergeRows),
+                           256, 0, stream, a)
+             ? MB_SUCCESS
+             : MB_E_CUDA;
 }
 
 // Boxes of `box` slots of 64 columns of a head, out of [pages, slots, heads, 128] with strides in bytes.
