@@ -29,12 +29,12 @@ static long long align_up(long long n) { return (n + 255) & ~255ll; }
 static int plan_paged(const mb_attn_paged_args* x, PagedPlan* p) {
   const mb_paged_kv& kv = x->kv;
   if (x->hq <= 0 || kv.hkv <= 0 || x->hq % kv.hkv != 0) return MB_E_INVALID;
-  if (x->max_queries < 0 || x->max_keys < 0 || !(x->softmax_scale > 0.f) || x->softmax_scale > 3e38f) return MB_E_INVALID;
+  if (x->max_queries < 0 || x->max_keys < 0 || !(x->softmax_scale > 0.f) || x->softmax_scale > 2e38f /* (times log2(e)) */) return MB_E_INVALID;
   if (kv.batch < 0 || kv.tokens < 0 || kv.page_size <= 0 || kv.max_pages < 0) return MB_E_INVALID;
   const long long heads = x->hq / kv.hkv, rows = x->max_queries * heads;
-  if (rows > 0x7fffff00ll) return MB_E_TOO_LARGE;
+  if (rows > 0x7fffff00ll) return MB_E_UNSUPPORTED;
   // steps of a launch are counted in 32 bits
-  if ((double)kv.batch * kv.hkv * ((double)x->max_keys / 128 + 1) > 2e9) return MB_E_TOO_LARGE;
+  if ((double)kv.batch * kv.hkv * ((double)x->max_keys / 128 + 1) > 2e9) return MB_E_UNSUPPORTED;
   const int sms = sm_count();
   if (sms <= 0) return MB_E_CUDA;
   memset(p, 0, sizeof(*p));
@@ -42,8 +42,9 @@ static int plan_paged(const mb_attn_paged_args* x, PagedPlan* p) {
   // Beside chunks the sequences with few rows are single tokens as a rule, which the kernels for fewer rows take faster.
   p->few = rows > kFewRows && heads <= 8 ? 8 : kFewRows;
   if (e4m3 && rows <= kFewRowsE4m3) p->few = kFewRowsE4m3;
+  p->few = (int)min(rows, (long long)p->few);
   if (rows <= p->few || !padded) {
-    p->rows = (int)min(rows, (long long)p->few);
+    p->rows = p->few;
     const int block = paged_rows_padded(p->rows);
     const long long units = (long long)kv.batch * kv.hkv * ((p->few + block - 1) / block);
     const int step = paged_rows_step(e4m3);
@@ -76,7 +77,7 @@ static int plan_paged(const mb_attn_paged_args* x, PagedPlan* p) {
     }
     p->share_tiles = (int)((tiles + best - 1) / best);
     const long long ctas = units * ((tiles + p->share_tiles - 1) / p->share_tiles);
-    if (ctas > 0x7fffff00ll) return MB_E_TOO_LARGE;
+    if (ctas > 0x7fffff00ll) return MB_E_UNSUPPORTED;
     p->tile_ctas = (int)ctas;
     p->split = best > 1;
     if (p->split) p->split_bytes = align_up(paged_tiles_workspace(p->tile_ctas));

@@ -164,9 +164,10 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
         ctl->last[0] = min(n[0], end);
         ctl->last[1] = min(n[1], end);
       }
-      // the merge finds a split unit at the CTA of its first share
+      // the merge finds a split unit at the CTA of its first share (offsets that do not ascend may ask for more CTAs than
+      // there are: what the last of them begin is left out)
       if (a.tile_open != nullptr)
-        a.tile_open[blockIdx.x] = ctl->valid && ctl->part == 0 && ctl->parts > 1
+        a.tile_open[blockIdx.x] = ctl->valid && ctl->part == 0 && ctl->parts > 1 && blockIdx.x + ctl->parts <= gridDim.x
                                       ? make_int4(ctl->b, ctl->h, ctl->block, ctl->parts) : make_int4(0, 0, 0, 0);
     }
   } else if (warp == 1 && lane == 0) {

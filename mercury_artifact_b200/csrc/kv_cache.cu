@@ -18,6 +18,7 @@ int paged_view(const mb_paged_kv* x, PagedView* c) {
   if (x->head_dim != kHeadDim) return MB_E_UNSUPPORTED;
   if (x->dtype != MB_DTYPE_BF16 && x->dtype != MB_DTYPE_E4M3) return MB_E_UNSUPPORTED;
   if (x->batch < 0 || x->tokens < 0 || x->pages < 0 || x->page_size <= 0 || x->max_pages < 0 || x->hkv <= 0) return MB_E_INVALID;
+  if (x->tokens > 0x7fffff00 || x->hkv > 1 << 20) return MB_E_UNSUPPORTED;  // (indices in 32 bits)
   const int size = x->dtype == MB_DTYPE_E4M3 ? 1 : 2;
   if (x->batch > 0 && (x->seq_lens == nullptr || (x->max_pages > 0 && x->page_table == nullptr))) return MB_E_INVALID;
   if (x->pages > 0) {
@@ -288,10 +289,17 @@ int launch_kv_cache_write(const mb_paged_kv* kv, const void* k_new, const void* 
                                                                                                                : MB_E_CUDA;
 }
 
-static int launch_read(const CacheMoveArgs& a, bool fp8, int sequences, cudaStream_t stream) {
-  const dim3 grid((a.rows + kReadTokens - 1) / kReadTokens, sequences);
+static int launch_read(CacheMoveArgs a, bool fp8, int sequences, cudaStream_t stream) {
+  constexpr int kMost = 65535;  // of a grid's second dimension
   const auto kernel = fp8 ? kv_cache_read_kernel<true> : kv_cache_read_kernel<false>;
-  return launch_overlapped("launch kv_cache_read_kernel", kernel, grid, kMoveThreads, 0, stream, a) ? MB_SUCCESS : MB_E_CUDA;
+  for (int done = 0; done < sequences; done += kMost) {
+    const dim3 grid((a.rows + kReadTokens - 1) / kReadTokens, min(sequences - done, kMost));
+    if (!launch_overlapped("launch kv_cache_read_kernel", kernel, grid, kMoveThreads, 0, stream, a)) return MB_E_CUDA;
+    a.first_seq += kMost;
+    a.k += kMost * a.sb;
+    a.v += kMost * a.sb;
+  }
+  return MB_SUCCESS;
 }
 
 int launch_read_e4m3(const PagedAttnArgs& x, int min_new, cudaStream_t stream) {
@@ -314,10 +322,9 @@ int launch_kv_cache_read(const mb_paged_kv* kv, void* k_out, void* v_out, long l
   CacheMoveArgs a;
   const int rc = paged_view(kv, &a.c);
   if (rc != MB_SUCCESS) return rc;
-  if (rows < 0) return MB_E_INVALID;
+  if (rows < 0 || rows > 0x7fffff00) return MB_E_INVALID;
   if (a.c.batch == 0 || rows == 0) return MB_SUCCESS;
   if (k_out == nullptr || v_out == nullptr || !aligned_rows(k_out, v_out, sb, ss, sh)) return MB_E_INVALID;
-  if (a.c.batch > 65535) return MB_E_UNSUPPORTED;  // grid dimension
   a.k = static_cast<uint8_t*>(k_out);
   a.v = static_cast<uint8_t*>(v_out);
   a.sb = sb * 2; a.st = ss * 2; a.sh = sh * 2;

@@ -38,7 +38,8 @@ class PagedKV:
     transposed) as long as head_dim is contiguous, k and v share their strides, and these are multiples of 16 bytes.
     bfloat16, or float8_e4m3fn with k_scale, v_scale: contiguous uint8 [pages, heads, page_size, 4].  Byte x is the power
     of two 2^(x - 127) that 32 values share: a code times its power of two is exact in bfloat16.  A write chooses 77 .. 191;
-    bytes from 192 on make their values NaN.  The NaN codes of e4m3 (0x7f, 0xff) are not used: they would count as 480.
+    bytes from 192 on make their values NaN.  No write makes e4m3's
+    NaN codes (0x7f, 0xff), and what the calls make of them is not defined.
     """
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
@@ -119,8 +120,8 @@ class PagedKV:
             cu = cu_seqlens.data_ptr()
         if columns * self.page_size > 0x7fffff00:
             raise ValueError("a page table may cover at most 2147483392 keys")
-        if tokens > 0x7fffffff:
-            raise ValueError("at most 2147483647 new tokens per call")
+        if tokens > 0x7fffff00:
+            raise ValueError("at most 2147483392 new tokens per call")
         return (*self._head, page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr(), cu, b, tokens, *self._tail,
                 columns, *self._kind)
 
@@ -249,6 +250,8 @@ def attn_fwd_paged(
     else:
         tokens = shape[0]
         max_queries = tokens if max_queries is None else min(int(max_queries), tokens)
+        if max_queries == 0 and tokens > 0:  # no sequence has new tokens, or the bound is wrong and the device says so
+            max_queries = 1
         lse_shape = (hq, tokens)
     if max_queries < 0 or max_keys < 0:
         raise ValueError("max_queries and max_keys must not be negative")

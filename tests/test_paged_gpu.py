@@ -390,6 +390,67 @@ def test_bad_pages_lengths_and_offsets_are_reported(fp8, new):
     check(batch, o, lse, want)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_offsets_that_ask_for_more_work_than_a_launch_has(fp8):
+    """Offsets that do not ascend give every other sequence all tokens: more units, each split over several SMs, than the
+    launch was cut for.  It is reported, and nothing but o and lse is written."""
+    from mercury_artifact_b200._lib import MercuryB200Error
+
+    mb = _mb()
+    batch = Batch([4096] * 6, [256] + [0] * 5, (8, 1), 16, fp8, seed=21)
+    cache = _cache(batch, batch.cache_tensors())
+    cu = torch.tensor([0, 256, 0, 256, 0, 256, 0], dtype=torch.int32, device="cuda")
+    guard = torch.full((300, 8, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    for _ in range(2):
+        mb.attn_fwd_paged(batch.on(batch.q), cache, batch.on(batch.table), batch.on(batch.seq_lens), SCALE, cu_seqlens=cu,
+                          out=guard[:256])
+        with pytest.raises(MercuryB200Error, match="page number"):
+            cache.check()
+    assert (guard[256:] == 7).all()
+    o, lse = mb.attn_fwd_paged(batch.on(batch.q), cache, batch.on(batch.table), batch.on(batch.seq_lens), SCALE,
+                               cu_seqlens=batch.on(batch.cu))
+    cache.check()
+    check(batch, o, lse, batch.expected(batch.cache_tensors(), True))
+
+
+def test_more_sequences_than_a_grid_dimension_has():
+    """70 000 sequences of at most one key share a page."""
+    mb = _mb()
+    n = 70000
+    cache = mb.PagedKV.empty(1, 16, 1)
+    g = torch.Generator().manual_seed(22)
+    rows = torch.randn(2, 16, 1, D, generator=g).to(torch.bfloat16).cuda()
+    cache.k[0], cache.v[0] = rows[0], rows[1]
+    table = torch.zeros(n, 1, dtype=torch.int32, device="cuda")
+    lens = (torch.arange(n, device="cuda") % 2).to(torch.int32)
+    got = mb.kv_cache_read(cache, table, lens, max_keys=1)
+    want = rows[:, None, :1] * lens.view(1, n, 1, 1, 1)
+    assert torch.equal(got, want.to(torch.bfloat16))
+    q = torch.randn(n, 1, 1, D, generator=g).to(torch.bfloat16).cuda()
+    o, lse = mb.attn_fwd_paged(q, cache, table, lens, SCALE)
+    cache.check()
+    assert torch.equal(o[1::2], rows[1, :1].expand(n // 2, 1, 1, D)) and (o[0::2] == 0).all()
+    assert torch.isinf(lse[0::2]).all() and torch.isfinite(lse[1::2]).all()
+
+
+def test_bound_of_no_new_tokens():
+    """max_queries=0: right where no sequence has any, reported where one has more than a token."""
+    from mercury_artifact_b200._lib import MercuryB200Error
+
+    mb = _mb()
+    batch = Batch([40, 50], [5, 2], (4, 2), 16, seed=23)
+    cache = _cache(batch, batch.cache_tensors())
+    q, table, lens = batch.on(batch.q), batch.on(batch.table), batch.on(batch.seq_lens)
+    out = torch.full_like(q, 7.0)
+    none = torch.zeros(3, dtype=torch.int32, device="cuda")
+    mb.attn_fwd_paged(q, cache, table, lens, SCALE, cu_seqlens=none, max_queries=0, out=out)
+    cache.check()
+    assert (out == 7).all()
+    mb.attn_fwd_paged(q, cache, table, lens, SCALE, cu_seqlens=batch.on(batch.cu), max_queries=0)
+    with pytest.raises(MercuryB200Error, match="page number"):
+        cache.check()
+
+
 @pytest.mark.parametrize("fp8", FP8)
 def test_captured_graph_replays_with_other_lengths(fp8):
     """Write, attend and attend with a chunk, captured once; the lengths, pages and rows change between replays."""
