@@ -7,16 +7,19 @@
 // per row, probabilities in bf16 as the tensor-memory operand of O += P V.
 //
 // What differs is how keys and values arrive.  A page may end anywhere inside a tile, pages lie anywhere, and
-// the slots behind a sequence's end hold anything (values that are not numbers among it).  Three ways:
+// the slots behind a sequence's end hold anything (values that are not numbers among it).  Two ways:
 //   kBoxes   bf16, pages of a multiple of 8 slots: TMA boxes of the largest power of two of slots that divides a page; boxes
 //            behind the end are fetched from behind the last page, which fills in zeros, and the rows of the
 //            last box that lie behind the end are cleared before the values are used (hidden scores are replaced anyway).
+//            Copies are issued at some 55 cycles a box, which is why two warps share them: 2 048 tokens against
+//            32 768 keys, 32/8 heads, take 801 us with pages of 64 (attn_fwd over contiguous keys: 808), 1 029 with pages of 16
+//            (1 177 with one warp), 1 327 with pages of 8.
 //   kRows    bf16, other pages: four more warps gather row by row with cp.async, 16 bytes a piece, straight into the
-//            swizzled layout that tcgen05 reads.
-// Codes (e4m3) are brought into bf16 before, into a buffer where every sequence is one page (launch_read_e4m3).  Turning them
-// on their way into shared memory instead, by four more warps, was built and measured: it took 1.35 ms where the copy
-// (35 us) and these tiles take 0.86 (2 048 tokens, 32 768 keys, 32/8 heads), because the tiles then stall on the
-// conversion's instructions, and no less time with one block of rows per sequence (64 tokens: 88 us, 85).
+//            swizzled layout that tcgen05 reads: the same with pages of 17 takes 1 094 us.
+// Codes (e4m3) are brought into bf16 before, into a buffer where every sequence is one page (launch_read_e4m3): 820 us for the
+// same tokens.  Turning them on their way into shared memory instead, by four more warps, took 1 354 us, because the tiles
+// then stall on the conversion's instructions; with 128 tokens against 8 192 keys 141 us where the copy and the tiles take 115.
+// (Only one block of rows per sequence gained: 64 tokens 89 us, 99 by the copy.)
 //
 //   warps 0-3   softmax + epilogue of query tile 0 (one thread per row)
 //   warps 4-7   softmax + epilogue of query tile 1; warps 0-7 also gather the queries
@@ -26,6 +29,12 @@
 // A launch has one CTA per (sequence, 256 rows, K/V head, share of the keys), found on the device from the lengths that
 // are there; CTAs beyond the last of them return.  Shares leave their unnormalised rows, maxima and sums in
 // the workspace and paged_tiles_merge_kernel joins them in order.
+//
+// Bound by the tensor cores and, as in attn_fwd, by the exponentials beside them: a step of 128 keys takes an SM some 1.9 us.
+// Unequal sequences cost more than that: 16 e4m3 sequences, 5 of them chunks of up to 512 tokens, up to 8 192 keys, take
+// 170 us, of which the longest unit's 64 steps are 124.  Choosing the shares on the device by the lengths that are there, and
+// starting the longest units first, was built: 187 us, as smaller shares only bring the tiles to 105-110 us and cost a
+// launch and the SMs on which the single tokens run meanwhile.
 #include "attn_paged.cuh"
 #include "attn_fwd_common.cuh"
 
@@ -34,7 +43,7 @@ namespace mb {
 enum TileMode { kBoxes, kRows };
 
 // Threads; registers at launch, of the softmax warps and of the others (an increase beyond what the CTA was launched with
-// would block forever, hence the check).  
+// would block forever, hence the check).
 template <int kMode>
 struct TileShape {
   static constexpr int kThreads = kMode == kBoxes ? 384 : 512;

@@ -4,7 +4,12 @@
 // A group of lanes moves one row (the 128 values of a head of K or V of a token): 16 lanes of 8 values in bf16, 8 lanes
 // of 16 values in e4m3, so that every access is 16 bytes a lane and whole rows at a time.  A block takes a run of
 // rows, its threads look the places of its tokens up first (in shared memory), then every group moves its rows with
-// all loads issued before the first store.
+// all loads issued before the first store.  Four rows a group measured best for many tokens (e4m3, two prompts of 32 768, 8
+// heads: 1, 2, 4 and 8 rows a group: 100, 85, 81, 99 us), one for few, which have too few blocks otherwise.
+//
+// Measured: that write 77-81 us, 407 MB, 5.2 TB/s of the 6.5 of a plain copy; three prompts of 1 500 to 9 001 tokens in bf16
+// 18 us, 5.5 TB/s; reading 62 768 e4m3 keys of 8 heads back 66 us, 5.9 TB/s; single tokens of 32 sequences 9 us, all of it the
+// host's launch.
 //
 // Why powers of two: a code has 4 significant bits, so code * 2^e is exact in bf16.  What is read back, and what the
 // attention kernels multiply, is the stored value itself with no second rounding; a factor of amax / 448 would use
