@@ -32,9 +32,9 @@
 //
 // Bound by the tensor cores and, as in attn_fwd, by the exponentials beside them: a step of 128 keys takes an SM some 1.9 us.
 // Unequal sequences cost more than that: 16 e4m3 sequences, 5 of them chunks of up to 512 tokens, up to 8 192 keys, take
-// 170 us, of which the longest unit's 64 steps are 124.  Choosing the shares on the device by the lengths that are there, and
-// starting the longest units first, was built: 187 us, as smaller shares only bring the tiles to 105-110 us and cost a
-// launch and the SMs on which the single tokens run meanwhile.
+// 170 us, of which the longest unit's 64 steps are 124.  Choosing the shares on the device by the lengths that are there was
+// built: 187 us, as smaller shares only bring the tiles to 105-110 us and cost a launch and the SMs on which the single
+// tokens run meanwhile.
 #include "attn_paged.cuh"
 #include "attn_fwd_common.cuh"
 
@@ -99,11 +99,13 @@ __device__ __forceinline__ int key_shares(const PagedAttnArgs& a, const PagedSeq
   return max(1, (tiles_of(s.len) + a.share_tiles - 1) / a.share_tiles);
 }
 
-// The item of this CTA: sequences one after the other; inside one, blocks of heads whose keys and values fit a part
-// of L2, in such a block the row blocks from the last (longest) to the first, then heads, then shares.  (One warp.)
+// The item of this CTA: sequences one after the other, up to 32 of them the longest first (then short units fill the end: 8
+// sequences of 100 to 448 tokens, 200 to 1 500 keys, 16 heads: 36.3 us, 38.8 in their own order); inside one, blocks of heads
+// whose keys and values fit a part of L2, in such a block the row blocks from the last (longest) to the first, then
+// heads, then shares.  (One warp.)
 __device__ __forceinline__ void find_item(const PagedAttnArgs& a, TileSmem* ctl, int lane) {
   int before = 0, found = 0;
-  const int want = blockIdx.x;
+  const int want = blockIdx.x, sequences = a.b_end - a.b_begin;
   for (int b0 = a.b_begin; b0 < a.b_end && !found; b0 += 32) {
     const int b = b0 + lane;
     PagedSeq s{0, 0, 0};
@@ -113,12 +115,20 @@ __device__ __forceinline__ void find_item(const PagedAttnArgs& a, TileSmem* ctl,
       items = row_blocks(a, s) * a.c.hkv * key_shares(a, s);
     }
     int incl = items;
+    if (sequences <= 32) {
+      incl = 0;
+      for (int i = 0; i < sequences; ++i) {
+        const int theirs = __shfl_sync(0xffffffffu, items, i), len = __shfl_sync(0xffffffffu, s.len, i);
+        if (len > s.len || (len == s.len && i <= lane)) incl += theirs;
+      }
+    } else {
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += up;
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += up;
+      }
+      incl += before;
     }
-    incl += before;
     const bool mine = want < incl && want >= incl - items;
     if (mine) {
       const int shares = key_shares(a, s), blocks = row_blocks(a, s);
