@@ -18,8 +18,8 @@ struct PagedAttnArgs {
   // rows of a sequence: new tokens x heads of a group.  Sequences with at most `few` rows belong to the kernel for
   // few rows, the others to the kernel for tiles.
   int few;
-  // partial results: [slot][row][128] and (maximum, sum) [slot][row]; open: the unit that a CTA began and left to the
-  // next ones (sequence, K/V head, number of CTAs; 0: none)
+  // partial results: [slot][head of a CTA][row][128] and (maximum, sum) [slot][head][row]; open: the unit that a CTA began and
+  // left to the next ones (sequence, K/V head / heads of a CTA, number of CTAs, block of rows; first token, rows; CTAs 0: none)
   float* part_o;
   float2* part_ml;
   int4* open;
@@ -43,15 +43,17 @@ struct PagedAttnArgs {
 
 constexpr float kLn2 = 0.6931471805599453f;
 
-int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream);
-long long paged_rows_workspace(int rows, int ctas);
+// heads: neighbouring K/V heads of a CTA, 1 or 2 (e4m3 only)
+int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int heads, int ctas, cudaStream_t stream);
+long long paged_rows_slots(int rows, int heads, int ctas);  // rows of partial results
+long long paged_rows_workspace(int rows, int heads, int ctas);
 int paged_rows_padded(int rows);
-int paged_rows_step(bool fp8);  // keys
+int paged_rows_step(bool fp8);  // keys of one head
 // The first a.packed_rows keys and values of the sequences [a.b_begin, a.b_end) with at least min_new new tokens, in bf16.
 int launch_read_e4m3(const PagedAttnArgs& a, int min_new, cudaStream_t stream);
 int launch_paged_tiles(const PagedAttnArgs& a, int ctas, cudaStream_t stream);
 int launch_paged_tiles_merge(const PagedAttnArgs& a, int ctas, cudaStream_t stream);
-int launch_paged_rows_merge(const PagedAttnArgs& a, int rows, int ctas, cudaStream_t stream);
+int launch_paged_rows_merge(const PagedAttnArgs& a, int rows, int heads, int ctas, cudaStream_t stream);
 long long paged_tiles_workspace(long long ctas);
 
 }  // namespace mb

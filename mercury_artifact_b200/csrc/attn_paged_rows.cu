@@ -13,6 +13,8 @@
 // probabilities through tensor memory and a hand-over between roles for every 128 keys; here a step's operands never leave
 // the warp's registers.  Only the end of a unit needs the other warps: their states are merged in shared memory.
 //
+// A CTA takes one K/V head, of e4m3 two neighbours with four warps each where it can, so that 256 bytes lie in a row.
+//
 // e4m3: codes are turned into f16 and multiplied by their powers of two relative to the step's largest (see
 // paged_common.cuh), which is what the instructions of a step go to; P is rounded to f16, scores and sums are fp32.
 //
@@ -22,8 +24,8 @@
 // several CTAs leaves a partial state in each, and paged_merge_kernel joins them in order: results do not depend on timing.
 //
 // Measured, one token each of 64 sequences, 32 query and 8 K/V heads, pages of 16: bf16, 50 to 8 192 keys, 1.15 GB: 192 us,
-// 6.0 TB/s (a plain copy: 6.5); e4m3, 100 to 16 384 keys, 1.04 GB: 200 us, 5.2 TB/s, where issuing the conversions takes
-// as long as the bytes.  The merge adds 4 us to a launch.
+// 6.0 TB/s (a plain copy: 6.5); e4m3, 100 to 16 384 keys, 1.04 GB: 187 us, 5.6 TB/s.  What is left of the difference is the start
+// (lengths, page numbers, first rows: a chain of loads) and the merge, some 4 us each, and unequal ends.
 #include "attn_paged.cuh"
 
 namespace mb {
@@ -40,7 +42,6 @@ struct RowShape {
   static constexpr int kHalf = kKeys * kRowBytes;                  // K or V of a stage: 4 KiB
   static constexpr int kScaleBytes = kFp8 ? kKeys * kScalesPerRow : 0;
   static constexpr int kStage = 2 * kHalf + 2 * kScaleBytes;
-  static constexpr int kStep = kKeys * kRowWarps;                  // keys of a CTA's step
   static_assert(kStage % 256 == 0, "rows are aligned to their size");
 };
 constexpr int kPitch = 132;  // of the merge buffers' rows, in floats: what the lanes of a warp store falls into different banks
@@ -49,14 +50,14 @@ struct RowSmem {
   int total, warp_sum[kRowWarps];
   int b, step;                               // where this CTA's part starts: sequence, and step inside it
   float2 ml[kRowWarps][16];                  // of a unit: every warp's maximum and sum,
-  float part_l[kRowWarps][16], row_top[16];  // its sum relative to the rows' maxima, these
-  float q_scale[16];  // e4m3: power of two that a row of queries was divided by
+  float part_l[kRowWarps][16], row_top[32];  // its sum relative to the rows' maxima, these
+  float q_scale[32];  // e4m3: power of two that a row of queries was divided by
 };
 
-template <bool kFp8>
+template <bool kFp8, int kHeads>
 constexpr int row_smem_bytes() {
-  // queries of 16 rows; merge buffers: 32 rows, of as many warps as fit
-  return kRowWarps * kRowStages * RowShape<kFp8>::kStage + 16 * 2 * kHeadDim + 32 * kPitch * 4 + (int)sizeof(RowSmem);
+  // queries of 16 rows a head; merge buffers: 32 rows, of as many warps as fit
+  return kRowWarps * kRowStages * RowShape<kFp8>::kStage + kHeads * 16 * 2 * kHeadDim + 32 * kPitch * 4 + (int)sizeof(RowSmem);
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -85,9 +86,9 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A place in the list of steps.  A sequence's units: K/V heads, and blocks of kRows rows of each.
+// A place in the list of steps.  A sequence's units: K/V heads (kHeads neighbours at once), and blocks of kRows rows of each.
 struct RowIter {
-  int b, h, block, blocks;  // block of rows, how many the sequence has
+  int b, h, block, blocks;  // heads / kHeads; block of rows, how many the sequence has
   int step, steps;          // of the unit
   PagedSeq s;
 };
@@ -100,17 +101,17 @@ template <int kRows>
 __device__ __forceinline__ int rows_blocks(const PagedAttnArgs& a, const PagedSeq& s) {
   return (s.n * a.group + kRows - 1) / kRows;
 }
-template <int kStep, int kRows>
+template <int kStep, int kRows, int kHeads>
 __device__ __forceinline__ int sequence_steps(const PagedAttnArgs& a, const PagedSeq& s) {
   const int steps = unit_steps<kStep>(a, s);
-  return steps == 0 ? 0 : steps * rows_blocks<kRows>(a, s) * a.c.hkv;
+  return steps == 0 ? 0 : steps * rows_blocks<kRows>(a, s) * (a.c.hkv / kHeads);
 }
-template <int kStep, int kRows>
+template <int kStep, int kRows, int kHeads>
 __device__ __forceinline__ void next_unit(const PagedAttnArgs& a, RowIter& it) {
   it.step = 0;
   if (++it.block < it.blocks) return;
   it.block = 0;
-  if (++it.h < a.c.hkv) return;
+  if (++it.h < a.c.hkv / kHeads) return;
   it.h = 0;
   it.steps = 0;
   while (++it.b < a.c.batch) {
@@ -120,9 +121,9 @@ __device__ __forceinline__ void next_unit(const PagedAttnArgs& a, RowIter& it) {
     if (it.steps > 0) return;
   }
 }
-template <int kStep, int kRows>
+template <int kStep, int kRows, int kHeads>
 __device__ __forceinline__ void next_step(const PagedAttnArgs& a, RowIter& it) {
-  if (++it.step >= it.steps) next_unit<kStep, kRows>(a, it);
+  if (++it.step >= it.steps) next_unit<kStep, kRows, kHeads>(a, it);
 }
 
 // Inclusive scan over the block of one value per thread, plus `before`; `all`: the last one's.
@@ -151,15 +152,17 @@ constexpr int kMinSteps = 2;
 __device__ __forceinline__ int row_ctas(int total, int grid) { return max(1, min(grid, total / kMinSteps)); }
 __device__ __forceinline__ int row_begin(int total, int i, int n) { return (int)((long long)total * i / n); }
 
-template <bool kFp8, int kTiles>
+template <bool kFp8, int kTiles, int kHeads>
 __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
   using S = RowShape<kFp8>;
-  constexpr int kStep = S::kStep, kKeys = S::kKeys, kGroups = kKeys / 16, kRows = 8 * kTiles;
+  constexpr int kWarps = kRowWarps / kHeads;  // of a head
+  constexpr int kKeys = S::kKeys, kStep = kWarps * kKeys, kGroups = kKeys / 16, kRows = 8 * kTiles;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int wh = warp / kWarps, wi = warp % kWarps;  // head of this warp, which of its warps it is
   uint8_t* stages = smem_raw + warp * (kRowStages * S::kStage);
   uint8_t* queries = smem_raw + kRowWarps * kRowStages * S::kStage;  // rows of 256 bytes, pieces swapped like the keys'
-  float* merge = reinterpret_cast<float*>(queries + 16 * 2 * kHeadDim);
+  float* merge = reinterpret_cast<float*>(queries + kHeads * 16 * 2 * kHeadDim);
   RowSmem* sm = reinterpret_cast<RowSmem*>(merge + 32 * kPitch);
   // e4m3: a step's powers of two in f16, twice [32 keys][4 blocks] for the keys, [4 blocks][32 keys] for the values; where
   // the states are merged at a unit's end
@@ -177,8 +180,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   if (a.whole) {
     const int most = (a.few + kRows - 1) / kRows;  // blocks of a sequence, at most
     int i = blockIdx.x;
-    in.b = i / (a.c.hkv * most);
-    i -= in.b * a.c.hkv * most;
+    in.b = i / (a.c.hkv / kHeads * most);
+    i -= in.b * (a.c.hkv / kHeads * most);
     in.h = i / most;
     in.block = i - in.h * most;
     in.step = 0;
@@ -194,20 +197,20 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       mine = 0;
       if (b < a.c.batch) {
         const PagedSeq s = paged_seq(a.c, b, a.max_queries, a.max_keys);
-        mine = sequence_steps<kStep, kRows>(a, s);
+        mine = sequence_steps<kStep, kRows, kHeads>(a, s);
         empty |= s.len == 0;
       }
       incl = row_scan(mine, total, sm->warp_sum, total);
     }
     ctas = row_ctas(total, gridDim.x);
-    if (tid == 0) a.open[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (tid == 0) a.open[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
     first = row_begin(total, blockIdx.x, ctas);
     last = row_begin(total, blockIdx.x + 1, ctas);
     int before = 0;
     for (int b0 = 0; b0 < a.c.batch; b0 += kRowThreads) {
       const int b = b0 + tid;
       if (a.c.batch > kRowThreads) {
-        mine = b < a.c.batch ? sequence_steps<kStep, kRows>(a, paged_seq(a.c, b, a.max_queries, a.max_keys)) : 0;
+        mine = b < a.c.batch ? sequence_steps<kStep, kRows, kHeads>(a, paged_seq(a.c, b, a.max_queries, a.max_keys)) : 0;
         incl = row_scan(mine, before, sm->warp_sum, before);
       }
       if (first >= incl - mine && first < incl) {
@@ -246,16 +249,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
 
   // the page table's entry for this lane's key of the step to load, fetched one step ahead
   auto entry_of = [&](const RowIter& it) {
-    const int pos = it.step * kStep + warp * kKeys + (lane & (kKeys - 1));
+    const int pos = it.step * kStep + wi * kKeys + (lane & (kKeys - 1));
     return pos < it.s.len ? paged_entry(a.c, it.b, pos) : 0;
   };
   int entry = entry_of(in);
 
   auto load = [&](int stage) {
-    const int pos = in.step * kStep + warp * kKeys + (lane & (kKeys - 1));
+    const int pos = in.step * kStep + wi * kKeys + (lane & (kKeys - 1));
     const int slot = pos - page_index(a.c, pos) * a.c.page_size;
     const int page = pos < in.s.len ? paged_id(a.c, entry, -1) : -1;
-    const long long off = page >= 0 ? paged_offset(a.c, page, slot, in.h) : -1;
+    const int head = in.h * kHeads + wh;
+    const long long off = page >= 0 ? paged_offset(a.c, page, slot, head) : -1;
     // Piece p of row r lies at place p ^ (r & 7) of its row.  With r = i * n + r0 (n: rows of a pass, a power of two above
     // r0) that is (p ^ r0) ^ (i * n & 7): one exclusive or with a constant, as rows are aligned to their size.
     constexpr int kPass = 32 / S::kPieces;
@@ -271,7 +275,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       cp_async16(to + S::kHalf, real ? a.c.v + from + piece * 16 : a.c.v, real);
     }
     if constexpr (kFp8) {
-      const long long so = page >= 0 ? scale_offset(a.c, page, slot, in.h) : 0;
+      const long long so = page >= 0 ? scale_offset(a.c, page, slot, head) : 0;
       cp_async4(dst + 2 * S::kHalf + lane * 4, a.c.k_scale + so, page >= 0);
       cp_async4(dst + 2 * S::kHalf + S::kScaleBytes + lane * 4, a.c.v_scale + so, page >= 0);
     }
@@ -283,7 +287,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     if (to_load > 0) {
       load(i);
       if (--to_load > 0) {
-        next_step<kStep, kRows>(a, in);
+        next_step<kStep, kRows, kHeads>(a, in);
         entry = entry_of(in);
       }
     }
@@ -292,16 +296,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
 
   // Queries: the next unit's are fetched into registers while this one's are in use (from shared memory).
   RowIter nx = at;  // the unit behind this one
-  constexpr int kPasses = (kTiles + 1) / 2;  // sixteen threads have a row, 16 rows at a time
+  constexpr int kPasses = (kHeads * kTiles + 1) / 2;  // sixteen threads have a row, 16 rows at a time
   uint4 qx[kPasses];
   auto fetch_q = [&]() {
 #pragma unroll
     for (int m = 0; m < kPasses; ++m) {
-      const int r = m * 16 + (tid >> 4), row = nx.block * kRows + r, tok = row / a.group, hd = row - tok * a.group;
+      const int at_row = m * 16 + (tid >> 4), h = at_row / kRows, row = nx.block * kRows + at_row % kRows;
+      const int tok = row / a.group, hd = row - tok * a.group;
       qx[m] = make_uint4(0, 0, 0, 0);
-      if (nx.b < a.c.batch && r < kRows && row < nx.s.n * a.group)
+      if (nx.b < a.c.batch && h < kHeads && row < nx.s.n * a.group)
         qx[m] = __ldg(reinterpret_cast<const uint4*>(a.q + nx.b * a.q_sb + (long long)(nx.s.start + tok) * a.q_st +
-                                                     (long long)(nx.h * a.group + hd) * a.q_sh) + (tid & 15));
+                                                     (long long)((nx.h * kHeads + h) * a.group + hd) * a.q_sh) + (tid & 15));
     }
   };
   // A lane of the matrix instruction takes element pairs (2 t, 2 t + 1) and (8 + 2 t, ...) of 16 along head_dim.  Of e4m3 keys
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     }
   };
   // Queries of 8 rows as the second operand, for 32 elements along head_dim (two products)
-  const uint32_t q_addr = smem_u32(queries) + (lane & 7) * 2 * kHeadDim + (((lane >> 3) ^ (lane & 7)) << 4);
+  const uint32_t q_addr = smem_u32(queries) + (wh * kRows + (lane & 7)) * 2 * kHeadDim + (((lane >> 3) ^ (lane & 7)) << 4);
   auto queries_of = [&](uint32_t (&qf)[4], int m, int k2) { ldsm4(qf, (q_addr ^ (k2 << 6)) + m * 8 * 2 * kHeadDim); };
 
   fetch_q();
@@ -335,7 +340,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     const int unit_end = min(last, s + at.steps - at.step);
     const bool done = unit_end == s + at.steps - at.step;
     store_q();
-    next_unit<kStep, kRows>(a, nx);
+    next_unit<kStep, kRows, kHeads>(a, nx);
     fetch_q();
     __syncthreads();  // the queries are there, and the buffers of the unit before are free again
     float acc[kTiles][8][4], m_ref[kTiles][2], l[kTiles][2];
@@ -356,7 +361,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         m_ref[m][e] = -INFINITY;
         l[m][e] = 0.f;
         limit[m][e] = a.causal ? min(at.s.len, at.s.len - at.s.n + (row0 + r) / a.group + 1) : at.s.len;
-        row_scale[m][e] = kFp8 ? sm->q_scale[r] : 1.f;
+        row_scale[m][e] = kFp8 ? sm->q_scale[wh * kRows + r] : 1.f;
       }
 #pragma unroll
       for (int k2 = 0; k2 < 4; ++k2) queries_of(qk[m][k2], m, k2);
@@ -368,7 +373,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       if (to_load > 0) {
         load(stage == 0 ? kRowStages - 1 : stage - 1);
         if (--to_load > 0) {
-          next_step<kStep, kRows>(a, in);
+          next_step<kStep, kRows, kHeads>(a, in);
           entry = entry_of(in);
         }
       }
@@ -378,7 +383,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
 
       // ---- one step
       const uint32_t sk = stage0 + stage * S::kStage, sv = sk + S::kHalf;
-      const int key0 = at.step * kStep + warp * kKeys;
+      const int key0 = at.step * kStep + wi * kKeys;
       float sc[kTiles][kGroups][4];  // of 16 keys each
 #pragma unroll
       for (int m = 0; m < kTiles; ++m)
@@ -578,7 +583,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         const int r = m * 8 + 2 * t + e;
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm->ml[w][r].x);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm->ml[wh * kWarps + w][r].x);
         f[m][e] = m_ref[m][e] == -INFINITY ? 0.f : fast_exp2(m_ref[m][e] - top);
         // a warp without a visible key has nothing, whatever its masked products gave
         const float mine = sm->ml[warp][r].y;
@@ -588,13 +593,14 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         }
         // (from here on: the row's maximum, and the warp's sum relative to it)
         if (g == 0) sm->part_l[warp][r] = m_ref[m][e] == -INFINITY ? mine : mine * f[m][e];
-        if (g == 0 && warp == 0) sm->row_top[r] = top;
+        if (g == 0 && wi == 0) sm->row_top[wh * kRows + r] = top;
       }
-    const int buffers = rows <= 4 ? 8 : 4 / kTiles, pitch = rows <= 4 ? 4 * kPitch : kRows * kPitch;
+    const int buffers = (rows <= 4 ? 8 : 4 / kTiles) / kHeads;  // of a head
+    const int pitch = rows <= 4 ? 4 * kPitch : kRows * kPitch;
 #pragma unroll 1
-    for (int round = 0; round < kRowWarps; round += buffers) {
-      if (warp >= round && warp < round + buffers) {
-        float* buf = merge + (warp - round) * pitch;
+    for (int round = 0; round < kWarps; round += buffers) {
+      if (wi >= round && wi < round + buffers) {
+        float* buf = merge + (wh * buffers + wi - round) * pitch;
 #pragma unroll
         for (int m = 0; m < kTiles; ++m)
 #pragma unroll
@@ -620,26 +626,29 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     }
     const bool whole = from_start && done;
     const int slot = 2 * blockIdx.x + (from_start ? 1 : 0);
-    for (int r = warp; r < rows; r += kRowWarps) {
+    for (int i = warp; i < kHeads * rows; i += kRowWarps) {
+      const int h = kHeads == 1 ? 0 : i / rows, r = i - h * rows;
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) sum += sm->part_l[w][r];
-      const float top = sm->row_top[r];
-      float4 x = *reinterpret_cast<const float4*>(merge + r * kPitch + lane * 4);
-      for (int i = 1; i < buffers; ++i) {
-        const float4 y = *reinterpret_cast<const float4*>(merge + i * pitch + r * kPitch + lane * 4);
+      for (int w = 0; w < kWarps; ++w) sum += sm->part_l[h * kWarps + w][r];
+      const float top = sm->row_top[h * kRows + r];
+      const float* buf = merge + h * buffers * pitch + r * kPitch + lane * 4;
+      float4 x = *reinterpret_cast<const float4*>(buf);
+      for (int b = 1; b < buffers; ++b) {
+        const float4 y = *reinterpret_cast<const float4*>(buf + b * pitch);
         x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
       }
       if (whole) {
-        const int tok = (row0 + r) / a.group, hd = at.h * a.group + row0 + r - tok * a.group;
+        const int tok = (row0 + r) / a.group, hd = (at.h * kHeads + h) * a.group + row0 + r - tok * a.group;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const uint2 w = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
         *reinterpret_cast<uint2*>(a.o + at.b * a.o_sb + (long long)(at.s.start + tok) * a.o_st + (long long)hd * a.o_sh + lane * 4) = w;
         if (lane == 0)
           a.lse[at.b * a.lse_sb + hd * a.lse_sh + at.s.start + tok] = sum == 0.f ? -INFINITY : top * kLn2 + __logf(sum);
       } else {
-        *reinterpret_cast<float4*>(a.part_o + ((long long)slot * kRows + r) * kHeadDim + lane * 4) = x;
-        if (lane == 0) a.part_ml[slot * kRows + r] = make_float2(top, sum);
+        const long long to = ((long long)slot * kHeads + h) * kRows + r;
+        *reinterpret_cast<float4*>(a.part_o + to * kHeadDim + lane * 4) = x;
+        if (lane == 0) a.part_ml[to] = make_float2(top, sum);
       }
     }
     if (from_start && !done && tid == 0) {
@@ -647,41 +656,38 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       const int end = s + at.steps - at.step;  // behind its last step
       int n = 1;
       while (row_begin(total, blockIdx.x + n, ctas) < end) ++n;
-      a.open[blockIdx.x] = make_int4(at.b, at.h, n, at.block);
+      a.open[2 * blockIdx.x] = make_int4(at.b, at.h, n, at.block);
+      a.open[2 * blockIdx.x + 1] = make_int4(at.s.start, rows, 0, 0);
     }
     at = nx;
   }
   if (a.beside) grid_dependency_wait();
 }
 
-// Joins the partial states of the unit that CTA blockIdx.x of the launch before began and did not finish (if there is one).
-// Of few parts a warp joins a row; of many, all warps join row after row, each an eighth of the parts.  A lane has four columns.
-// The parts are added in order.
-template <int kRows>
-__global__ void __launch_bounds__(kRowThreads) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
-  __shared__ float4 part[kRowWarps][32];
-  __shared__ float part_l[kRowWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// Joins the partial states of the unit that CTA blockIdx.x of the launch before began and did not finish (if there is one):
+// four rows of a head a block, two warps a row, each every other part; a lane has four columns.  The parts are added in order.
+// Bound by latency: the first parts are fetched before the maximum is known.
+constexpr int kMergeRows = 4, kMergeAhead = 4;
+template <int kRows, int kHeads>
+__global__ void __launch_bounds__(64 * kMergeRows) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
+  __shared__ float4 part[kMergeRows][32];
+  __shared__ float part_l[kMergeRows];
+  const int row = threadIdx.x >> 6, odd = (threadIdx.x >> 5) & 1, lane = threadIdx.x & 31;
   grid_dependents_launch();
   grid_dependency_wait();
-  const int4 unit = a.open[blockIdx.x];
-  if (unit.z == 0) return;
-  const PagedSeq seq = paged_seq(a.c, unit.x, a.max_queries, a.max_keys);
-  const int n = unit.z, row0 = unit.w * kRows, rows = min(seq.n * a.group - row0, kRows);
-  const bool many = n > 16;
-  for (int r = many ? 0 : warp; r < rows; r += many ? 1 : kRowWarps) {
-    // slot of the unit's p-th CTA: it ends the list of the first one and starts those of the others
-    auto slot = [&](int p) { return (long long)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * kRows + r; };
-    float top = -INFINITY;
-    for (int p = lane; p < n; p += 32) top = fmaxf(top, a.part_ml[slot(p)].x);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    float sum = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int p = many ? warp : 0; p < n; p += many ? kRowWarps : 1) {
-      const float2 ml = a.part_ml[slot(p)];
-      const float4 y = *reinterpret_cast<const float4*>(a.part_o + slot(p) * kHeadDim + lane * 4);
+  const int4 unit = a.open[2 * blockIdx.x], more = a.open[2 * blockIdx.x + 1];
+  const int n = unit.z, rows = more.y;
+  if (n == 0) return;
+  const int groups = gridDim.y / kHeads, h = blockIdx.y / groups, r = (blockIdx.y - h * groups) * kMergeRows + row;
+  const bool real = r < rows;
+  float sum = 0.f, top = -INFINITY;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (real) {
+    // row of the unit's p-th CTA: it ends the list of the first one and starts those of the others
+    auto slot = [&](int p) { return ((long long)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * kHeads + h) * kRows + r; };
+    auto state = [&](int p) { return a.part_ml[slot(p)]; };
+    auto values = [&](int p) { return *reinterpret_cast<const float4*>(a.part_o + slot(p) * kHeadDim + lane * 4); };
+    auto add = [&](const float2& ml, const float4& y) {
       // (a part without visible keys holds zeros, or what is not a number)
       const float w = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top);
       sum = fmaf(w, ml.y, sum);
@@ -689,65 +695,79 @@ __global__ void __launch_bounds__(kRowThreads) paged_merge_kernel(const __grid_c
       x.y = fmaf(w, y.y, x.y);
       x.z = fmaf(w, y.z, x.z);
       x.w = fmaf(w, y.w, x.w);
-    }
-    if (many) {
-      part[warp][lane] = x;
-      if (lane == 0) part_l[warp] = sum;
-      __syncthreads();
-      if (warp == 0) {
+    };
+    float2 ml[kMergeAhead];
+    float4 y[kMergeAhead];
 #pragma unroll
-        for (int w = 1; w < kRowWarps; ++w) {
-          const float4 y = part[w][lane];
-          sum += part_l[w];
-          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-        }
-      }
-      __syncthreads();
-      if (warp != 0) continue;
+    for (int i = 0; i < kMergeAhead; ++i) {
+      const int p = min(odd + 2 * i, n - 1);
+      ml[i] = state(p);
+      y[i] = values(p);
     }
-    const int tok = (row0 + r) / a.group, hd = unit.y * a.group + row0 + r - tok * a.group;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const uint2 w = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
-    *reinterpret_cast<uint2*>(a.o + unit.x * a.o_sb + (long long)(seq.start + tok) * a.o_st + (long long)hd * a.o_sh + lane * 4) = w;
-    if (lane == 0) a.lse[unit.x * a.lse_sb + hd * a.lse_sh + seq.start + tok] = sum == 0.f ? -INFINITY : top * kLn2 + __logf(sum);
+    for (int p = lane; p < n; p += 32) top = fmaxf(top, state(p).x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+#pragma unroll
+    for (int i = 0; i < kMergeAhead; ++i)
+      if (odd + 2 * i < n) add(ml[i], y[i]);
+#pragma unroll 4
+    for (int p = odd + 2 * kMergeAhead; p < n; p += 2) add(state(p), values(p));
+    if (odd) {
+      part[row][lane] = x;
+      if (lane == 0) part_l[row] = sum;
+    }
   }
+  __syncthreads();
+  if (!real || odd) return;
+  const float4 y = part[row][lane];
+  sum += part_l[row];
+  const int first = unit.w * kRows + r, tok = first / a.group, hd = (unit.y * kHeads + h) * a.group + first - tok * a.group;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const uint2 w = make_uint2(pack_bf16x2((x.x + y.x) * inv, (x.y + y.y) * inv), pack_bf16x2((x.z + y.z) * inv, (x.w + y.w) * inv));
+  *reinterpret_cast<uint2*>(a.o + unit.x * a.o_sb + (long long)(more.x + tok) * a.o_st + (long long)hd * a.o_sh + lane * 4) = w;
+  if (lane == 0) a.lse[unit.x * a.lse_sb + hd * a.lse_sh + more.x + tok] = sum == 0.f ? -INFINITY : top * kLn2 + __logf(sum);
 }
 
-int paged_rows_step(bool fp8) { return fp8 ? RowShape<true>::kStep : RowShape<false>::kStep; }
+int paged_rows_step(bool fp8) { return kRowWarps * (fp8 ? RowShape<true>::kKeys : RowShape<false>::kKeys); }
 
 // Rows of a block, for which the kernel is compiled
 int paged_rows_padded(int rows) { return rows <= 8 ? 8 : 16; }
 
-long long paged_rows_workspace(int rows, int ctas) {
-  return 2ll * ctas * paged_rows_padded(rows) * (kHeadDim * (long long)sizeof(float) + (long long)sizeof(float2)) + ctas * (long long)sizeof(int4);
+long long paged_rows_slots(int rows, int heads, int ctas) { return 2ll * ctas * heads * paged_rows_padded(rows); }
+long long paged_rows_workspace(int rows, int heads, int ctas) {
+  return paged_rows_slots(rows, heads, ctas) * (kHeadDim * (long long)sizeof(float) + (long long)sizeof(float2)) +
+         2ll * ctas * (long long)sizeof(int4);
 }
 
-template <bool kFp8, int kTiles>
+template <bool kFp8, int kTiles, int kHeads>
 static int launch_rows(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   static bool attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MB_E_CUDA;
-  constexpr int bytes = row_smem_bytes<kFp8>();
+  constexpr int bytes = row_smem_bytes<kFp8, kHeads>();
   static_assert(bytes <= 232448, "shared memory budget of one CTA");
+  const auto kernel = paged_rows_kernel<kFp8, kTiles, kHeads>;
   if (!attr_set[dev]) {
-    if (!cuda_ok(cudaFuncSetAttribute(paged_rows_kernel<kFp8, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
-                 "paged_rows_kernel shared memory"))
+    if (!cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "paged_rows_kernel shared memory"))
       return MB_E_CUDA;
     attr_set[dev] = true;
   }
-  if (!launch_overlapped("launch paged_rows_kernel", paged_rows_kernel<kFp8, kTiles>, dim3(ctas), kRowThreads, bytes, stream, a))
-    return MB_E_CUDA;
-  return MB_SUCCESS;
+  return launch_overlapped("launch paged_rows_kernel", kernel, dim3(ctas), kRowThreads, bytes, stream, a) ? MB_SUCCESS : MB_E_CUDA;
 }
 
-int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int ctas, cudaStream_t stream) {
-  if (paged_rows_padded(rows) == 8) return fp8 ? launch_rows<true, 1>(a, ctas, stream) : launch_rows<false, 1>(a, ctas, stream);
-  return fp8 ? launch_rows<true, 2>(a, ctas, stream) : launch_rows<false, 2>(a, ctas, stream);
+int launch_paged_rows(const PagedAttnArgs& a, bool fp8, int rows, int heads, int ctas, cudaStream_t stream) {
+  const bool one = paged_rows_padded(rows) == 8;
+  if (!fp8) return one ? launch_rows<false, 1, 1>(a, ctas, stream) : launch_rows<false, 2, 1>(a, ctas, stream);
+  if (heads == 1) return one ? launch_rows<true, 1, 1>(a, ctas, stream) : launch_rows<true, 2, 1>(a, ctas, stream);
+  return one ? launch_rows<true, 1, 2>(a, ctas, stream) : launch_rows<true, 2, 2>(a, ctas, stream);
 }
 
-int launch_paged_rows_merge(const PagedAttnArgs& a, int rows, int ctas, cudaStream_t stream) {
-  const auto kernel = paged_rows_padded(rows) == 8 ? paged_merge_kernel<8> : paged_merge_kernel<16>;
-  return launch_overlapped("launch paged_merge_kernel", kernel, dim3(ctas), kRowThreads, 0, stream, a) ? MB_SUCCESS : MB_E_CUDA;
+int launch_paged_rows_merge(const PagedAttnArgs& a, int rows, int heads, int ctas, cudaStream_t stream) {
+  const int block = paged_rows_padded(rows);
+  const auto kernel = block == 8 ? (heads == 1 ? paged_merge_kernel<8, 1> : paged_merge_kernel<8, 2>)
+                                 : (heads == 1 ? paged_merge_kernel<16, 1> : paged_merge_kernel<16, 2>);
+  const dim3 grid(ctas, heads * ((min(rows, block) + kMergeRows - 1) / kMergeRows));
+  return launch_overlapped("launch paged_merge_kernel", kernel, grid, 64 * kMergeRows, 0, stream, a) ? MB_SUCCESS : MB_E_CUDA;
 }
 
 }  // namespace mb
