@@ -157,6 +157,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   using S = RowShape<kFp8>;
   constexpr int kWarps = kRowWarps / kHeads;  // of a head
   constexpr int kKeys = S::kKeys, kStep = kWarps * kKeys, kGroups = kKeys / 16, kRows = 8 * kTiles;
+  constexpr bool kScaled = kFp8 && kTiles == 1;  // scores, not keys, are multiplied by the keys' powers of two
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int wh = warp / kWarps, wi = warp % kWarps;  // head of this warp, which of its warps it is
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   uint8_t* queries = smem_raw + kRowWarps * kRowStages * S::kStage;  // rows of 256 bytes, pieces swapped like the keys'
   float* merge = reinterpret_cast<float*>(queries + kHeads * 16 * 2 * kHeadDim);
   RowSmem* sm = reinterpret_cast<RowSmem*>(merge + 32 * kPitch);
-  // e4m3: a step's powers of two in f16, twice [32 keys][4 blocks] for the keys, [4 blocks][32 keys] for the values; where
+  // e4m3: a step's powers of two: [32 keys][4 blocks] for the keys, f16 twice (kScaled: fp32), [4 blocks][32 keys] for the values; where
   // the states are merged at a unit's end
   uint32_t* key_scale = reinterpret_cast<uint32_t*>(merge) + warp * 192;
   uint16_t* value_scale = reinterpret_cast<uint16_t*>(key_scale + 128);
@@ -409,16 +410,20 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
           }
         }
       } else {
-        // The powers of two of this lane's key, relative to the largest of the step
+        // The powers of two of this lane's key.  The values' are taken relative to the largest of the step, so that f16 holds the
+        // products; the keys' too, or with 8 rows the scores of 32 columns at a time are multiplied by them (kScaled: half as
+        // many products, and no rounding; 64 single tokens up to 16 384 keys 186 us and 182, 8 tokens each up to 8 192, 16 rows,
+        // 333 and 347).
         const uint32_t* words = reinterpret_cast<const uint32_t*>(stages + stage * S::kStage + 2 * S::kHalf);
         const uint32_t kw = words[lane], vw = words[kKeys + lane];
-        const int k_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(kw)), kMinScale);
+        int k_top = 127;
+        if constexpr (!kScaled) k_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(kw)), kMinScale);
         const int v_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(vw)), kMinScale);
         uint32_t ks[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const float k2 = scale_relative((kw >> (8 * b)) & 0xffu, k_top);
-          ks[b] = pack_f16x2(k2, k2);
+          ks[b] = kScaled ? __float_as_uint(k2) : pack_f16x2(k2, k2);
           value_scale[b * kKeys + lane] = (uint16_t)pack_f16x2(scale_relative((vw >> (8 * b)) & 0xffu, v_top), 0.f);
         }
         *reinterpret_cast<uint4*>(key_scale + lane * 4) = make_uint4(ks[0], ks[1], ks[2], ks[3]);
@@ -439,10 +444,14 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
             ldsm4(b, k_addr ^ ((2 * k2 + i) << 4));
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              kf[i][j][0] = mul_f16x2(e4m3_f16(b[2 * j]), mult[2 * j]);
-              kf[i][j][1] = mul_f16x2(e4m3_f16(b[2 * j + 1]), mult[2 * j + 1]);
-              kf[i][j][2] = mul_f16x2(e4m3_f16_high(b[2 * j]), mult[2 * j]);
-              kf[i][j][3] = mul_f16x2(e4m3_f16_high(b[2 * j + 1]), mult[2 * j + 1]);
+              kf[i][j][0] = e4m3_f16(b[2 * j]);
+              kf[i][j][1] = e4m3_f16(b[2 * j + 1]);
+              kf[i][j][2] = e4m3_f16_high(b[2 * j]);
+              kf[i][j][3] = e4m3_f16_high(b[2 * j + 1]);
+              if constexpr (!kScaled) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) kf[i][j][e] = mul_f16x2(kf[i][j][e], mult[2 * j + (e & 1)]);
+              }
             }
           }
 #pragma unroll
@@ -450,8 +459,16 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
             const uint32_t(&q)[4] = qk[m][k2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              mma16816<kFp8>(sc[m][j], kf[0][j], q[0], q[1]);
-              mma16816<kFp8>(sc[m][j], kf[1][j], q[2], q[3]);
+              if constexpr (kScaled) {
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816<kFp8>(part, kf[0][j], q[0], q[1]);
+                mma16816<kFp8>(part, kf[1][j], q[2], q[3]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[m][j][e] = fmaf(part[e], __uint_as_float(mult[2 * j + (e >> 1)]), sc[m][j][e]);
+              } else {
+                mma16816<kFp8>(sc[m][j], kf[0][j], q[0], q[1]);
+                mma16816<kFp8>(sc[m][j], kf[1][j], q[2], q[3]);
+              }
             }
           }
         }
