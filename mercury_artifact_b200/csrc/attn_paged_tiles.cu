@@ -11,9 +11,10 @@
 //   kBoxes   bf16, pages of a multiple of 8 slots: TMA boxes of the largest power of two of slots that divides a page; boxes
 //            behind the end are fetched from behind the last page, which fills in zeros, and the rows of the
 //            last box that lie behind the end are cleared before the values are used (hidden scores are replaced anyway).
-//            Copies are issued at some 55 cycles a box, which is why two warps share them: 2 048 tokens against
-//            32 768 keys, 32/8 heads, take 801 us with pages of 64 (attn_fwd over contiguous keys: 808), 1 029 with pages of 16
-//            (1 177 with one warp), 1 327 with pages of 8.
+//            Lanes issue one after the other, some 55 cycles a box, so that two warps share them, and four where boxes
+//            have fewer than 64 slots (kSmallBoxes; 512 threads, whose softmax warps have fewer registers).
+//            2 048 tokens against 32 768 keys, 32/8 heads, with two warps and with four (attn_fwd over contiguous
+//            keys: 808): pages of 64 840 and 858 us, of 32 960 and 844, of 16 1 120 and 965, of 8 1 347 and 1 110.
 //   kRows    bf16, other pages: four more warps gather row by row with cp.async, 16 bytes a piece, straight into the
 //            swizzled layout that tcgen05 reads: the same with pages of 17 takes 1 094 us.
 // Codes (e4m3) are brought into bf16 before, into a buffer where every sequence is one page (launch_read_e4m3): 820 us for the
@@ -23,7 +24,7 @@
 //
 //   warps 0-3   softmax + epilogue of query tile 0 (one thread per row)
 //   warps 4-7   softmax + epilogue of query tile 1; warps 0-7 also gather the queries
-//   warp  8     issues Q K^T, owns tensor memory;  warp 10 issues P V;  warps 9 and 11 issue TMA (kBoxes)
+//   warp  8     issues Q K^T, owns tensor memory;  warp 10 issues P V;  warps 9 and 11 issue TMA (kSmallBoxes: 12 and 13 too)
 //   warps 12-15 gather keys and values (kRows)
 //
 // A launch has one CTA per (sequence, 256 rows, K/V head, share of the keys), found on the device from the lengths that
@@ -40,7 +41,7 @@
 
 namespace mb {
 
-enum TileMode { kBoxes, kRows };
+enum TileMode { kBoxes, kSmallBoxes, kRows };
 
 // Threads; registers at launch, of the softmax warps and of the others (an increase beyond what the CTA was launched with
 // would block forever, hence the check).
@@ -193,7 +194,7 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
     mbar_init(&ctl->q_full, 256);
     mbar_init(&ctl->tail, 1);
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&ctl->kv_full[s], kMode == kBoxes ? 1 : 128);
+      mbar_init(&ctl->kv_full[s], kMode == kRows ? 128 : 1);
       mbar_init(&ctl->kv_empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -243,7 +244,7 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
     return n == positions - 1 ? total - 1 : which ? n / 2 - 1 : (n + 1) / 2;
   };
 
-  if (warp >= 12) {
+  if (warp >= (kMode == kSmallBoxes ? 14 : 12)) {
     // ------------------------------------------------------------------ gather
     give_registers<Shape::kOthers>();
     const int r = tid - 12 * 32;
@@ -298,16 +299,16 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
       fence_proxy_async_smem();
       for (int n = max(positions - 2, 0); n < positions; ++n) mbar_arrive(&ctl->kv_full[n % kStages]);
     }
-  } else if (warp == 9 || warp == 11) {
+  } else if (warp == 9 || warp == 11 || warp >= 12) {
     give_registers<Shape::kOthers>();
-    if constexpr (kMode == kBoxes) {
+    if constexpr (kMode != kRows) {
       // ---------------------------------------------------------------- TMA: a lane has a box of a tile, a warp half of
-      // its columns (lanes issue one after the other, some 55 cycles each: small pages are bound by it)
-      const int half = warp == 11;
-      const int len = ctl->seq.len, boxes = kBN / maps.box;
+      // its columns (kSmallBoxes: of half of the boxes)
+      const int half = warp == 11 || warp == 13, second = warp >= 12;
+      const int len = ctl->seq.len, boxes = kBN / maps.box / (kMode == kSmallBoxes ? 2 : 1), box0 = second ? boxes : 0;
       bool ok = true;
       auto page_of = [&](int j) {
-        const int pos = (first + j) * kBN + lane * maps.box;
+        const int pos = (first + j) * kBN + (box0 + lane) * maps.box;
         if (j >= total || lane >= boxes || pos >= len) return -1;
         return maps.packed ? ctl->b - a.b_begin : paged_entry(a.c, ctl->b, pos);
       };
@@ -318,7 +319,7 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
         const int j = tile_of(n, which);
         const int stage = n % kStages, round = n / kStages;
         const int entry = !which ? page : n == positions - 1 ? page1 : page2;
-        const int pos = (first + j) * kBN + lane * maps.box;
+        const int pos = (first + j) * kBN + (box0 + lane) * maps.box;
         const bool real = lane < boxes && pos < len;  // else zeros: a page behind the last one
         const int id = !real ? maps.pages : maps.packed ? entry : paged_id(a.c, entry, maps.pages);
         const int slot = !real ? 0 : maps.packed ? pos : pos - page_index(a.c, pos) * a.c.page_size;
@@ -327,11 +328,11 @@ paged_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant_
         const int k0 = (first + j) * kBN;
         const bool tail = which && k0 + kBN > len && len % maps.box != 0;  // a box holds rows behind the end
         uint64_t* full = tail ? &ctl->tail : &ctl->kv_full[stage];
-        uint8_t* dst = sKV + stage * kTileBytes + lane * maps.box * 128;
-        if (lane == 0 && half == 0) mbar_expect_tx(full, kTileBytes);  // (of both warps)
+        uint8_t* dst = sKV + stage * kTileBytes + (box0 + lane) * maps.box * 128;
+        if (lane == 0 && warp == 9) mbar_expect_tx(full, kTileBytes);  // (of all warps)
         __syncwarp();
         if (lane < boxes) tma_load_4d(dst + half * kHalfBytes, which ? &maps.v : &maps.k, full, half * 64, ctl->h, slot, id);
-        if (tail && half == 0) {  // (the last position: no other tile reaches the end)
+        if (tail && warp == 9) {  // (the last position: no other tile reaches the end)
           ok = mbar_wait_warp(&ctl->tail, 0, abort_word, MB_ERR_TIMEOUT_KV_FULL);
           const int from = len - k0, to = (from + maps.box - 1) / maps.box * maps.box;
           for (int i = from * 16 + lane; i < to * 16; i += 32)
@@ -702,7 +703,7 @@ int launch_paged_tiles(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   if (!page_map(&maps.k, c.k, c.hkv, c.page_size, c.pages, c.head_sb, c.slot_sb, c.page_sb, maps.box) ||
       !page_map(&maps.v, c.v, c.hkv, c.page_size, c.pages, c.head_sb, c.slot_sb, c.page_sb, maps.box))
     return MB_E_TENSORMAP;
-  return launch_tiles<kBoxes>(maps, a, ctas, stream);
+  return maps.box < 64 ? launch_tiles<kSmallBoxes>(maps, a, ctas, stream) : launch_tiles<kBoxes>(maps, a, ctas, stream);
 }
 
 }  // namespace mb
