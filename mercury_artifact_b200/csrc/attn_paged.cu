@@ -5,8 +5,9 @@ namespace mb {
 
 // Most rows of a sequence (new tokens x heads of a group) that the kernel for few rows takes.  bf16: 17 to 32 rows are faster
 // as (an eighth of) a tile, 64 sequences of 8 tokens, 32/8 heads, up to 8 192 keys: 281 us, 394 as rows; 8 of them: 71, 71.
-// e4m3: a tile's sequence is first brought into bf16, which few rows do not pay for: the same 64 sequences take 387 us as 32
-// rows; 64 rows of them (16 tokens) take 620 as tiles, of which some 270 are the copy.
+// e4m3: a tile's sequence is first brought into bf16, which few rows do not pay for: 64 sequences as 32 rows take 333 us.  From
+// there on it depends: with 10 tokens they take 562 us as tiles and 472 as 40 rows, 8 of them 86 and 111, 64 up to 1 000 keys
+// 96 and 131, one of 32 768 keys 80 and 58.
 constexpr int kFewRows = 16, kFewRowsE4m3 = 32;
 // Steps up to which a unit of few rows is left to one CTA where there are no more units than SMs.  One token, 16 sequences of
 // 2 000 keys, 8 heads: 26 us, split 35; one sequence, 2 heads: 20 and 28 (the host's time included).
