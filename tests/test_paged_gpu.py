@@ -170,6 +170,32 @@ def test_few_tokens(fp8, causal, new):
 
 
 @pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,new", [((8, 2), 1), ((8, 2), 2), ((8, 2), 3), ((8, 2), 8), ((12, 6), 5), ((3, 3), 7), ((6, 3), 2),
+                                       ((14, 2), 1), ((14, 2), 2), ((4, 4), 32)])
+def test_few_tokens_split_over_sms(fp8, causal, heads, new):
+    """Units that several SMs share, of an even and an odd number of K/V heads, in one block of rows and in more; bits repeat."""
+    batch = Batch([5000, 4097, new, 129 + new, 700], [new] * 5, heads, 16, fp8, ragged=False, seed=24, spread=2.0)
+    tensors = batch.cache_tensors()
+    cache = _cache(batch, tensors)
+    o, lse = _attend(batch, cache, causal)
+    o2, lse2 = _attend(batch, cache, causal)
+    assert _status() == 0
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    check(batch, o, lse, batch.expected(tensors, causal))
+
+
+@pytest.mark.parametrize("page", [8, 32, 40, 64, 96])
+def test_chunks_box_sizes(page):
+    """Every way a tile of keys is cut into boxes of pages."""
+    batch = Batch([page, 127, 129, 1000, 385], [page, 127, 100, 64, 385], (8, 2), page, seed=25)
+    tensors = batch.cache_tensors()
+    o, lse = _attend(batch, _cache(batch, tensors))
+    assert _status() == 0
+    check(batch, o, lse, batch.expected(tensors, True))
+
+
+@pytest.mark.parametrize("fp8", FP8)
 def test_one_long_sequence_over_all_sms(fp8):
     """One sequence, one K/V head: its keys are split over every SM and merged; and bits repeat."""
     batch = Batch([70001], [1], (4, 1), 64, fp8, ragged=False, seed=6, spread=2.0)
