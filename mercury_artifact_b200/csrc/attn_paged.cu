@@ -10,7 +10,7 @@ namespace mb {
 // 96 and 131, one of 32 768 keys 80 and 58.
 constexpr int kFewRows = 16, kFewRowsE4m3 = 32;
 // Steps up to which a unit of few rows is left to one CTA where there are no more units than SMs.  One token, 16 sequences of
-// 2 000 keys, 8 heads: 26 us, split 35; one sequence, 2 heads: 20 and 28 (the host's time included).
+// 2 000 keys, 8 heads: 27 us, split 32; one sequence, 2 heads: 20 and 28 (the host's time included).
 constexpr int kWholeSteps = 16;
 // e4m3: sequences that go to the tiles are brought into bf16 in groups that take no more than this (or one by one).  64
 // sequences of 16 tokens, up to 8 192 keys: 620 us; groups of 256 MiB 688, of 4 GiB 570, which is not worth the memory.

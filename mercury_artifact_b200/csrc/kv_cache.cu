@@ -5,9 +5,9 @@
 // of 16 values in e4m3, so that every access is 16 bytes a lane and whole rows at a time.  A block takes a run of
 // rows, its threads look the places of its tokens up first (in shared memory), then every group moves its rows with
 // all loads issued before the first store.  Four rows a group measured best for many tokens (e4m3, two prompts of 32 768, 8
-// heads: 1, 2, 4 and 8 rows a group: 100, 85, 81, 99 us), one for few, which have too few blocks otherwise.
+// heads, one turn: 1, 2, 4 and 8 rows a group: 100, 85, 81, 99 us), one for few, which have too few blocks otherwise.
 //
-// Measured: that write 77-81 us, 407 MB, 5.2 TB/s of the 6.5 of a plain copy; three prompts of 1 500 to 9 001 tokens in bf16
+// Measured: that write 74-76 us, 407 MB, 5.4 TB/s of the 6.5 of a plain copy; three prompts of 1 500 to 9 001 tokens in bf16
 // 18 us, 5.5 TB/s; reading 62 768 e4m3 keys of 8 heads back 66 us, 5.9 TB/s; single tokens of 32 sequences 9 us, all of it the
 // host's launch.
 //
@@ -110,11 +110,16 @@ __device__ __forceinline__ uint4 quantise16(const uint4 (&x)[2], uint32_t& byte)
   return make_uint4(q[0], q[1], q[2], q[3]);
 }
 
-// Rows of a block: r = (token * 2 + which) * hkv + head, `kIters` rows per group of lanes.
+// Rows of a block: r = (token * 2 + which) * hkv + head, `kIters` rows per group of lanes at a time.  Blocks of e4m3, which
+// are bound by their instructions and barriers as much as by memory, take two turns of them for one lookup (the prompts above:
+// 80.6 us with one turn, 75.8, 74.1 with four, which however leave short prompts too few blocks; bf16, two prompts of 32 768:
+// 83.6, 84.8, 86.9).
+template <bool kFp8, int kIters>
+constexpr int kTurns = kFp8 && kIters > 1 ? 2 : 1;
 template <bool kFp8, int kIters>
 __global__ void __launch_bounds__(kMoveThreads) kv_cache_write_kernel(const __grid_constant__ CacheMoveArgs a) {
   using S = MoveShape<kFp8>;
-  constexpr int kRows = S::kGroups * kIters;
+  constexpr int kRows = S::kGroups * kIters * kTurns<kFp8, kIters>;
   __shared__ long long place[kRows / 2 + 2], source[kRows / 2 + 2];  // of a token: byte offsets (-1: not stored)
   __shared__ long long place_scale[kFp8 ? kRows / 2 + 2 : 1];
   const PagedView& c = a.c;
@@ -172,43 +177,46 @@ __global__ void __launch_bounds__(kMoveThreads) kv_cache_write_kernel(const __gr
   // a group's i-th row and the end, counted from the first row of token t0 (divisions in 32 bits)
   const int row_in = (int)(row0 - (long long)t0 * per_token) + group;
   const int rows = (int)min(total - (long long)t0 * per_token, (long long)(kRows + per_token));
-  uint4 x[kIters][kFp8 ? 2 : 1];
-  uint8_t* dst[kIters];
-  uint8_t* dst_scale[kIters];
+#pragma unroll 1
+  for (int turn = 0; turn < kTurns<kFp8, kIters>; ++turn) {
+    uint4 x[kIters][kFp8 ? 2 : 1];
+    uint8_t* dst[kIters];
+    uint8_t* dst_scale[kIters];
 #pragma unroll
-  for (int i = 0; i < kIters; ++i) {
-    const int r = row_in + i * S::kGroups;
-    dst[i] = nullptr;
-    dst_scale[i] = nullptr;
+    for (int i = 0; i < kIters; ++i) {
+      const int r = row_in + (turn * kIters + i) * S::kGroups;
+      dst[i] = nullptr;
+      dst_scale[i] = nullptr;
 #pragma unroll
-    for (int j = 0; j < (kFp8 ? 2 : 1); ++j) x[i][j] = make_uint4(0, 0, 0, 0);
-    if (r < rows) {
-      const int in = r / per_token, rem = r - in * per_token;
-      const int which = rem >= c.hkv, h = rem - which * c.hkv;
-      if (place[in] >= 0) {
-        const uint4* src = reinterpret_cast<const uint4*>((which ? a.v : a.k) + source[in] + h * a.sh);
+      for (int j = 0; j < (kFp8 ? 2 : 1); ++j) x[i][j] = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const int in = r / per_token, rem = r - in * per_token;
+        const int which = rem >= c.hkv, h = rem - which * c.hkv;
+        if (place[in] >= 0) {
+          const uint4* src = reinterpret_cast<const uint4*>((which ? a.v : a.k) + source[in] + h * a.sh);
 #pragma unroll
-        for (int j = 0; j < (kFp8 ? 2 : 1); ++j) x[i][j] = __ldcs(src + lane * (kFp8 ? 2 : 1) + j);
-        dst[i] = (which ? c.v : c.k) + place[in] + h * c.head_sb + lane * 16;
-        if constexpr (kFp8)
-          dst_scale[i] = (which ? c.v_scale : c.k_scale) + place_scale[in] + (long long)h * c.page_size * kScalesPerRow;
+          for (int j = 0; j < (kFp8 ? 2 : 1); ++j) x[i][j] = __ldcs(src + lane * (kFp8 ? 2 : 1) + j);
+          dst[i] = (which ? c.v : c.k) + place[in] + h * c.head_sb + lane * 16;
+          if constexpr (kFp8)
+            dst_scale[i] = (which ? c.v_scale : c.k_scale) + place_scale[in] + (long long)h * c.page_size * kScalesPerRow;
+        }
       }
     }
-  }
 #pragma unroll
-  for (int i = 0; i < kIters; ++i) {
-    if constexpr (kFp8) {
-      uint32_t byte;
-      const uint4 q = quantise16(x[i], byte);
-      // the row's four bytes to its first lane
-      byte |= __shfl_down_sync(0xffffffffu, byte, 2, 8) << 8;
-      byte |= __shfl_down_sync(0xffffffffu, byte, 4, 8) << 16;
-      if (dst[i] != nullptr) {
-        __stcs(reinterpret_cast<uint4*>(dst[i]), q);
-        if (lane == 0) *reinterpret_cast<uint32_t*>(dst_scale[i]) = byte;
+    for (int i = 0; i < kIters; ++i) {
+      if constexpr (kFp8) {
+        uint32_t byte;
+        const uint4 q = quantise16(x[i], byte);
+        // the row's four bytes to its first lane
+        byte |= __shfl_down_sync(0xffffffffu, byte, 2, 8) << 8;
+        byte |= __shfl_down_sync(0xffffffffu, byte, 4, 8) << 16;
+        if (dst[i] != nullptr) {
+          __stcs(reinterpret_cast<uint4*>(dst[i]), q);
+          if (lane == 0) *reinterpret_cast<uint32_t*>(dst_scale[i]) = byte;
+        }
+      } else {
+        if (dst[i] != nullptr) __stcs(reinterpret_cast<uint4*>(dst[i]), x[i][0]);
       }
-    } else {
-      if (dst[i] != nullptr) __stcs(reinterpret_cast<uint4*>(dst[i]), x[i][0]);
     }
   }
 }
@@ -286,7 +294,8 @@ int launch_kv_cache_write(const mb_paged_kv* kv, const void* k_new, const void* 
   const bool fp8 = kv->dtype == MB_DTYPE_E4M3;
   const int groups = fp8 ? MoveShape<true>::kGroups : MoveShape<false>::kGroups;
   const bool many = rows >= 4ll * groups * sm_count();
-  const long long blocks = (rows + (many ? 4 : 1) * groups - 1) / ((many ? 4 : 1) * groups);
+  const int block = groups * (many ? 4 * (fp8 ? kTurns<true, 4> : kTurns<false, 4>) : 1);
+  const long long blocks = (rows + block - 1) / block;
   if (blocks > 0x7fffffffll) return MB_E_INVALID;
   const auto kernel = fp8 ? (many ? kv_cache_write_kernel<true, 4> : kv_cache_write_kernel<true, 1>)
                           : (many ? kv_cache_write_kernel<false, 4> : kv_cache_write_kernel<false, 1>);
