@@ -144,7 +144,7 @@ int launch_attn_paged(const mb_attn_paged_args* x, void* ws, unsigned long long 
   a.share_tiles = max(p.share_tiles, 1);
 
   uint8_t* at = static_cast<uint8_t*>(ws);
-  if (p.tile_ctas > 0 && e4m3) {  // [keys | values]
+  if (p.tile_ctas > 0 && e4m3 && a.max_keys > 0) {  // [keys | values]
     a.packed_rows = x->max_keys;
     a.packed_k = reinterpret_cast<const __nv_bfloat16*>(at);
     a.packed_v = a.packed_k + (long long)p.group * x->max_keys * a.c.hkv * kHeadDim;
@@ -169,7 +169,7 @@ int launch_attn_paged(const mb_attn_paged_args* x, void* ws, unsigned long long 
   for (int b = 0; p.tile_ctas > 0 && b < a.c.batch; b += p.group) {
     a.b_begin = b;
     a.b_end = min(b + p.group, a.c.batch);
-    if (e4m3) {
+    if (a.packed_k != nullptr) {
       rc = launch_read_e4m3(a, p.few / a.group + 1, stream);
       if (rc != MB_SUCCESS) return rc;
     }

@@ -459,6 +459,25 @@ def test_more_sequences_than_a_grid_dimension_has():
     assert torch.isinf(lse[0::2]).all() and torch.isfinite(lse[1::2]).all()
 
 
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("new", [1, 5, 100])
+def test_bound_of_no_keys(fp8, new):
+    """max_keys=0: rows that see nothing; a sequence that has keys is reported."""
+    from mercury_artifact_b200._lib import MercuryB200Error
+
+    mb = _mb()
+    batch = Batch([0, 0], [new] * 2, (8, 2), 16, fp8, ragged=False, seed=26)
+    tensors = batch.cache_tensors()
+    o, lse = _attend(batch, _cache(batch, tensors), max_keys=0)
+    assert _status() == 0
+    check(batch, o, lse, batch.expected(tensors, True))
+    batch = Batch([0, 9], [new] * 2, (8, 2), 16, fp8, ragged=False, seed=27)
+    cache = _cache(batch, batch.cache_tensors())
+    _attend(batch, cache, max_keys=0)
+    with pytest.raises(MercuryB200Error, match="page number"):
+        cache.check()
+
+
 def test_bound_of_no_new_tokens():
     """max_queries=0: right where no sequence has any, reported where one has more than a token."""
     from mercury_artifact_b200._lib import MercuryB200Error
