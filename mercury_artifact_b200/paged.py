@@ -256,17 +256,20 @@ def attn_fwd_paged(
     if max_queries < 0 or max_keys < 0:
         raise ValueError("max_queries and max_keys must not be negative")
     batch = cache._batch(page_table, seq_lens, cu_seqlens, tokens)
+    checked = False
     if out is None:
         out = torch.empty_like(q)
+        checked = out.stride() == q.stride()
     elif out.shape != shape:
         raise ValueError(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
+    out_rows = (out.data_ptr(), *q_rows[1:]) if checked else _rows(out, "out", cache, dims)
     if lse is None:
         lse = q.new_empty(lse_shape, dtype=torch.float32)
     elif (lse.dtype != torch.float32 or lse.shape != lse_shape or lse.device != cache.device
           or (lse_shape[-1] > 1 and lse.stride(-1) != 1)):
         raise ValueError(f"lse must be fp32 {lse_shape} with contiguous rows on {cache.device}")
     lse_strides = lse.stride()
-    args = _lib.ATTN_PAGED.pack(*batch, *q_rows, *_rows(out, "out", cache, dims), lse.data_ptr(),
+    args = _lib.ATTN_PAGED.pack(*batch, *q_rows, *out_rows, lse.data_ptr(),
                                 lse_strides[0] if dims == 4 else 0, lse_strides[-2], hq, max_queries, max_keys,
                                 1 if causal else 0, softmax_scale)
     with _on(cache.device):
