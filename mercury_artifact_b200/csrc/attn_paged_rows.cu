@@ -15,8 +15,9 @@
 //
 // A CTA takes one K/V head, of e4m3 two neighbours with four warps each where it can, so that 256 bytes lie in a row.
 //
-// e4m3: codes are turned into f16 and multiplied by their powers of two relative to the step's largest (see
-// paged_common.cuh), which is what the instructions of a step go to; P is rounded to f16, scores and sums are fp32.
+// e4m3: codes are turned into f16; values (and keys, with 16 rows) are multiplied by their powers of two relative to the
+// step's largest (see paged_common.cuh), with 8 rows the scores by the keys'.  Half of a step's instructions go there.  P is
+// rounded to f16, scores and sums are fp32.
 //
 // The work of a launch is a list of steps (128 keys of one block of rows in bf16, 256 in e4m3), sequence by
 // sequence, head by head; every CTA takes an equal, contiguous part, so that lengths need not balance.  The lengths are on
@@ -24,7 +25,7 @@
 // several CTAs leaves a partial state in each, and paged_merge_kernel joins them in order: results do not depend on timing.
 //
 // Measured, one token each of 64 sequences, 32 query and 8 K/V heads, pages of 16: bf16, 50 to 8 192 keys, 1.15 GB: 192 us,
-// 6.0 TB/s (a plain copy: 6.5); e4m3, 100 to 16 384 keys, 1.04 GB: 187 us, 5.6 TB/s.  What is left of the difference is the start
+// 6.0 TB/s (a plain copy: 6.5); e4m3, 100 to 16 384 keys, 1.04 GB: 183 us, 5.7 TB/s.  What is left of the difference is the start
 // (lengths, page numbers, first rows: a chain of loads) and the merge, some 4 us each, and unequal ends.
 #include "attn_paged.cuh"
 
@@ -47,7 +48,7 @@ struct RowShape {
 constexpr int kPitch = 132;  // of the merge buffers' rows, in floats: what the lanes of a warp store falls into different banks
 
 struct RowSmem {
-  int total, warp_sum[kRowWarps];
+  int warp_sum[kRowWarps];
   int b, step;                               // where this CTA's part starts: sequence, and step inside it
   float2 ml[kRowWarps][16];                  // of a unit: every warp's maximum and sum,
   float part_l[kRowWarps][16], row_top[32];  // its sum relative to the rows' maxima, these
