@@ -436,7 +436,8 @@ typedef struct mb_paged_kv {
   void* v;
   int64_t stride_page, stride_slot, stride_h; /* elements, shared by k and v; multiples of 16 bytes */
   /* e4m3: [pages, hkv, page_size, head_dim / 32] bytes, contiguous.  Byte x is the power of two
-   * 2^(x - 127) that 32 values along head_dim share (77..191 as written; from 192 on: not a number).  bf16: NULL. */
+   * 2^(x - 127) that 32 values along head_dim share (77..191 as written; from 192 on: not a number,
+   * as the codes 0x7f and 0xff).  bf16: NULL. */
   uint8_t* k_scale;
   uint8_t* v_scale;
   const int32_t* page_table; /* [batch, max_pages] */

@@ -256,14 +256,13 @@ __global__ void __launch_bounds__(kMoveThreads) kv_cache_read_kernel(const __gri
     uint4* dst = reinterpret_cast<uint4*>((which ? a.v : a.k) + blockIdx.y * a.sb + (p0 + t) * a.st + h * a.sh) + lane * (kFp8 ? 2 : 1);
     if constexpr (kFp8) {
       const uint32_t byte = __ldg((which ? c.v_scale : c.k_scale) + place_scale[t] + (long long)h * c.page_size * kScalesPerRow + lane / 2);
-      // code * 2^-120 from the bits, then two exact factors: 2^120 and the block's own
       const uint32_t own = byte > (uint32_t)kMaxScale ? 0x7fc07fc0u : byte == 0 ? 0x00400040u : (byte << 7) * 0x10001u;
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
       uint32_t y[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        y[2 * i] = mul_bf16x2(mul_bf16x2(e4m3_bits(__byte_perm(w[i], 0, 0x1404)), 0x7b807b80u), own);
-        y[2 * i + 1] = mul_bf16x2(mul_bf16x2(e4m3_bits(__byte_perm(w[i], 0, 0x3424)), 0x7b807b80u), own);
+        y[2 * i] = mul_bf16x2(f16_bf16(e4m3_f16(w[i])), own);
+        y[2 * i + 1] = mul_bf16x2(f16_bf16(e4m3_f16_high(w[i])), own);
       }
       dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
       dst[1] = make_uint4(y[4], y[5], y[6], y[7]);

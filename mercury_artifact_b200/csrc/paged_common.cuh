@@ -85,20 +85,23 @@ __device__ __forceinline__ long long scale_offset(const PagedView& c, int id, in
   return (((long long)id * c.hkv + h) * c.page_size + slot) * kScalesPerRow;
 }
 
-// ---- e4m3 codes as bf16 and f16 ------------------------------------------------------------
-// The bits of a code, put into the fraction and the low exponent bits of a bf16, stand for its value times 2^-120
-// (exponent biases 7 and 127; subnormal codes become subnormal bf16), so that one exact product gives code * 2^n.
-// x holds the codes in the high byte of each half.
-__device__ __forceinline__ uint32_t e4m3_bits(uint32_t x) { return (x & 0x80008000u) | ((x >> 4) & 0x07f007f0u); }
+// ---- e4m3 codes as f16 and bf16 ------------------------------------------------------------
+// Both hold every code as it is, and a code times a power of two is exact in bf16.
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// The attention kernels multiply in f16, which holds a code as it is: code * 2^(n - N) with N the largest exponent of the
+__device__ __forceinline__ uint32_t f16_bf16(uint32_t two) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\t.reg .f32 x, y;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.f32.f16 x, lo;\n\tcvt.f32.f16 y, hi;\n\t"
+      "cvt.rn.bf16x2.f32 %0, y, x;\n\t}" : "=r"(r) : "r"(two));
+  return r;
+}
+// The kernel for few rows multiplies in f16: code * 2^(n - N) with N the largest exponent of the
 // keys (or values) that one product takes, in units of 2^N.  That is exact down to n = N - 15 (f16 ends at 2^-24, a code at
 // 2^-9), off by less than bf16 would be down to N - 23, by less than e4m3's own rounding down to N - 27, and zero below N - 34.
-// (One conversion for two codes and one product, where the way through the bits above takes four integer instructions at
+// (One conversion for two codes and one product; putting a code's bits into a bf16 instead takes four integer instructions at
 // half rate: 64 tokens against up to 16 384 keys of 8 heads took 302 us with those and 238 without, all else alike.)
 __device__ __forceinline__ uint32_t e4m3_f16(uint32_t two) {  // the two low bytes
   uint32_t r;

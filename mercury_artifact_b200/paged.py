@@ -38,9 +38,8 @@ class PagedKV:
     transposed) as long as head_dim is contiguous, k and v share their strides, and these are multiples of 16 bytes.
     bfloat16, or float8_e4m3fn with k_scale, v_scale: contiguous uint8 [pages, heads, page_size, 4].  Byte x is the power
     of two 2^(x - 127) that 32 values share: a code times its power of two is exact in bfloat16.  A write chooses 77 .. 191;
-    bytes from 192 on make their values NaN.  No write makes e4m3's
-    NaN codes (0x7f, 0xff), and what the calls make of them is not defined.  The calls go to the memory that these
-    tensors have when the cache is made.
+    bytes from 192 on make their values NaN, and so do e4m3's NaN codes (0x7f, 0xff), which no write makes.  The calls go to
+    the memory that these tensors have when the cache is made.
     """
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,

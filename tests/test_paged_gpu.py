@@ -617,6 +617,33 @@ def test_blocks_that_are_not_numbers(new):
         check(second, o[1:], lse[1:], second.expected(tensors, True))
 
 
+@pytest.mark.parametrize("new", [1, 8, 60])
+def test_codes_that_are_not_numbers(new):
+    """A NaN code in a cache that something else has written: NaN wherever it is read, by every kernel, and nowhere else."""
+    for which in (0, 1):
+        batch = Batch([200, 90], [new, new], (4, 2), 16, True, ragged=False, seed=28)
+        tensors = batch.cache_tensors()
+        want = batch.expected(tensors, True)
+        cache = _cache(batch, tensors)
+        page, slot = batch.table[0, 100 // 16].item(), 100 % 16
+        (cache.v if which else cache.k).view(torch.uint8)[page, slot, 0, 40] = 0xff if which else 0x7f
+        kv = _mb().kv_cache_read(cache, batch.on(batch.table), batch.on(batch.seq_lens), max_keys=200)
+        assert torch.isnan(kv).sum().item() == 1 and torch.isnan(kv[which, 0, 100, 0, 40])
+        o, lse = _attend(batch, cache)
+        assert _status() == 0
+        first = o[0, :, :2].float()  # the query heads of K/V head 0; every new token sees key 100
+        if which:
+            assert torch.isnan(first[..., 40]).all() and torch.isnan(o).sum().item() == 2 * new
+            assert not torch.isnan(lse).any()
+        else:
+            assert torch.isnan(first).all() and torch.isnan(o).sum().item() == 2 * new * D and torch.isnan(lse).sum().item() == 2 * new
+        nan = torch.isnan(o).view(-1, 4, D).cpu()
+        clean = torch.where(nan, want[0].to(torch.bfloat16), o.view(-1, 4, D).cpu())
+        none = torch.isnan(lse).cpu()
+        clean_lse = torch.where(none, want[1].view(4, 2, new).permute(1, 0, 2).float(), lse.cpu())
+        check(batch, clean, clean_lse, want)
+
+
 # -- together ----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("fp8", FP8)
 def test_serving_run(fp8):
