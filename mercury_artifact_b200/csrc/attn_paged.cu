@@ -93,7 +93,7 @@ static int plan_paged(const mb_attn_paged_args* x, PagedPlan* p) {
   return MB_SUCCESS;
 }
 
-// The two kernels run side by side: [bf16 copy | shares of the tiles | parts of the rows]
+// [bf16 copy | shares of the tiles | parts of the rows]
 static long long workspace_of(const PagedPlan& p) { return p.packed_bytes + p.split_bytes + p.rows_bytes; }
 
 long long attn_paged_workspace(const mb_attn_paged_args* x) {
@@ -164,8 +164,6 @@ int launch_attn_paged(const mb_attn_paged_args* x, void* ws, unsigned long long 
     a.open = reinterpret_cast<int4*>(a.part_ml + slots);
   }
 
-  // Beside chunks, which are bound by the tensor cores and leave SMs idle at their end, single tokens cost little: 16
-  // sequences, 5 of them chunks, up to 8 192 e4m3 keys, 32/8 heads: 175 us one after the other, 170 side by side.
   for (int b = 0; p.tile_ctas > 0 && b < a.c.batch; b += p.group) {
     a.b_begin = b;
     a.b_end = min(b + p.group, a.c.batch);
@@ -175,17 +173,12 @@ int launch_attn_paged(const mb_attn_paged_args* x, void* ws, unsigned long long 
     }
     rc = launch_paged_tiles(a, p.tile_ctas, stream);
     if (rc != MB_SUCCESS) return rc;
-    if (a.b_end == a.c.batch && p.row_ctas > 0) {
-      a.beside = 1;
-      rc = launch_paged_rows(a, e4m3, p.rows, p.row_heads, p.row_ctas, stream);
-      if (rc != MB_SUCCESS) return rc;
-    }
     if (p.split) {
       rc = launch_paged_tiles_merge(a, p.tile_ctas, stream);
       if (rc != MB_SUCCESS) return rc;
     }
   }
-  if (p.row_ctas > 0 && !a.beside) {
+  if (p.row_ctas > 0) {
     rc = launch_paged_rows(a, e4m3, p.rows, p.row_heads, p.row_ctas, stream);
     if (rc != MB_SUCCESS) return rc;
   }

@@ -24,9 +24,6 @@ struct PagedAttnArgs {
   float2* part_ml;
   int4* open;
   int whole;  // few rows: CTA i has unit i, and nothing is joined
-  // The kernel for few rows comes right behind one for tiles and runs beside it: it starts as soon as all of that one's CTAs
-  // have (these wait for what came before them first), and does not end before it.
-  int beside;
   // tiles: keys (in tiles of 128) of a share of a unit; partial results [CTA][32 column groups][256 rows], (maximum, sum)
   // [CTA][256]; tile_open: the split unit whose first share a CTA has (sequence, K/V head, row block, shares; 0: none).
   // All null where no unit is split.

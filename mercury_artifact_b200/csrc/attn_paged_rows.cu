@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   const uint32_t stage0 = smem_u32(stages);
 
   grid_dependents_launch();
-  if (!a.beside) grid_dependency_wait();
+  grid_dependency_wait();
 
   // This CTA's part of the list.  A thread looks at every 256th sequence; up to 256 of them are looked at once.
   RowIter in;  // what is loaded next
@@ -233,10 +233,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       if (lane == 0) a.lse[b * a.lse_sb + hd * a.lse_sh + tok] = -INFINITY;
     }
   }
-  if (total == 0) {
-    if (a.beside) grid_dependency_wait();
-    return;
-  }
+  if (total == 0) return;
   if (!a.whole) {
     in.b = sm->b;
     in.s = paged_seq(a.c, in.b, a.max_queries, a.max_keys);
@@ -679,7 +676,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     }
     at = nx;
   }
-  if (a.beside) grid_dependency_wait();
 }
 
 // Joins the partial states of the unit that CTA blockIdx.x of the launch before began and did not finish (if there is one):

@@ -33,9 +33,8 @@
 //
 // Bound by the tensor cores and, as in attn_fwd, by the exponentials beside them: a step of 128 keys takes an SM some 1.9 us.
 // Unequal sequences cost more than that: 16 e4m3 sequences, 5 of them chunks of up to 512 tokens, up to 8 192 keys, take
-// 170 us, of which the longest unit's 64 steps are 124.  Choosing the shares on the device by the lengths that are there was
-// built: 187 us, as smaller shares only bring the tiles to 105-110 us and cost a launch and the SMs on which the single
-// tokens run meanwhile.
+// 172 us, of which the longest unit's 64 steps are 118.  Choosing the shares on the device by the lengths that are there was
+// built: 187 us where this took 170, as smaller shares only bring the tiles to 105-110 us and cost a launch.
 #include "attn_paged.cuh"
 #include "attn_fwd_common.cuh"
 
