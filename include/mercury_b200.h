@@ -472,7 +472,7 @@ typedef struct mb_attn_paged_args {
   float* lse; /* written: cu_seqlens: [hq, tokens]; else [batch, hq, tokens / batch] */
   int64_t lse_stride_b, lse_stride_h;
   int32_t hq;
-  int32_t max_queries; /* no sequence has more new tokens */
+  int32_t max_queries; /* no sequence has more new tokens (a bound by which the launch is cut where cu_seqlens is given) */
   int32_t max_keys;    /* no sequence has more keys */
   int32_t causal;      /* new token i of n sees keys j <= seq_lens - n + i; else all keys */
   float softmax_scale; /* > 0 */

@@ -35,14 +35,16 @@ static int plan_paged(const mb_attn_paged_args* x, PagedPlan* p) {
   if (x->hq <= 0 || kv.hkv <= 0 || x->hq % kv.hkv != 0) return MB_E_INVALID;
   if (x->max_queries < 0 || x->max_keys < 0 || !(x->softmax_scale > 0.f) || x->softmax_scale > 2e38f /* (times log2(e)) */) return MB_E_INVALID;
   if (kv.batch < 0 || kv.tokens < 0 || kv.page_size <= 0 || kv.max_pages < 0) return MB_E_INVALID;
-  const long long heads = x->hq / kv.hkv, rows = x->max_queries * heads;
+  // The kernels divide the work by the rows that a sequence has.  In a padded batch these are known, whatever the bound.
+  const bool padded = kv.cu_seqlens == nullptr, e4m3 = kv.dtype == MB_DTYPE_E4M3;
+  const int queries = padded && kv.batch > 0 ? kv.tokens / kv.batch : x->max_queries;
+  const long long heads = x->hq / kv.hkv, rows = queries * heads;
   if (rows > 0x7fffff00ll) return MB_E_UNSUPPORTED;
   // steps of a launch are counted in 32 bits
   if ((double)kv.batch * kv.hkv * ((double)x->max_keys / 128 + 1) > 2e9) return MB_E_UNSUPPORTED;
   const int sms = sm_count();
   if (sms <= 0) return MB_E_CUDA;
   memset(p, 0, sizeof(*p));
-  const bool padded = kv.cu_seqlens == nullptr, e4m3 = kv.dtype == MB_DTYPE_E4M3;
   // Beside chunks the sequences with few rows are single tokens as a rule, which the kernels for fewer rows take faster.
   p->few = rows > kFewRows && heads <= 8 ? 8 : kFewRows;
   if (e4m3 && rows <= kFewRowsE4m3) p->few = kFewRowsE4m3;

@@ -1,0 +1,52 @@
+"""The paged calls through the C ABI, where a caller chooses bounds and workspace itself."""
+import pytest
+import torch
+
+from tests.paged_cases import D, SCALE, Batch, check
+
+pytestmark = pytest.mark.gpu
+
+FP8 = [False, True]
+
+
+def attend(batch, cache, max_queries, max_keys=None, causal=True, table=None, fill=None):
+    """o, lse of mb_attn_paged in buffers that held 7; the workspace holds bytes of `fill`."""
+    from mercury_artifact_b200 import _lib
+
+    ragged = batch.ragged
+    q = batch.on(batch.shaped(batch.q))
+    b, n = len(batch.lens), batch.new[0]
+    cu = batch.on(batch.cu) if ragged else None
+    table = batch.on(batch.table) if table is None else table
+    lens = batch.on(batch.seq_lens)
+    o = torch.full_like(q, 7.0)
+    lse = torch.full((batch.hq, batch.tokens) if ragged else (b, batch.hq, n), 7.0, device="cuda")
+    rows = (0, batch.hq * D, D) if ragged else (n * batch.hq * D, batch.hq * D, D)
+    args = _lib.ATTN_PAGED.pack(
+        *cache._batch(table, lens, cu, batch.tokens), q.data_ptr(), *rows, o.data_ptr(), *rows, lse.data_ptr(),
+        0 if ragged else batch.hq * n, batch.tokens if ragged else n, batch.hq, max_queries,
+        table.shape[1] * batch.page_size if max_keys is None else max_keys, int(causal), SCALE)
+    need = _lib.lib.mb_attn_paged_workspace(args)
+    ws = torch.full((max(need, 1),), 0 if fill is None else fill, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.check(_lib.lib.mb_attn_paged(args, ws.data_ptr() if need else None, need, stream), "mb_attn_paged")
+    return o, lse
+
+
+def make(batch):
+    import mercury_artifact_b200 as mb
+
+    tensors = batch.cache_tensors()
+    return tensors, mb.PagedKV(*(batch.on(t) for t in tensors))
+
+
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("heads", [(8, 2), (8, 8), (32, 1)])
+@pytest.mark.parametrize("n,bound", [(1, 1), (1, 2), (1, 64), (2, 5), (3, 300), (5, 2 ** 30), (40, 41), (40, 1000)])
+def test_bound_above_the_new_tokens_of_a_padded_batch(fp8, heads, n, bound):
+    """max_queries is an upper bound: every row is written, whichever kernel the bound alone would have chosen."""
+    batch = Batch([700, 1, 130, 0, 2 * n], [n] * 5, heads, 16, fp8, ragged=False, seed=41)
+    tensors, cache = make(batch)
+    o, lse = attend(batch, cache, bound)
+    cache.check()
+    check(batch, o, lse, batch.expected(tensors, True))
