@@ -37,7 +37,8 @@ static int plan_paged(const mb_attn_paged_args* x, PagedPlan* p) {
   if (kv.batch < 0 || kv.tokens < 0 || kv.page_size <= 0 || kv.max_pages < 0) return MB_E_INVALID;
   // The kernels divide the work by the rows that a sequence has.  In a padded batch these are known, whatever the bound.
   const bool padded = kv.cu_seqlens == nullptr, e4m3 = kv.dtype == MB_DTYPE_E4M3;
-  const int queries = padded && kv.batch > 0 ? kv.tokens / kv.batch : x->max_queries;
+  // (a ragged batch with a bound of no new tokens is launched all the same: the kernel reports the sequences that have some)
+  const int queries = padded && kv.batch > 0 ? kv.tokens / kv.batch : max(x->max_queries, 1);
   const long long heads = x->hq / kv.hkv, rows = queries * heads;
   if (rows > 0x7fffff00ll) return MB_E_UNSUPPORTED;
   // steps of a launch are counted in 32 bits
@@ -115,7 +116,7 @@ int launch_attn_paged(const mb_attn_paged_args* x, void* ws, unsigned long long 
   if (rc != MB_SUCCESS) return rc;
   if (x->max_keys > (long long)x->kv.max_pages * x->kv.page_size) return MB_E_INVALID;
   if (a.c.cu == nullptr && a.c.per_seq > x->max_queries) return MB_E_INVALID;
-  if (a.c.batch == 0 || a.c.tokens == 0 || x->max_queries == 0) return MB_SUCCESS;
+  if (a.c.batch == 0 || a.c.tokens == 0) return MB_SUCCESS;
   if (x->q == nullptr || x->o == nullptr || x->lse == nullptr) return MB_E_INVALID;
   const uintptr_t al = reinterpret_cast<uintptr_t>(x->q) | reinterpret_cast<uintptr_t>(x->o) | (uintptr_t)(x->q_stride_b * 2) |
                        (uintptr_t)(x->q_stride_t * 2) | (uintptr_t)(x->q_stride_h * 2) | (uintptr_t)(x->o_stride_b * 2) |

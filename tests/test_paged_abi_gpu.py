@@ -50,3 +50,22 @@ def test_bound_above_the_new_tokens_of_a_padded_batch(fp8, heads, n, bound):
     o, lse = attend(batch, cache, bound)
     cache.check()
     check(batch, o, lse, batch.expected(tensors, True))
+
+
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("new,known", [([0, 0], True), ([1, 0], False), ([0, 40], False)])
+def test_bound_of_no_new_tokens(fp8, new, known):
+    """max_queries = 0 of a ragged batch: nothing to write, or a report."""
+    from mercury_artifact_b200._lib import MercuryB200Error
+
+    batch = Batch([100, 50], new, (8, 2), 16, fp8, seed=42)
+    _, cache = make(batch)
+    if known:  # rows behind the last sequence
+        batch.q, batch.tokens = torch.zeros(3, 8, D, dtype=torch.bfloat16), 3
+    o, lse = attend(batch, cache, 0)
+    if known:
+        cache.check()
+    else:
+        with pytest.raises(MercuryB200Error, match="page number"):
+            cache.check()
+    assert (o == 7).all() and (lse == 7).all()
