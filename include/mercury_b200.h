@@ -428,7 +428,8 @@ MB_API int mb_version(void);
  * Lengths, offsets and page numbers are read on the device (a captured graph may be
  * replayed with others).  One that lies outside the table, the pages or the
  * rows does not leave them: it is clamped or skipped and reported as status 110,
- * and the results of that call are invalid. */
+ * and the results of that call are invalid.  A write under offsets that do not ascend
+ * within [0, tokens] stores nothing. */
 #define MB_DTYPE_E4M3 2
 
 typedef struct mb_paged_kv {

@@ -155,7 +155,7 @@ def kv_cache_write(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table:
 
     k, v: bfloat16 [batch, n, heads, 128], or [tokens, heads, 128] with cu_seqlens.  The new tokens are the
     last ones of the seq_lens[b] keys; where a sequence has more of them than keys, the first ones are not stored.  No
-    two new tokens may lie in the same slot."""
+    two new tokens may lie in the same slot.  Nothing is stored under offsets that do not ascend within [0, tokens]."""
     dims = 3 if cu_seqlens is not None else 4
     shape = k.shape
     k_ptr, *strides = _rows(k, "k", cache, dims)
