@@ -76,6 +76,7 @@ struct CacheMoveArgs {
   int rows;              // read: rows per sequence
   int first_seq;         // read: sequences from this one on, the first one's rows at k, v
   int min_new, max_new;  // read: those with at least min_new new tokens only
+  bool zeros;            // read: rows of bad pages become zeros, which the attention takes there (else they are left alone)
 };
 
 constexpr int kMoveThreads = 256;
@@ -247,7 +248,13 @@ __global__ void __launch_bounds__(kMoveThreads) kv_cache_read_kernel(const __gri
     const int pos = p0 + threadIdx.x, p = page_index(c, pos), slot = pos - p * c.page_size;
     const int id = c.table[b * c.table_stride + p];
     const bool bad = id < 0 || id >= c.pages;
-    if (bad) paged_error(c);
+    if (bad) {
+      paged_error(c);
+      for (int i = 0; a.zeros && i < 2 * c.hkv * (kHeadDim / 8); ++i) {  // (here, where it costs the loop below nothing)
+        const int row = i / (kHeadDim / 8), h = row >> 1;
+        reinterpret_cast<uint4*>((row & 1 ? a.v : a.k) + blockIdx.y * a.sb + pos * a.st + h * a.sh)[i % (kHeadDim / 8)] = make_uint4(0, 0, 0, 0);
+      }
+    }
     place[threadIdx.x] = bad ? -1 : paged_offset(c, id, slot, 0);
     if constexpr (kFp8) place_scale[threadIdx.x] = bad ? 0 : scale_offset(c, id, slot, 0);
   }
@@ -296,6 +303,7 @@ int launch_kv_cache_write(const mb_paged_kv* kv, const void* k_new, const void* 
   a.v = static_cast<uint8_t*>(const_cast<void*>(v_new));
   a.sb = sb * 2; a.st = st * 2; a.sh = sh * 2;
   a.rows = a.first_seq = a.min_new = a.max_new = 0;
+  a.zeros = false;
   const long long rows = (long long)a.c.tokens * 2 * a.c.hkv;
   const bool fp8 = kv->dtype == MB_DTYPE_E4M3;
   const int groups = fp8 ? MoveShape<true>::kGroups : MoveShape<false>::kGroups;
@@ -334,6 +342,7 @@ int launch_read_e4m3(const PagedAttnArgs& x, int min_new, cudaStream_t stream) {
   a.first_seq = x.b_begin;
   a.min_new = min_new;
   a.max_new = x.max_queries;
+  a.zeros = true;
   return launch_read(a, true, x.b_end - x.b_begin, stream);
 }
 
@@ -350,6 +359,7 @@ int launch_kv_cache_read(const mb_paged_kv* kv, void* k_out, void* v_out, long l
   a.sb = sb * 2; a.st = ss * 2; a.sh = sh * 2;
   a.rows = rows;
   a.first_seq = a.min_new = a.max_new = 0;
+  a.zeros = false;
   a.c.cu = nullptr;
   return launch_read(a, kv->dtype == MB_DTYPE_E4M3, a.c.batch, stream);
 }

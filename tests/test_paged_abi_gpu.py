@@ -69,3 +69,30 @@ def test_bound_of_no_new_tokens(fp8, new, known):
         with pytest.raises(MercuryB200Error, match="page number"):
             cache.check()
     assert (o == 7).all() and (lse == 7).all()
+
+
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("page", [16, 24, 7])
+@pytest.mark.parametrize("new", [1, 5, 40, 100])
+def test_keys_of_a_bad_page_are_zeros(fp8, page, new):
+    """Every path puts zeros where a page number is bad, whatever the workspace held: results are finite and repeat."""
+    from mercury_artifact_b200._lib import MercuryB200Error
+
+    batch = Batch([130, 260, 100], [new] * 3, (8, 2), page, fp8, ragged=False, seed=43)
+    tensors, cache = make(batch)
+    good = batch.table.clone()
+    used = {int(x) for i, n in enumerate(batch.lens) for x in good[i, :-(-n // page)]}
+    zeros = next(p for p in range(batch.pages) if p not in used)
+    for t, value in zip(tensors, (0, 0, 127, 127)):
+        if t is not None:
+            t[zeros].view(torch.uint8).fill_(value)
+    batch.table[1, 2] = zeros
+    want = batch.expected(tensors, True)
+    bad = good.clone()
+    bad[1, 2] = batch.pages + 3
+    results = [attend(batch, cache, new, table=bad.cuda(), fill=fill) for fill in (0, 0xff, 0x7f)]
+    with pytest.raises(MercuryB200Error, match="page number"):
+        cache.check()
+    for o, lse in results:
+        check(batch, o, lse, want)
+        assert torch.equal(o, results[0][0]) and torch.equal(lse, results[0][1])
