@@ -96,3 +96,23 @@ def test_keys_of_a_bad_page_are_zeros(fp8, page, new):
     for o, lse in results:
         check(batch, o, lse, want)
         assert torch.equal(o, results[0][0]) and torch.equal(lse, results[0][1])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,new,covered", [([300, 700, 64, 129, 1000], [40, 100, 64, 33, 257], 131072),  # two sequences a group
+                                              ([300, 0, 700, 500, 64, 200, 90], [40, 0, 1, 3, 64, 0, 90], 131072),  # single tokens too
+                                              ([700, 40, 1300], [90, 40, 100], 300000)])  # one sequence a group
+def test_chunks_of_a_quantised_cache_in_groups(causal, lens, new, covered):
+    """A bound on the keys so high that the bf16 copy of all sequences would not fit: group by group, in the same memory.
+    The copy starts as NaN."""
+    batch = Batch(lens, new, (16, 8), 16, True, seed=44)
+    tensors, cache = make(batch)
+    want = batch.expected(tensors, causal)
+    table = torch.full((len(lens), covered // 16), 2 ** 30, dtype=torch.int32, device="cuda")
+    table[:, :batch.table.shape[1]] = batch.on(batch.table)
+    assert len(lens) * covered * 8 * 512 > 1 << 30
+    results = [attend(batch, cache, max(new), causal=causal, table=table, fill=0xff) for _ in range(2)]
+    cache.check()
+    for o, lse in results:
+        check(batch, o, lse, want)
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
