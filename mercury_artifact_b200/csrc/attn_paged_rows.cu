@@ -15,9 +15,9 @@
 //
 // A CTA takes one K/V head, of e4m3 two neighbours with four warps each where it can, so that 256 bytes lie in a row.
 //
-// e4m3: codes are turned into f16; values (and keys, with 16 rows) are multiplied by their powers of two relative to the
-// step's largest (see paged_common.cuh), with 8 rows the scores by the keys'.  Half of a step's instructions go there.  P is
-// rounded to f16, scores and sums are fp32.
+// e4m3: codes are turned into f16; values are multiplied by their powers of two there while these lie close together, else in
+// bf16 (see paged_common.cuh).  Keys are multiplied by theirs relative to the step's largest (16 rows), or the scores by the
+// keys' (8 rows).  Half of a step's instructions go there.  P is rounded with the values, scores and sums are fp32.
 //
 // The work of a launch is a list of steps (128 keys of one block of rows in bf16, 256 in e4m3), sequence by
 // sequence, head by head; every CTA takes an equal, contiguous part, so that lengths need not balance.  The lengths are on
@@ -46,6 +46,9 @@ struct RowShape {
   static_assert(kStage % 256 == 0, "rows are aligned to their size");
 };
 constexpr int kPitch = 132;  // of the merge buffers' rows, in floats: what the lanes of a warp store falls into different banks
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 
 struct RowSmem {
   int warp_sum[kRowWarps];
@@ -346,6 +349,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     int limit[kTiles][2];        // keys that the row sees; the first of the unit's rows sees the fewest
     float row_scale[kTiles][2];  // e4m3: power of two of the row's queries
     uint32_t qk[kTiles][4][4];
+    int unit = 0;       // e4m3: acc is in units of 2^(unit - 127) (see paged_common.cuh; 0: no step yet),
+    bool wide = false;  // and values go by way of bf16
     const int row0 = at.block * kRows, rows = min(at.s.n * a.group - row0, kRows);
     const int seen_by_all = a.causal ? at.s.len - at.s.n + row0 / a.group + 1 : at.s.len;
 #pragma unroll
@@ -391,7 +396,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[m][j][e] = 0.f;
       float step_scale = a.scale_log2;  // of the step's scores; e4m3: with the keys' power of two
-      int value_exp = 0;                // exponent of the power of two that the values were divided by
       if constexpr (!kFp8) {
         // four 8 x 8 matrices: keys 0-7 and 8-15 of one 16-byte piece, then of the next
         const uint32_t k_addr = sk + (lane & 15) * S::kRowBytes + (((lane >> 4) ^ (lane & 7)) << 4);
@@ -408,26 +412,51 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
           }
         }
       } else {
-        // The powers of two of this lane's key.  The values' are taken relative to the largest of the step, so that f16 holds the
-        // products; the keys' too, or with 8 rows the scores of 32 columns at a time are multiplied by them (kScaled: half as
+        // The powers of two of this lane's key.  The keys' are taken relative to the largest of the step, so that f16 holds the
+        // products, or with 8 rows the scores of 32 columns at a time are multiplied by them (kScaled: half as
         // many products, and no rounding; 64 single tokens up to 16 384 keys 186 us and 182, 8 tokens each up to 8 192, 16 rows,
         // 333 and 347).
         const uint32_t* words = reinterpret_cast<const uint32_t*>(stages + stage * S::kStage + 2 * S::kHalf);
-        const uint32_t kw = words[lane], vw = words[kKeys + lane];
+        const uint32_t kw = words[lane];
+        // (behind the sequence's end: of no effect on the unit, and a number)
+        uint32_t vw = key0 + lane < at.s.len ? words[kKeys + lane] : unit * 0x01010101u;
+        if (__any_sync(0xffffffffu, unit == 0 || values_outside(vw, unit))) {
+          const int top = max((int)__reduce_max_sync(0xffffffffu, scale_top(vw)), kLeastUnit);
+          wide = unit > 0;
+          if (top > unit + kAboveUnit) {
+            const float f = unit - top < -126 ? 0.f : exp2_int(unit - top);
+#pragma unroll
+            for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[m][j][e] *= f;
+            unit = top;
+          }
+          if (key0 + lane >= at.s.len) vw = unit * 0x01010101u;
+          if (!wide) wide = __any_sync(0xffffffffu, values_outside(vw, unit));
+        }
         int k_top = 127;
         if constexpr (!kScaled) k_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(kw)), kMinScale);
-        const int v_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(vw)), kMinScale);
         uint32_t ks[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const float k2 = scale_relative((kw >> (8 * b)) & 0xffu, k_top);
           ks[b] = kScaled ? __float_as_uint(k2) : pack_f16x2(k2, k2);
-          value_scale[b * kKeys + lane] = (uint16_t)pack_f16x2(scale_relative((vw >> (8 * b)) & 0xffu, v_top), 0.f);
+        }
+        if (!wide) {
+          const uint2 x = unit_f16(vw, unit);
+          value_scale[lane] = (uint16_t)x.x;
+          value_scale[kKeys + lane] = (uint16_t)x.y;
+          value_scale[2 * kKeys + lane] = (uint16_t)(x.x >> 16);
+          value_scale[3 * kKeys + lane] = (uint16_t)(x.y >> 16);
+        } else {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) value_scale[b * kKeys + lane] = (uint16_t)unit_bf16((vw >> (8 * b)) & 0xffu, unit);
         }
         *reinterpret_cast<uint4*>(key_scale + lane * 4) = make_uint4(ks[0], ks[1], ks[2], ks[3]);
         __syncwarp();
         step_scale = a.scale_log2 * exp2_int(k_top - 127);
-        value_exp = v_top - 127;
         // four matrices: the 32 keys x one piece of 16 values, which makes two operands of 16 keys x 16 values
         const uint32_t k_addr = sk + lane * S::kRowBytes + ((lane & 7) << 4);
 #pragma unroll
@@ -482,8 +511,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
             for (int e = 0; e < 4; ++e)
               if (key0 + j * 16 + (e >> 1) * 8 + g >= limit[m][e & 1]) sc[m][j][e] = -INFINITY;
       }
-      // A row's reference is the exponent of its largest term exp2(score) * 2^value_exp; it only moves when a term exceeds
-      // it by 2^8.  Each lane looks at its own keys, and the row's maximum is only taken when one of them does.
+      // A row's reference only moves when a score exceeds it by kAhead.  Each lane looks at its own keys, and the row's maximum is
+      // only taken when one of them does.
+      constexpr float kAhead = kFp8 ? kAheadF16 : 8.f;
       float c[kTiles][2], top[kTiles][2];
       bool need = false;
 #pragma unroll
@@ -494,8 +524,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
           if constexpr (kGroups == 2) x = max3(x, sc[m][kGroups - 1][e], sc[m][kGroups - 1][2 + e]);
           // (not zero, with which hidden scores would make no number)
           c[m][e] = kFp8 ? fmaxf(step_scale * row_scale[m][e], 1.2e-38f) : step_scale;
-          top[m][e] = x == -INFINITY ? -INFINITY : fmaf(x, c[m][e], (float)value_exp);
-          need |= top[m][e] - m_ref[m][e] > 8.f;
+          top[m][e] = x == -INFINITY ? -INFINITY : x * c[m][e];
+          need |= top[m][e] - m_ref[m][e] > kAhead;
         }
       if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
@@ -505,7 +535,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
             float x = top[m][e];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-            const bool moves = x - m_ref[m][e] > 8.f;
+            const bool moves = x - m_ref[m][e] > kAhead;
             const float f = moves ? fast_exp2(m_ref[m][e] - x) : 1.f;
             if (moves) m_ref[m][e] = x;
             l[m][e] *= f;
@@ -521,7 +551,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       for (int m = 0; m < kTiles; ++m) {
         float lift[2], sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) lift[e] = (float)value_exp - (m_ref[m][e] == -INFINITY ? 0.f : m_ref[m][e]);
+        for (int e = 0; e < 2; ++e) lift[e] = (kFp8 ? kLiftF16 : 0.f) - (m_ref[m][e] == -INFINITY ? 0.f : m_ref[m][e]);
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)
 #pragma unroll
@@ -530,10 +560,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
             const float p1 = fast_exp2(fmaf(sc[m][j][2 * i + 1], c[m][1], lift[1]));
             sum[0] += p0;
             sum[1] += p1;
-            pf[m][j][i] = transpose8x8(kFp8 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1));
+            uint32_t both;
+            if (kFp8 && !wide) both = pack_f16x2(p0, p1);
+            else both = pack_bf16x2(p0, p1);
+            pf[m][j][i] = transpose8x8(both);
           }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) l[m][e] = kFp8 ? fmaf(sum[e], exp2_int(-value_exp), l[m][e]) : l[m][e] + sum[e];
+        for (int e = 0; e < 2; ++e) l[m][e] += sum[e];
       }
 
       // ---- values, transposed, as the first operand: 16 columns x 16 keys
@@ -551,29 +584,35 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         // Transposed 16-bit units are pairs of neighbouring values: a lane gets values (2 g, 2 g + 1) of keys (2 t, 2 t + 1) of
         // each 8; the even ones are the product's rows 0-7, the odd ones rows 8-15.
         const uint32_t v_addr = sv + lane * S::kRowBytes + ((lane & 7) << 4);
+        auto add_values = [&](auto f16) {
+          constexpr bool kF16 = decltype(f16)::value;
 #pragma unroll
-        for (int j2 = 0; j2 < 4; ++j2) {
-          uint32_t mult[4];
+          for (int j2 = 0; j2 < 4; ++j2) {
+            uint32_t mult[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mult[i] = *reinterpret_cast<const uint32_t*>(value_scale + j2 * kKeys + i * 8 + 2 * t);
+            for (int i = 0; i < 4; ++i) mult[i] = *reinterpret_cast<const uint32_t*>(value_scale + j2 * kKeys + i * 8 + 2 * t);
 #pragma unroll
-          for (int j = 2 * j2; j < 2 * j2 + 2; ++j) {
-            uint32_t b[4];
-            ldsm4_t(b, v_addr ^ (j << 4));
-            uint32_t v[2][4];
+            for (int j = 2 * j2; j < 2 * j2 + 2; ++j) {
+              uint32_t b[4];
+              ldsm4_t(b, v_addr ^ (j << 4));
+              uint32_t v[2][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t x = __byte_perm(b[i], 0, 0x3120);  // the even ones of both keys, then the odd ones
-              v[i >> 1][(i & 1) * 2] = mul_f16x2(e4m3_f16(x), mult[i]);
-              v[i >> 1][(i & 1) * 2 + 1] = mul_f16x2(e4m3_f16_high(x), mult[i]);
-            }
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t x = __byte_perm(b[i], 0, 0x3120);  // the even ones of both keys, then the odd ones
+                const uint32_t even = e4m3_f16(x), odd = e4m3_f16_high(x);
+                v[i >> 1][(i & 1) * 2] = kF16 ? mul_f16x2(even, mult[i]) : mul_bf16x2(f16_bf16(even), mult[i]);
+                v[i >> 1][(i & 1) * 2 + 1] = kF16 ? mul_f16x2(odd, mult[i]) : mul_bf16x2(f16_bf16(odd), mult[i]);
+              }
 #pragma unroll
-            for (int m = 0; m < kTiles; ++m) {
-              mma16816<kFp8>(acc[m][j], v[0], pf[m][0][0], pf[m][0][1]);
-              mma16816<kFp8>(acc[m][j], v[1], pf[m][kGroups - 1][0], pf[m][kGroups - 1][1]);
+              for (int m = 0; m < kTiles; ++m) {
+                mma16816<kF16>(acc[m][j], v[0], pf[m][0][0], pf[m][0][1]);
+                mma16816<kF16>(acc[m][j], v[1], pf[m][kGroups - 1][0], pf[m][kGroups - 1][1]);
+              }
             }
           }
-        }
+        };
+        if (!wide) add_values(Yes{});
+        else add_values(No{});
       }
       __syncwarp();
       stage = stage + 1 == kRowStages ? 0 : stage + 1;
@@ -584,6 +623,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     for (int m = 0; m < kTiles; ++m)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        if constexpr (kFp8) m_ref[m][e] -= kLiftF16;
         float x = l[m][e];
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
@@ -609,6 +649,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         // (from here on: the row's maximum, and the warp's sum relative to it)
         if (g == 0) sm->part_l[warp][r] = m_ref[m][e] == -INFINITY ? mine : mine * f[m][e];
         if (g == 0 && wi == 0) sm->row_top[wh * kRows + r] = top;
+        if constexpr (kFp8) f[m][e] *= exp2_int(unit - 127);
       }
     const int buffers = (rows <= 4 ? 8 : 4 / kTiles) / kHeads;  // of a head
     const int pitch = rows <= 4 ? 4 * kPitch : kRows * kPitch;

@@ -98,9 +98,15 @@ __device__ __forceinline__ uint32_t f16_bf16(uint32_t two) {
       "cvt.rn.bf16x2.f32 %0, y, x;\n\t}" : "=r"(r) : "r"(two));
   return r;
 }
-// The kernel for few rows multiplies in f16: code * 2^(n - N) with N the largest exponent of the
-// keys (or values) that one product takes, in units of 2^N.  That is exact down to n = N - 15 (f16 ends at 2^-24, a code at
-// 2^-9), off by less than bf16 would be down to N - 23, by less than e4m3's own rounding down to N - 27, and zero below N - 34.
+// The kernel for few rows adds values in f16 where it can: code * 2^(n - U), with U the largest exponent of the first values that
+// a warp sees of a unit.  With n - U in [-kBelowUnit, kAboveUnit] the products are exact (2^-9 * 2^-11 to 448 * 2^4, of f16's 2^-24 to
+// 65504).  From the first step on that holds another n, for whatever row or column, the warp goes on in bf16, where a code
+// times a power of two is exact for every n; U, which is the unit of the fp32 sums, then rises with the largest n.
+// Probabilities go with the values.  f16: multiplied by 2^kLiftF16, so that the largest lies between 2^11 and 2^15 (a row's
+// reference moves when a score is kAheadF16 above it).  They are rounded by 2^-11 down to 2^-25 of the largest, below that by no
+// more than 2^-36 of it, against values whose blocks' largest are no more than 2^16 apart.  (Going back to f16 after other
+// values would end that: small probabilities of large values would be measured by large probabilities of small ones.)
+// bf16: rounded by 2^-8, whatever their size.
 // (One conversion for two codes and one product; putting a code's bits into a bf16 instead takes four integer instructions at
 // half rate: 64 tokens against up to 16 384 keys of 8 heads took 302 us with those and 238 without, all else alike.)
 __device__ __forceinline__ uint32_t e4m3_f16(uint32_t two) {  // the two low bytes
@@ -122,6 +128,26 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+constexpr int kBelowUnit = 11, kAboveUnit = 4;
+constexpr int kLeastUnit = 17;  // 2^-110
+constexpr float kAheadF16 = 4.f, kLiftF16 = 11.f;
+// Whether one of four scale bytes lies outside the unit's range (or beyond the written one).
+__device__ __forceinline__ bool values_outside(uint32_t w, int unit) {
+  const uint32_t even = w & 0x00ff00ffu, odd = (w >> 8) & 0x00ff00ffu;
+  const uint32_t high = min(unit + kAboveUnit, kMaxScale) * 0x10001u, low = (unit - kBelowUnit) * 0x10001u;
+  // (a difference below zero sets its half's top bit; what it borrows from the other half can only do the same there)
+  return ((high - __vmaxu2(even, odd)) | (__vminu2(even, odd) - low)) & 0x80008000u;
+}
+// 2^(byte - unit), in f16 for four bytes inside the range: of the first and third, of the second and fourth.
+__device__ __forceinline__ uint2 unit_f16(uint32_t w, int unit) {
+  const uint32_t bias = (uint32_t)(15 - unit) * 0x10001u;
+  return make_uint2(((w & 0x00ff00ffu) + bias) << 10, (((w >> 8) & 0x00ff00ffu) + bias) << 10);
+}
+// In bf16, for any byte (zero below 2^-133; beyond the written range: not a number).
+__device__ __forceinline__ uint32_t unit_bf16(uint32_t byte, int unit) {
+  const int e = (int)byte - unit + 127;
+  return byte > (uint32_t)kMaxScale ? 0x7fc0u : e > 0 ? (uint32_t)e << 7 : 0x80u >> min(1 - e, 15);
 }
 // 2^(byte - top), top >= byte, as a float (0 below 2^-126); bytes beyond the written range: not a number.
 __device__ __forceinline__ float scale_relative(uint32_t byte, int top) {
