@@ -15,9 +15,12 @@
 //
 // A CTA takes one K/V head, of e4m3 two neighbours with four warps each where it can, so that 256 bytes lie in a row.
 //
-// e4m3: codes are turned into f16; values are multiplied by their powers of two there while these lie close together, else in
-// bf16 (see paged_common.cuh).  Keys are multiplied by theirs relative to the step's largest (16 rows), or the scores by the
-// keys' (8 rows).  Half of a step's instructions go there.  P is rounded with the values, scores and sums are fp32.
+// e4m3: codes are turned into f16, queries too.  Values are multiplied by their powers of two, and with 16 rows keys are; with 8
+// the scores of 32 columns at a time are multiplied by the keys', in fp32 (half as many products).  This is exact as long as the powers
+// lie close together (see paged_common.cuh).  The loop over steps leaves at the first step where they do not, and a second one goes
+// on, with values by way of bf16, keys' and queries' powers in fp32, and P in bf16: 64 tokens against up to 16 384 keys take
+// 181 us in the first loop and 226 in the second.  Half of a step's instructions go there.  P is rounded with the values, scores and
+// sums are fp32.
 //
 // The work of a launch is a list of steps (128 keys of one block of rows in bf16, 256 in e4m3), sequence by
 // sequence, head by head; every CTA takes an equal, contiguous part, so that lengths need not balance.  The lengths are on
@@ -55,7 +58,8 @@ struct RowSmem {
   int b, step;                               // where this CTA's part starts: sequence, and step inside it
   float2 ml[kRowWarps][16];                  // of a unit: every warp's maximum and sum,
   float part_l[kRowWarps][16], row_top[32];  // its sum relative to the rows' maxima, these
-  float q_scale[32];  // e4m3: power of two that a row of queries was divided by
+  float q_scale[32];     // e4m3: power of two that a row of queries was divided by,
+  float q_block[32][4];  // and what its blocks were divided by beside it
 };
 
 template <bool kFp8, int kHeads>
@@ -161,7 +165,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   using S = RowShape<kFp8>;
   constexpr int kWarps = kRowWarps / kHeads;  // of a head
   constexpr int kKeys = S::kKeys, kStep = kWarps * kKeys, kGroups = kKeys / 16, kRows = 8 * kTiles;
-  constexpr bool kScaled = kFp8 && kTiles == 1;  // scores, not keys, are multiplied by the keys' powers of two
+  constexpr bool kKeyUnits = kFp8 && kTiles > 1;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int wh = warp / kWarps, wi = warp % kWarps;  // head of this warp, which of its warps it is
@@ -169,9 +173,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   uint8_t* queries = smem_raw + kRowWarps * kRowStages * S::kStage;  // rows of 256 bytes, pieces swapped like the keys'
   float* merge = reinterpret_cast<float*>(queries + kHeads * 16 * 2 * kHeadDim);
   RowSmem* sm = reinterpret_cast<RowSmem*>(merge + 32 * kPitch);
-  // e4m3: a step's powers of two: [32 keys][4 blocks] for the keys, f16 twice (kScaled: fp32), [4 blocks][32 keys] for the values; where
+  // e4m3: a step's powers of two: [32 keys][4 blocks] for the keys, [4 blocks][32 keys] in f16 or bf16 for the values; where
   // the states are merged at a unit's end
-  uint32_t* key_scale = reinterpret_cast<uint32_t*>(merge) + warp * 192;
+  float* key_scale = merge + warp * 192;
   uint16_t* value_scale = reinterpret_cast<uint16_t*>(key_scale + 128);
   const uint32_t stage0 = smem_u32(stages);
 
@@ -314,13 +318,18 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
   // A lane of the matrix instruction takes element pairs (2 t, 2 t + 1) and (8 + 2 t, ...) of 16 along head_dim.  Of e4m3 keys
   // it gets four neighbouring values at once, so that its two pairs are 4 t .. 4 t + 3; the queries are put in that order.
   auto store_q = [&]() {
+    bool uneven = false;
 #pragma unroll
     for (int m = 0; m < kPasses; ++m) {
       const int r = m * 16 + (tid >> 4), piece = tid & 15;
       uint8_t* row = queries + r * 2 * kHeadDim;
       if constexpr (kFp8) {
-        const float scale = query_to_f16(qx[m]);
+        float block;
+        bool row_uneven;
+        const float scale = query_to_f16(qx[m], block, row_uneven);
+        uneven |= row_uneven;
         if (piece == 0) sm->q_scale[r] = scale;
+        if ((piece & 3) == 0) sm->q_block[r][piece >> 2] = block;
       }
       if constexpr (!kFp8) {
         *reinterpret_cast<uint4*>(row + ((piece ^ (r & 7)) << 4)) = qx[m];
@@ -329,6 +338,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         *reinterpret_cast<uint2*>(row + (((piece | 1) ^ (r & 7)) << 4) + (piece & 1) * 8) = make_uint2(qx[m].y, qx[m].w);
       }
     }
+    return uneven;
   };
   // Queries of 8 rows as the second operand, for 32 elements along head_dim (two products)
   const uint32_t q_addr = smem_u32(queries) + (wh * kRows + (lane & 7)) * 2 * kHeadDim + (((lane >> 3) ^ (lane & 7)) << 4);
@@ -341,17 +351,22 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
     const bool from_start = at.step == 0;  // its earlier steps are not another CTA's
     const int unit_end = min(last, s + at.steps - at.step);
     const bool done = unit_end == s + at.steps - at.step;
-    store_q();
+    bool uneven = store_q();
     next_unit<kStep, kRows, kHeads>(a, nx);
     fetch_q();
-    __syncthreads();  // the queries are there, and the buffers of the unit before are free again
+    // the queries are there, and the buffers of the unit before are free again
+    if constexpr (kFp8) uneven = __syncthreads_or(uneven);
+    else __syncthreads();
     float acc[kTiles][8][4], m_ref[kTiles][2], l[kTiles][2];
     int limit[kTiles][2];        // keys that the row sees; the first of the unit's rows sees the fewest
-    float row_scale[kTiles][2];  // e4m3: power of two of the row's queries
+    float c[kTiles][2];          // of its scores; e4m3: with the power of two of the row's queries
     uint32_t qk[kTiles][4][4];
-    int unit = 0;       // e4m3: acc is in units of 2^(unit - 127) (see paged_common.cuh; 0: no step yet),
-    bool wide = false;  // and values go by way of bf16
+    int unit = 0, key_unit = 0;  // e4m3: acc is in units of 2^(unit - 127), scores of 2^(key_unit - 127) (0: no step yet)
     const int row0 = at.block * kRows, rows = min(at.s.n * a.group - row0, kRows);
+    auto factor = [&](int m, int e, float keys) {  // of a row's scores, in units of the exponent of two
+      // (not zero and not infinite, with which hidden or zero scores would make no number)
+      return kFp8 ? fminf(fmaxf(a.scale_log2 * sm->q_scale[wh * kRows + m * 8 + 2 * t + e] * keys, 1.2e-38f), 3.4e38f) : a.scale_log2;
+    };
     const int seen_by_all = a.causal ? at.s.len - at.s.n + row0 / a.group + 1 : at.s.len;
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
@@ -365,27 +380,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         m_ref[m][e] = -INFINITY;
         l[m][e] = 0.f;
         limit[m][e] = a.causal ? min(at.s.len, at.s.len - at.s.n + (row0 + r) / a.group + 1) : at.s.len;
-        row_scale[m][e] = kFp8 ? sm->q_scale[wh * kRows + r] : 1.f;
+        c[m][e] = factor(m, e, 1.f);
       }
 #pragma unroll
       for (int k2 = 0; k2 < 4; ++k2) queries_of(qk[m][k2], m, k2);
     }
 
-#pragma unroll 1
-    for (; s < unit_end; ++s, ++at.step) {
-      // ---- keep the loads going
-      if (to_load > 0) {
-        load(stage == 0 ? kRowStages - 1 : stage - 1);
-        if (--to_load > 0) {
-          next_step<kStep, kRows, kHeads>(a, in);
-          entry = entry_of(in);
-        }
-      }
-      cp_async_commit();
-      cp_async_wait<kRowStages - 1>();
-      __syncwarp();
-
-      // ---- one step
+    // ---- one step; kWide (e4m3): values by way of bf16, blocks of queries with powers of their own.  False, and nothing done, where
+    // the step needs kWide.  (That is asked where the maximum is looked at: a branch of its own before the products cost 3 to 5 %.)
+    uint32_t kw = 0, vw = 0;  // e4m3: the powers of two of this lane's key and value
+    auto step = [&](auto wide) {
+      constexpr bool kWide = decltype(wide)::value, kF16 = kFp8 && !kWide, kKeysF16 = kKeyUnits && !kWide;
       const uint32_t sk = stage0 + stage * S::kStage, sv = sk + S::kHalf;
       const int key0 = at.step * kStep + wi * kKeys;
       float sc[kTiles][kGroups][4];  // of 16 keys each
@@ -395,7 +400,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         for (int j = 0; j < kGroups; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[m][j][e] = 0.f;
-      float step_scale = a.scale_log2;  // of the step's scores; e4m3: with the keys' power of two
       if constexpr (!kFp8) {
         // four 8 x 8 matrices: keys 0-7 and 8-15 of one 16-byte piece, then of the next
         const uint32_t k_addr = sk + (lane & 15) * S::kRowBytes + (((lane >> 4) ^ (lane & 7)) << 4);
@@ -412,56 +416,20 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
           }
         }
       } else {
-        // The powers of two of this lane's key.  The keys' are taken relative to the largest of the step, so that f16 holds the
-        // products, or with 8 rows the scores of 32 columns at a time are multiplied by them (kScaled: half as
-        // many products, and no rounding; 64 single tokens up to 16 384 keys 186 us and 182, 8 tokens each up to 8 192, 16 rows,
-        // 333 and 347).
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(stages + stage * S::kStage + 2 * S::kHalf);
-        const uint32_t kw = words[lane];
-        // (behind the sequence's end: of no effect on the unit, and a number)
-        uint32_t vw = key0 + lane < at.s.len ? words[kKeys + lane] : unit * 0x01010101u;
-        if (__any_sync(0xffffffffu, unit == 0 || values_outside(vw, unit))) {
-          const int top = max((int)__reduce_max_sync(0xffffffffu, scale_top(vw)), kLeastUnit);
-          wide = unit > 0;
-          if (top > unit + kAboveUnit) {
-            const float f = unit - top < -126 ? 0.f : exp2_int(unit - top);
-#pragma unroll
-            for (int m = 0; m < kTiles; ++m)
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[m][j][e] *= f;
-            unit = top;
-          }
-          if (key0 + lane >= at.s.len) vw = unit * 0x01010101u;
-          if (!wide) wide = __any_sync(0xffffffffu, values_outside(vw, unit));
-        }
-        int k_top = 127;
-        if constexpr (!kScaled) k_top = max((int)__reduce_max_sync(0xffffffffu, scale_top(kw)), kMinScale);
-        uint32_t ks[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const float k2 = scale_relative((kw >> (8 * b)) & 0xffu, k_top);
-          ks[b] = kScaled ? __float_as_uint(k2) : pack_f16x2(k2, k2);
-        }
-        if (!wide) {
-          const uint2 x = unit_f16(vw, unit);
-          value_scale[lane] = (uint16_t)x.x;
-          value_scale[kKeys + lane] = (uint16_t)x.y;
-          value_scale[2 * kKeys + lane] = (uint16_t)(x.x >> 16);
-          value_scale[3 * kKeys + lane] = (uint16_t)(x.y >> 16);
-        } else {
-#pragma unroll
-          for (int b = 0; b < 4; ++b) value_scale[b * kKeys + lane] = (uint16_t)unit_bf16((vw >> (8 * b)) & 0xffu, unit);
-        }
-        *reinterpret_cast<uint4*>(key_scale + lane * 4) = make_uint4(ks[0], ks[1], ks[2], ks[3]);
+        // Keys are multiplied by their powers of two in f16, or the scores of 32 columns at a time in fp32.
+        if constexpr (kKeysF16)
+          *reinterpret_cast<uint4*>(key_scale + lane * 4) = unit_f16_pairs(kw, key_unit);
+        else
+          *reinterpret_cast<float4*>(key_scale + lane * 4) =
+              make_float4(scale_value(kw & 0xffu), scale_value((kw >> 8) & 0xffu), scale_value((kw >> 16) & 0xffu), scale_value(kw >> 24));
+        if constexpr (kWide) store_unit_bf16(value_scale + lane, vw, unit);
+        else store_unit_f16(value_scale + lane, vw, unit);
         __syncwarp();
-        step_scale = a.scale_log2 * exp2_int(k_top - 127);
         // four matrices: the 32 keys x one piece of 16 values, which makes two operands of 16 keys x 16 values
         const uint32_t k_addr = sk + lane * S::kRowBytes + ((lane & 7) << 4);
 #pragma unroll
         for (int k2 = 0; k2 < 4; ++k2) {
-          uint32_t mult[4];
+          float mult[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) mult[j] = key_scale[(j * 8 + g) * 4 + k2];
           uint32_t kf[2][2][4];  // [piece][16 keys]
@@ -475,9 +443,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
               kf[i][j][1] = e4m3_f16(b[2 * j + 1]);
               kf[i][j][2] = e4m3_f16_high(b[2 * j]);
               kf[i][j][3] = e4m3_f16_high(b[2 * j + 1]);
-              if constexpr (!kScaled) {
+              if constexpr (kKeysF16) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) kf[i][j][e] = mul_f16x2(kf[i][j][e], mult[2 * j + (e & 1)]);
+                for (int e = 0; e < 4; ++e) kf[i][j][e] = mul_f16x2(kf[i][j][e], __float_as_uint(mult[2 * j + (e & 1)]));
               }
             }
           }
@@ -486,15 +454,18 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
             const uint32_t(&q)[4] = qk[m][k2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              if constexpr (kScaled) {
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816<kFp8>(part, kf[0][j], q[0], q[1]);
-                mma16816<kFp8>(part, kf[1][j], q[2], q[3]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sc[m][j][e] = fmaf(part[e], __uint_as_float(mult[2 * j + (e >> 1)]), sc[m][j][e]);
-              } else {
+              if constexpr (kKeysF16) {
                 mma16816<kFp8>(sc[m][j], kf[0][j], q[0], q[1]);
                 mma16816<kFp8>(sc[m][j], kf[1][j], q[2], q[3]);
+                continue;
+              }
+              float part[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816<kFp8>(part, kf[0][j], q[0], q[1]);
+              mma16816<kFp8>(part, kf[1][j], q[2], q[3]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if constexpr (kWide) part[e] *= sm->q_block[wh * kRows + m * 8 + 2 * t + (e & 1)][k2];
+                sc[m][j][e] = fmaf(part[e], mult[2 * j + (e >> 1)], sc[m][j][e]);
               }
             }
           }
@@ -514,7 +485,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
       // A row's reference only moves when a score exceeds it by kAhead.  Each lane looks at its own keys, and the row's maximum is
       // only taken when one of them does.
       constexpr float kAhead = kFp8 ? kAheadF16 : 8.f;
-      float c[kTiles][2], top[kTiles][2];
+      float top[kTiles][2];
       bool need = false;
 #pragma unroll
       for (int m = 0; m < kTiles; ++m)
@@ -522,12 +493,14 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         for (int e = 0; e < 2; ++e) {
           float x = fmaxf(sc[m][0][e], sc[m][0][2 + e]);
           if constexpr (kGroups == 2) x = max3(x, sc[m][kGroups - 1][e], sc[m][kGroups - 1][2 + e]);
-          // (not zero, with which hidden scores would make no number)
-          c[m][e] = kFp8 ? fmaxf(step_scale * row_scale[m][e], 1.2e-38f) : step_scale;
           top[m][e] = x == -INFINITY ? -INFINITY : x * c[m][e];
           need |= top[m][e] - m_ref[m][e] > kAhead;
         }
+      if constexpr (kF16) need |= outside_unit(vw, unit) || (kKeyUnits && outside_unit(kw, key_unit));
       if (__any_sync(0xffffffffu, need)) {
+        if constexpr (kF16) {
+          if (__any_sync(0xffffffffu, outside_unit(vw, unit) || (kKeyUnits && outside_unit(kw, key_unit)))) return false;
+        }
 #pragma unroll
         for (int m = 0; m < kTiles; ++m)
 #pragma unroll
@@ -560,10 +533,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
             const float p1 = fast_exp2(fmaf(sc[m][j][2 * i + 1], c[m][1], lift[1]));
             sum[0] += p0;
             sum[1] += p1;
-            uint32_t both;
-            if (kFp8 && !wide) both = pack_f16x2(p0, p1);
-            else both = pack_bf16x2(p0, p1);
-            pf[m][j][i] = transpose8x8(both);
+            pf[m][j][i] = transpose8x8(kF16 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1));
           }
 #pragma unroll
         for (int e = 0; e < 2; ++e) l[m][e] += sum[e];
@@ -584,38 +554,104 @@ __global__ void __launch_bounds__(kRowThreads, 1) paged_rows_kernel(const __grid
         // Transposed 16-bit units are pairs of neighbouring values: a lane gets values (2 g, 2 g + 1) of keys (2 t, 2 t + 1) of
         // each 8; the even ones are the product's rows 0-7, the odd ones rows 8-15.
         const uint32_t v_addr = sv + lane * S::kRowBytes + ((lane & 7) << 4);
-        auto add_values = [&](auto f16) {
-          constexpr bool kF16 = decltype(f16)::value;
 #pragma unroll
-          for (int j2 = 0; j2 < 4; ++j2) {
-            uint32_t mult[4];
+        for (int j2 = 0; j2 < 4; ++j2) {
+          uint32_t mult[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mult[i] = *reinterpret_cast<const uint32_t*>(value_scale + j2 * kKeys + i * 8 + 2 * t);
+          for (int i = 0; i < 4; ++i) mult[i] = *reinterpret_cast<const uint32_t*>(value_scale + j2 * kKeys + i * 8 + 2 * t);
 #pragma unroll
-            for (int j = 2 * j2; j < 2 * j2 + 2; ++j) {
-              uint32_t b[4];
-              ldsm4_t(b, v_addr ^ (j << 4));
-              uint32_t v[2][4];
+          for (int j = 2 * j2; j < 2 * j2 + 2; ++j) {
+            uint32_t b[4];
+            ldsm4_t(b, v_addr ^ (j << 4));
+            uint32_t v[2][4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t x = __byte_perm(b[i], 0, 0x3120);  // the even ones of both keys, then the odd ones
-                const uint32_t even = e4m3_f16(x), odd = e4m3_f16_high(x);
-                v[i >> 1][(i & 1) * 2] = kF16 ? mul_f16x2(even, mult[i]) : mul_bf16x2(f16_bf16(even), mult[i]);
-                v[i >> 1][(i & 1) * 2 + 1] = kF16 ? mul_f16x2(odd, mult[i]) : mul_bf16x2(f16_bf16(odd), mult[i]);
-              }
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t x = __byte_perm(b[i], 0, 0x3120);  // the even ones of both keys, then the odd ones
+              const uint32_t even = e4m3_f16(x), odd = e4m3_f16_high(x);
+              v[i >> 1][(i & 1) * 2] = kF16 ? mul_f16x2(even, mult[i]) : mul_bf16x2(f16_bf16(even), mult[i]);
+              v[i >> 1][(i & 1) * 2 + 1] = kF16 ? mul_f16x2(odd, mult[i]) : mul_bf16x2(f16_bf16(odd), mult[i]);
+            }
 #pragma unroll
-              for (int m = 0; m < kTiles; ++m) {
-                mma16816<kF16>(acc[m][j], v[0], pf[m][0][0], pf[m][0][1]);
-                mma16816<kF16>(acc[m][j], v[1], pf[m][kGroups - 1][0], pf[m][kGroups - 1][1]);
-              }
+            for (int m = 0; m < kTiles; ++m) {
+              mma16816<kF16>(acc[m][j], v[0], pf[m][0][0], pf[m][0][1]);
+              mma16816<kF16>(acc[m][j], v[1], pf[m][kGroups - 1][0], pf[m][kGroups - 1][1]);
             }
           }
-        };
-        if (!wide) add_values(Yes{});
-        else add_values(No{});
+        }
       }
       __syncwarp();
       stage = stage + 1 == kRowStages ? 0 : stage + 1;
+      return true;
+    };
+    auto fetch = [&]() {  // keeps the loads going, and waits for the step's own
+      if (to_load > 0) {
+        load(stage == 0 ? kRowStages - 1 : stage - 1);
+        if (--to_load > 0) {
+          next_step<kStep, kRows, kHeads>(a, in);
+          entry = entry_of(in);
+        }
+      }
+      cp_async_commit();
+      cp_async_wait<kRowStages - 1>();
+      __syncwarp();
+      if constexpr (kFp8) {  // (behind the sequence's end: of no effect on the unit, and a number)
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(stages + stage * S::kStage + 2 * S::kHalf);
+        const bool real = at.step * kStep + wi * kKeys + lane < at.s.len;
+        kw = real ? words[lane] : key_unit * 0x01010101u;
+        vw = real ? words[kKeys + lane] : unit * 0x01010101u;
+      }
+    };
+    fetch();
+    if constexpr (kFp8) {  // the units, by the first step
+      const bool real = at.step * kStep + wi * kKeys + lane < at.s.len;
+      unit = max((int)__reduce_max_sync(0xffffffffu, scale_top(vw)), kLeastUnit);
+      if (!real) vw = unit * 0x01010101u;
+      if constexpr (kKeyUnits) {
+        key_unit = max((int)__reduce_max_sync(0xffffffffu, scale_top(kw)), kMinScale);
+        if (!real) kw = key_unit * 0x01010101u;
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) c[m][e] = factor(m, e, exp2_int(key_unit - 127));
+      }
+    }
+    bool more = true;
+    if (!kFp8 || !uneven) {
+#pragma unroll 1
+      while (step(No{})) {
+        ++s;
+        ++at.step;
+        more = s < unit_end;
+        if (!more) break;
+        fetch();
+      }
+    }
+    if (kFp8 && more) {
+      if constexpr (kKeyUnits) {
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) c[m][e] = factor(m, e, 1.f);
+      }
+#pragma unroll 1
+      while (true) {
+        const int most = (int)__reduce_max_sync(0xffffffffu, scale_top(vw));
+        if (most > unit + kAboveUnit) {
+          const float f = unit - most < -126 ? 0.f : exp2_int(unit - most);
+#pragma unroll
+          for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[m][j][e] *= f;
+          unit = most;
+        }
+        step(Yes{});
+        ++s;
+        ++at.step;
+        if (s == unit_end) break;
+        fetch();
+      }
     }
 
     // ---- the warps' states become one: through as many buffers as fit, in turns where these are fewer than warps

@@ -102,6 +102,7 @@ __device__ __forceinline__ uint32_t f16_bf16(uint32_t two) {
 // a warp sees of a unit.  With n - U in [-kBelowUnit, kAboveUnit] the products are exact (2^-9 * 2^-11 to 448 * 2^4, of f16's 2^-24 to
 // 65504).  From the first step on that holds another n, for whatever row or column, the warp goes on in bf16, where a code
 // times a power of two is exact for every n; U, which is the unit of the fp32 sums, then rises with the largest n.
+// Keys that are multiplied in f16 have a U of their own and the same range; else scores are multiplied by 2^n in fp32.
 // Probabilities go with the values.  f16: multiplied by 2^kLiftF16, so that the largest lies between 2^11 and 2^15 (a row's
 // reference moves when a score is kAheadF16 above it).  They are rounded by 2^-11 down to 2^-25 of the largest, below that by no
 // more than 2^-36 of it, against values whose blocks' largest are no more than 2^16 apart.  (Going back to f16 after other
@@ -133,25 +134,38 @@ constexpr int kBelowUnit = 11, kAboveUnit = 4;
 constexpr int kLeastUnit = 17;  // 2^-110
 constexpr float kAheadF16 = 4.f, kLiftF16 = 11.f;
 // Whether one of four scale bytes lies outside the unit's range (or beyond the written one).
-__device__ __forceinline__ bool values_outside(uint32_t w, int unit) {
+__device__ __forceinline__ bool outside_unit(uint32_t w, int unit) {
   const uint32_t even = w & 0x00ff00ffu, odd = (w >> 8) & 0x00ff00ffu;
   const uint32_t high = min(unit + kAboveUnit, kMaxScale) * 0x10001u, low = (unit - kBelowUnit) * 0x10001u;
   // (a difference below zero sets its half's top bit; what it borrows from the other half can only do the same there)
   return ((high - __vmaxu2(even, odd)) | (__vminu2(even, odd) - low)) & 0x80008000u;
 }
-// 2^(byte - unit), in f16 for four bytes inside the range: of the first and third, of the second and fourth.
-__device__ __forceinline__ uint2 unit_f16(uint32_t w, int unit) {
+// 2^(byte - unit) of a word's four bytes, to places 32 apart: in f16 for bytes inside the range,
+__device__ __forceinline__ void store_unit_f16(uint16_t* to, uint32_t w, int unit) {
   const uint32_t bias = (uint32_t)(15 - unit) * 0x10001u;
-  return make_uint2(((w & 0x00ff00ffu) + bias) << 10, (((w >> 8) & 0x00ff00ffu) + bias) << 10);
+  const uint32_t even = ((w & 0x00ff00ffu) + bias) << 10, odd = (((w >> 8) & 0x00ff00ffu) + bias) << 10;
+  to[0] = (uint16_t)even;
+  to[32] = (uint16_t)odd;
+  to[64] = (uint16_t)(even >> 16);
+  to[96] = (uint16_t)(odd >> 16);
 }
-// In bf16, for any byte (zero below 2^-133; beyond the written range: not a number).
-__device__ __forceinline__ uint32_t unit_bf16(uint32_t byte, int unit) {
-  const int e = (int)byte - unit + 127;
-  return byte > (uint32_t)kMaxScale ? 0x7fc0u : e > 0 ? (uint32_t)e << 7 : 0x80u >> min(1 - e, 15);
+// or twice each in a word of their own,
+__device__ __forceinline__ uint4 unit_f16_pairs(uint32_t w, int unit) {
+  const uint32_t bias = (uint32_t)(15 - unit) * 0x10001u;
+  const uint32_t even = ((w & 0x00ff00ffu) + bias) << 10, odd = (((w >> 8) & 0x00ff00ffu) + bias) << 10;
+  return make_uint4(__byte_perm(even, 0, 0x1010), __byte_perm(odd, 0, 0x1010), __byte_perm(even, 0, 0x3232), __byte_perm(odd, 0, 0x3232));
 }
-// 2^(byte - top), top >= byte, as a float (0 below 2^-126); bytes beyond the written range: not a number.
-__device__ __forceinline__ float scale_relative(uint32_t byte, int top) {
-  return byte > (uint32_t)kMaxScale ? __int_as_float(0x7fc00000) : __int_as_float(max((int)byte - top + 127, 0) << 23);
+// in bf16 for any (zero below 2^-133; beyond the written range: not a number).
+__device__ __forceinline__ void store_unit_bf16(uint16_t* to, uint32_t w, int unit) {
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const int byte = (w >> (8 * b)) & 0xffu, e = byte - unit + 127;
+    to[32 * b] = (uint16_t)(byte > kMaxScale ? 0x7fc0 : e > 0 ? e << 7 : 0x80 >> min(1 - e, 15));
+  }
+}
+// 2^(byte - 127); bytes beyond the written range: not a number.
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return byte > (uint32_t)kMaxScale ? __int_as_float(0x7fc00000) : __int_as_float(max((int)(byte << 23), 0x00400000));
 }
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 // The largest of four scale bytes, those beyond the written range left out.
@@ -162,22 +176,40 @@ __device__ __forceinline__ uint32_t scale_top(uint32_t w) {
   return max(m & 0xffffu, m >> 16);
 }
 
-// A row of 16 lanes' queries, eight bf16 values each, as f16 in [-2, 2) (or (-4, 4)) times a power of two, which is returned.
-__device__ __forceinline__ float query_to_f16(uint4& x) {
+// A row of 16 lanes' queries, eight bf16 values each, as f16 times a power of two, which is returned: the largest lies in [2^15,
+// 2^16), so that f16 holds every value down to 2^-32 of it as it is.  A row with smaller ones is `uneven`: each block of 32
+// has a power of its own, `block` times that of the row (else 1).
+__device__ __forceinline__ float query_to_f16(uint4& x, float& block, bool& uneven) {
   uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t m = 0;
+  uint32_t hi = 0, lo = 0x7fff7fffu;  // |x| of bf16 orders like its bits; the least one that is not zero
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);  // |x| of bf16 orders like its bits
-  m = max(m & 0xffffu, m >> 16);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t v = w[i] & 0x7fff7fffu;
+    hi = __vmaxu2(hi, v);
+    lo = __vminu2(lo, v | (__vcmpeq2(v, 0) & 0x7fff7fffu));
+  }
+  hi = max(hi & 0xffffu, hi >> 16);
+  lo = min(lo & 0xffffu, lo >> 16);
+  uint32_t both = hi << 16 | (0x7fffu - lo);  // (the two go through the lanes together)
 #pragma unroll
-  for (int d = 1; d < 16; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-  const int e = m == 0 ? 0 : min(max((int)(m >> 7) - 127, -126), 126);
+  for (int d = 1; d < 16; d <<= 1) {
+    both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, d));
+    if (d == 2) hi = both >> 16;
+  }
+  const uint32_t own = hi;  // of the block
+  hi = both >> 16;
+  lo = 0x7fffu - (both & 0xffffu);
+  auto exponent = [](uint32_t most) { return min(max((int)(most >> 7) - 142, -126), 111); };
+  const int row = exponent(hi);
+  uneven = hi != 0 && (int)(hi >> 7) - (int)(lo >> 7) > 25;  // (7 bits less: bf16's subnormals have them)
+  const int e = uneven ? max(exponent(own), row - 126) : row;
+  block = exp2_int(e - row);
   const float inv = exp2_int(-e);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     w[i] = pack_f16x2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
   x = make_uint4(w[0], w[1], w[2], w[3]);
-  return exp2_int(e);
+  return exp2_int(row);
 }
 
 // ---- 16 or 4 bytes into shared memory, zeros where they are not real --------------------------

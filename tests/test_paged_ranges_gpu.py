@@ -112,3 +112,54 @@ def test_values_grow_as_probabilities_fall(lens, heads, new, order, most):
         kv[0, :, :, 0] = (-e * 0.6931 / (4.0 * SCALE)).to(torch.bfloat16)  # (e4m3 makes of it what it can: within 2^(e / 16))
         kv[1] = times(kv[1], torch.exp2(e)[..., None])
     run(batch)
+
+
+@pytest.mark.parametrize("lens", LENS)
+@pytest.mark.parametrize("heads,new", ROWS)
+@pytest.mark.parametrize("exponents", [(0, 6, -9, 3), (0, 15, -15, 0), (0, 20, 5, -10), (0, 28, 14, 2)])
+def test_key_blocks_of_unequal_size(lens, heads, new, exponents):
+    """Keys are large where the queries are small, so that every block counts alike in the scores."""
+    batch = Batch(lens, [new] * len(lens), heads, 16, True, ragged=False, seed=66, spread=2.0)
+    batch.q = times(batch.q, 1 / powers(exponents))
+    for kv in batch.kv:
+        kv[0] = times(kv[0], powers(exponents))
+    run(batch)
+
+
+@pytest.mark.parametrize("lens", LENS)
+@pytest.mark.parametrize("heads,new", ROWS)
+@pytest.mark.parametrize("size", [12, 18, 24, 40])
+def test_keys_that_are_large_where_the_queries_are_zero(lens, heads, new, size):
+    """One block of some keys is 2^size times the others, and no query looks there."""
+    batch = Batch(lens, [new] * len(lens), heads, 16, True, ragged=False, seed=67, spread=2.0)
+    batch.q[..., 64:96] = 0
+    for kv in batch.kv:
+        kv[0, ::5, :, 64:96] = times(kv[0, ::5, :, 64:96], 2.0 ** size)
+    run(batch)
+
+
+@pytest.mark.parametrize("lens", LENS)
+@pytest.mark.parametrize("heads,new", ROWS)
+def test_zero_values_and_keys(lens, heads, new):
+    """Blocks of zeros get the least power of two; beside others they change nothing."""
+    batch = Batch(lens, [new] * len(lens), heads, 16, True, ragged=False, seed=68)
+    for kv in batch.kv:
+        kv[1, ::3] = 0
+        kv[1, 1::3, :, :32] = 0
+        kv[0, ::4] = 0
+        kv[:, :40] = 0
+    run(batch)
+
+
+@pytest.mark.parametrize("lens", LENS)
+@pytest.mark.parametrize("heads,new", ROWS)
+def test_powers_of_two_that_no_write_makes(lens, heads, new):
+    """Scale bytes from 3 to 76, which the cache of another program may hold."""
+    batch = Batch(lens, [new] * len(lens), heads, 16, True, ragged=False, seed=69)
+    g = torch.Generator().manual_seed(70)
+    for lo, hi in ((60, 76), (30, 45), (3, 76)):
+        k, v, ks, vs = batch.cache_tensors()
+        used = vs != 255
+        vs = torch.where(used, torch.randint(lo, hi + 1, vs.shape, generator=g, dtype=torch.uint8), vs)
+        ks = torch.where(used, torch.randint(max(lo, 30), hi + 1, ks.shape, generator=g, dtype=torch.uint8), ks)
+        run(batch, (k, v, ks, vs))
