@@ -460,7 +460,7 @@ MB_API int mb_kv_cache_write(const mb_paged_kv* kv, const void* k_new, const voi
 
 /* The first min(seq_lens[b], rows) keys and values of every sequence, in bf16, into k_out and v_out [batch, rows,
  * hkv, head_dim]; the rows behind a sequence's last key are left as they are.  A code times its power of two is
- * exact in bf16.  cu_seqlens and tokens are not used. */
+ * exact in bf16 from scale byte 3 on (below, rounded to multiples of 2^-133).  cu_seqlens and tokens are not used. */
 MB_API int mb_kv_cache_read(const mb_paged_kv* kv, void* k_out, void* v_out, int64_t stride_b, int64_t stride_s,
                             int64_t stride_h, int32_t rows, void* cuda_stream);
 

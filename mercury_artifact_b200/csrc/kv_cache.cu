@@ -11,8 +11,8 @@
 // 18 us, 5.5 TB/s; reading 62 768 e4m3 keys of 8 heads back 66 us, 5.9 TB/s; single tokens of 32 sequences 9 us, all of it the
 // host's launch.
 //
-// Why powers of two: a code has 4 significant bits, so code * 2^e is exact in bf16.  What is read back, and what the
-// attention kernels multiply, is the stored value itself with no second rounding; a factor of amax / 448 would use
+// Why powers of two: a code has 4 significant bits, so code * 2^e is exact in bf16 (for every e that a write chooses).  What is
+// read back, and what the attention kernels multiply, is the stored value itself with no second rounding; a factor of amax / 448 would use
 // the top of the range a little better (at most one binade), but e4m3's step is relative, so that nothing is gained.
 #include "attn_paged.cuh"
 

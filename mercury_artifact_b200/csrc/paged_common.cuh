@@ -86,7 +86,7 @@ __device__ __forceinline__ long long scale_offset(const PagedView& c, int id, in
 }
 
 // ---- e4m3 codes as f16 and bf16 ------------------------------------------------------------
-// Both hold every code as it is, and a code times a power of two is exact in bf16.
+// Both hold every code as it is, and a code times a power of two is exact in bf16 (down to its least value, 2^-133).
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));

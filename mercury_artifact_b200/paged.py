@@ -37,9 +37,10 @@ class PagedKV:
     k, v: [pages, page_size, heads, 128], views are fine (a cache laid out [pages, heads, page_size, 128] goes in
     transposed) as long as head_dim is contiguous, k and v share their strides, and these are multiples of 16 bytes.
     bfloat16, or float8_e4m3fn with k_scale, v_scale: contiguous uint8 [pages, heads, page_size, 4].  Byte x is the power
-    of two 2^(x - 127) that 32 values share: a code times its power of two is exact in bfloat16.  A write chooses 77 .. 191;
-    bytes from 192 on make their values NaN, and so do e4m3's NaN codes (0x7f, 0xff), which no write makes.  The calls go to
-    the memory that these tensors have when the cache is made.
+    of two 2^(x - 127) that 32 values share: a code times its power of two is exact in bfloat16 from byte 3 on (below, the
+    least codes fall under bfloat16's least value, 2^-133, and are rounded to it or zero when they are read).  A write chooses
+    77 .. 191; bytes from 192 on make their values NaN, and so do e4m3's NaN codes (0x7f, 0xff), which no write makes.  The
+    calls go to the memory that these tensors have when the cache is made.
     """
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
@@ -177,7 +178,7 @@ def kv_cache_read(cache: PagedKV, page_table: torch.Tensor, seq_lens: torch.Tens
 
     out: the buffer to write to; rows behind a sequence's last key are left as they are, keys beyond its rows are left out.
     Without it a zero-filled one of max_keys rows is made (default: what the page table covers).  Values of a
-    float8_e4m3fn cache are exact: the code times its power of two."""
+    float8_e4m3fn cache are the code times its power of two, exact from scale byte 3 on."""
     args = cache._batch(page_table, seq_lens, None, 0)
     b, columns = page_table.shape
     if out is None:

@@ -163,3 +163,26 @@ def test_powers_of_two_that_no_write_makes(lens, heads, new):
         vs = torch.where(used, torch.randint(lo, hi + 1, vs.shape, generator=g, dtype=torch.uint8), vs)
         ks = torch.where(used, torch.randint(max(lo, 30), hi + 1, ks.shape, generator=g, dtype=torch.uint8), ks)
         run(batch, (k, v, ks, vs))
+
+
+def test_every_code_under_every_scale_byte_is_read_back():
+    """The code times its power of two to the nearest bf16: exact from byte 3 on; NaN from byte 192 on and for NaN codes."""
+    import mercury_artifact_b200 as mb
+    from oracle import paged as oracle
+
+    cache = mb.PagedKV.empty(16, 16, 2, torch.float8_e4m3fn)
+    codes = torch.arange(256, dtype=torch.uint8).view(1, 1, 2, 128).expand(16, 16, 2, 128)
+    scales = torch.arange(256, dtype=torch.uint8).view(16, 1, 16, 1).expand(16, 2, 16, 4)  # a byte a slot
+    for t, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        t.view(torch.uint8).copy_(codes)
+        s.copy_(scales)
+    table = torch.arange(16, dtype=torch.int32, device="cuda").view(1, 16)
+    got = mb.kv_cache_read(cache, table, torch.tensor([256], dtype=torch.int32, device="cuda"))[:, 0].cpu()
+    cache.check()
+    flat = torch.arange(256, dtype=torch.uint8).view(1, 2, 128).expand(256, 2, 128)
+    want = oracle.values(flat, torch.arange(256, dtype=torch.uint8).view(256, 1, 1).expand(256, 2, 4))
+    want = torch.where((flat & 127) == 127, torch.full_like(want, torch.nan), want)
+    assert torch.equal(want[3:192].to(torch.bfloat16).double()[~torch.isnan(want[3:192])], want[3:192][~torch.isnan(want[3:192])])
+    for c in range(2):
+        assert torch.equal(torch.isnan(got[c]), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(got[c].float()), torch.nan_to_num(want.to(torch.bfloat16).float()))
