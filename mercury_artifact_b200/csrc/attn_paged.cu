@@ -4,16 +4,16 @@
 namespace mb {
 
 // Most rows of a sequence (new tokens x heads of a group) that the kernel for few rows takes.  bf16: 17 to 32 rows are faster
-// as (an eighth of) a tile, 64 sequences of 8 tokens, 32/8 heads, up to 8 192 keys: 281 us, 394 as rows; 8 of them: 71, 71.
-// e4m3: a tile's sequence is first brought into bf16, which few rows do not pay for: 64 sequences as 32 rows take 333 us.  From
-// there on it depends: with 10 tokens they take 562 us as tiles and 472 as 40 rows, 8 of them 86 and 111, 64 up to 1 000 keys
-// 96 and 131, one of 32 768 keys 80 and 58.
+// as (an eighth of) a tile, 64 sequences of 8 tokens, 32/8 heads, up to 8 192 keys: 252 us, 428 as rows; 8 of them: 61, 112.
+// e4m3: a tile's sequence is first brought into bf16, which few rows do not pay for: 64 sequences as 32 rows take 330 us.  From
+// there on it depends: with 10 tokens they take 562 us as tiles and 468 as 40 rows, 8 of them 89 and 113, 64 up to 1 000 keys
+// 94 and 160, one of 32 768 keys 85 and 56.
 constexpr int kFewRows = 16, kFewRowsE4m3 = 32;
 // Steps up to which a unit of few rows is left to one CTA where there are no more units than SMs.  One token, 16 sequences of
 // 2 000 keys, 8 heads: 27 us, split 32; one sequence, 2 heads: 20 and 28 (the host's time included).
 constexpr int kWholeSteps = 16;
 // e4m3: sequences that go to the tiles are brought into bf16 in groups that take no more than this (or one by one).  64
-// sequences of 16 tokens, up to 8 192 keys: 620 us; groups of 256 MiB 688, of 4 GiB 570, which is not worth the memory.
+// sequences of 16 tokens, up to 8 192 keys: 563 us; groups of 256 MiB 706, of 4 GiB 557, which is not worth the memory.
 constexpr long long kPackedBytes = 1ll << 30;
 
 struct PagedPlan {
@@ -59,7 +59,7 @@ static int plan_paged(const mb_attn_paged_args* x, PagedPlan* p) {
     p->whole = units <= sms && x->max_keys <= kWholeSteps * step;
     p->row_ctas = p->whole ? (int)units : sms;
     // A head's row of e4m3 is 128 bytes.  Two neighbours at once read 256 in a row, as bf16 does: 64 single tokens, 32/8 heads, up
-    // to 16 384 keys 187 us, 202 one by one; 8 tokens each, up to 8 192 keys 337, 386.  Whole units stay one head's, which spreads
+    // to 16 384 keys 182 us, 202 one by one; 8 tokens each, up to 8 192 keys 330, 409.  Whole units stay one head's, which spreads
     // them over twice the SMs.
     p->row_heads = e4m3 && !p->whole && kv.hkv % 2 == 0 ? 2 : 1;
     p->rows_bytes = p->whole ? 0 : paged_rows_workspace(p->rows, p->row_heads, p->row_ctas);

@@ -27,9 +27,10 @@
 // the device: every CTA finds its part itself (one look at the sequences and a scan).  A unit that lies in
 // several CTAs leaves a partial state in each, and paged_merge_kernel joins them in order: results do not depend on timing.
 //
-// Measured, one token each of 64 sequences, 32 query and 8 K/V heads, pages of 16: bf16, 50 to 8 192 keys, 1.15 GB: 192 us,
-// 6.0 TB/s (a plain copy: 6.5); e4m3, 100 to 16 384 keys, 1.04 GB: 183 us, 5.7 TB/s.  What is left of the difference is the start
-// (lengths, page numbers, first rows: a chain of loads) and the merge, some 4 us each, and unequal ends.
+// Measured among other calls, one token each of 64 sequences, 32 query and 8 K/V heads, pages of 16: bf16, 50 to 8 192 keys,
+// 1.15 GB: 187-195 us, 5.9-6.1 TB/s (a plain copy: 6.5); e4m3, 100 to 16 384 keys, 1.04 GB: 185-199 us, 5.2-5.6 TB/s.  What is left
+// of the difference is the start (lengths, page numbers, first rows: a chain of loads) and the merge, some 4 us each, and unequal
+// ends.
 #include "attn_paged.cuh"
 
 namespace mb {

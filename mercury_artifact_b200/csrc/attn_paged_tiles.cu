@@ -13,8 +13,9 @@
 //            last box that lie behind the end are cleared before the values are used (hidden scores are replaced anyway).
 //            Lanes issue one after the other, some 55 cycles a box, so that two warps share them, and four where boxes
 //            have fewer than 64 slots (kSmallBoxes; 512 threads, whose softmax warps have fewer registers).
-//            2 048 tokens against 32 768 keys, 32/8 heads, with two warps and with four (attn_fwd over contiguous
-//            keys: 808): pages of 64 840 and 858 us, of 32 960 and 844, of 16 1 120 and 965, of 8 1 347 and 1 110.
+//            2 048 tokens against 32 768 keys, 32/8 heads, with two warps and with four, in a short burst (attn_fwd over
+//            contiguous keys: 808; under the power limit 947, pages of 64): pages of 64 840 and 858 us, of 32 960 and 844, of
+//            16 1 120 and 965, of 8 1 347 and 1 110.
 //   kRows    bf16, other pages: four more warps gather row by row with cp.async, 16 bytes a piece, straight into the
 //            swizzled layout that tcgen05 reads: the same with pages of 17 takes 1 094 us.
 // Codes (e4m3) are brought into bf16 before, into a buffer where every sequence is one page (launch_read_e4m3): 820 us for the

@@ -220,7 +220,9 @@ def attn_fwd_paged(
     q: bfloat16 [batch, n, hq, 128], or [tokens, hq, 128] with cu_seqlens; hq a multiple of the cache's heads.
     causal: new token i of n sees keys j <= seq_lens[b] - n + i (the last one sees all); causal=False: every key, as in
     cross attention to states of another length.  max_queries, max_keys: upper bounds on a sequence's new tokens
-    (with cu_seqlens; default: all tokens) and keys (default: what the page table covers), by which the launch is cut.
+    (with cu_seqlens; default: all tokens) and keys (default: what the page table covers), by which the launch is cut, and
+    scratch: where a float8_e4m3fn sequence may have more than 32 rows (new tokens x heads of a group), sequences of many rows
+    are computed from a bfloat16 copy, 512 bytes per key and K/V head of max_keys, as many at once as take 1 GiB, or one.
     Returns (o like q, lse fp32 [batch, hq, n] or [hq, tokens]).  A row that sees no key gets o = 0, lse = -inf;
     rows behind the last sequence are left as they are.  out must not overlap q.
 
