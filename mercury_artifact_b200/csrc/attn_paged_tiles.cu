@@ -698,8 +698,10 @@ int launch_paged_tiles(const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   maps.box = 1;
   maps.pages = c.pages;
   while (maps.box < kBN && c.page_size % (2 * maps.box) == 0) maps.box *= 2;
-  // (rows of the swizzled layout go in groups of 8; without a page or a key there is nothing to map, and nothing to fetch)
-  if (maps.box < 8 || a.max_keys == 0) return launch_tiles<kRows>(maps, a, ctas, stream);
+  // (rows of the swizzled layout go in groups of 8; without a page or a key there is nothing to map, and nothing to fetch; a map
+  // has no dimension whose entries are one, like heads that a view repeats)
+  const bool repeats = c.head_sb == 0 || c.slot_sb == 0 || c.page_sb == 0;
+  if (maps.box < 8 || a.max_keys == 0 || repeats) return launch_tiles<kRows>(maps, a, ctas, stream);
   if (!page_map(&maps.k, c.k, c.hkv, c.page_size, c.pages, c.head_sb, c.slot_sb, c.page_sb, maps.box) ||
       !page_map(&maps.v, c.v, c.hkv, c.page_size, c.pages, c.head_sb, c.slot_sb, c.page_sb, maps.box))
     return MB_E_TENSORMAP;

@@ -116,3 +116,24 @@ def test_chunks_of_a_quantised_cache_in_groups(causal, lens, new, covered):
     for o, lse in results:
         check(batch, o, lse, want)
     assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+
+
+@pytest.mark.parametrize("fp8", FP8)
+@pytest.mark.parametrize("new", [1, 40, 300])
+def test_cache_whose_heads_are_one(fp8, new):
+    """A view that repeats one head: read, and attended to by few and by many rows, like its copy."""
+    import mercury_artifact_b200 as mb
+
+    batch = Batch([500, 300], [new, new], (8, 2), 16, fp8, ragged=False, seed=45)
+    for kv in batch.kv:
+        kv[:, :, 1] = kv[:, :, 0]
+    k, v, ks, vs = batch.cache_tensors()
+    want = batch.expected((k, v, ks, vs), True)
+    one = torch.stack([k.view(torch.uint8), v.view(torch.uint8)])[:, :, :, :1].contiguous().cuda().view(k.dtype)
+    cache = mb.PagedKV(one[0].expand(-1, -1, 2, -1), one[1].expand(-1, -1, 2, -1), batch.on(ks), batch.on(vs))
+    assert cache.k.stride(2) == 0
+    o, lse = attend(batch, cache, new)
+    cache.check()
+    check(batch, o, lse, want)
+    kv = mb.kv_cache_read(cache, batch.on(batch.table), batch.on(batch.seq_lens), max_keys=300)
+    assert torch.equal(kv[:, 1, :, 0], kv[:, 1, :, 1]) and not torch.isnan(kv).any()
